@@ -334,7 +334,7 @@ def _run_own(state):
             h["cache"] = A.KvCache(state["pages"], state["table"], case["page"], case["kv_heads"], case["dim"], case["cache"])
             h["batch"] = A.KvBatch(state["offsets"], state["lengths"], _row_count(case))
         if case["kind"] == "attend":
-            h["scratch"] = A.tree_attention_scratch(h["cache"], case["q_heads"], case["dtype"], "cuda")
+            h["scratch"] = A.tree_attention_scratch("cuda")
     h = state["handles"]
     if case["kind"] == "turn":
         A.qk_norm_rope(h["turn"], state["q"], state["k"], state["positions"], state["q_out"], state["k_out"], state["error"])
