@@ -43,6 +43,7 @@ extern "C" {
 
 /* GGUF tensor type ids (gguf.cpp:21-32). */
 #define TSP_TYPE_F32 0u
+#define TSP_TYPE_F16 1u    /* key / value cache only */
 #define TSP_TYPE_Q5_1 7u   /* decode-size kernels only, GGUF layout (the reference model's down tensors) */
 #define TSP_TYPE_Q8_0 8u
 #define TSP_TYPE_Q4_K 12u
@@ -246,6 +247,108 @@ int tsp_residual_read(const float* d_normalized, const float* d_scores, const fl
                       uint32_t tokens, float* d_output, float* d_scales, uint32_t* d_error, void* stream);
 int tsp_residual_write(const float* d_streams, const float* d_output, const float* d_scales, uint32_t branches, uint32_t channels,
                        uint32_t tokens, float* d_destination, uint32_t* d_error, void* stream);
+
+/* ---- attention of a verify / decode step ----------------------------------------------------------------
+ * No reference counterpart at this boundary (its attention layers are composed inside the engine): the operators that stand before
+ * the FFN sub-layer of the same rows, for hosts that keep the whole layer on the GPU. A step's rows are described once
+ * (tsp_kv_batch) and go through tsp_qk_norm_rope_append -> tsp_tree_attention; after the verify tsp_kv_cache_keep compacts the
+ * accepted path. dtype arguments: 0 = FP32 rows, 1 = binary16 rows. A row holds its heads densely ([heads][head_dim]); rows are a
+ * byte stride apart (a multiple of 16), so that q, k and v may be parts of one fused row. head_dim 64, 128 or 256.
+ *
+ * Paged key / value cache. Token slot i of sequence s lies in page d_page_table[s * table_stride + i / page_tokens]; pages are
+ * page_stride_bytes apart (a multiple of 16, >= tsp_kv_page_bytes). Inside a page (what tsp_kv_cache_append writes and
+ * tsp_kv_cache_read gives back; a page may be copied or stored as it is):
+ *   [kv_head][group of 16 slots][K values | K scales | V values | V scales]
+ *   Q8_0: one byte a value, code + 128, and a binary16 scale per 32 dims; K values [64 dims][slot 16][64], the 64 as four times (8 of
+ *         the first 32 dims, 8 of the second); V values [32 dims][g 8][t 4][i 4][e 4] = dim 8i + g of slot 2t + (e & 1) + 8(e >> 1);
+ *         scales [32 dims][slot 16].
+ *   F16:  K values [32 dims][slot 16][32]; V values [32 dims][m 2][g 8][t 4][i 2][e 4] = dim 8(2m + i) + g of that slot; no scales.
+ * Slots that no call has written may hold anything. */
+#define TSP_KV_MAX_SEQUENCES 1024u
+#define TSP_KV_MAX_DRAFT 64u
+typedef struct tsp_kv_cache {
+    void* d_pages;                 /* 16-byte aligned */
+    uint64_t page_stride_bytes;
+    const uint32_t* d_page_table;  /* [sequences x table_stride]; entries behind a sequence's last slot are not read */
+    uint32_t table_stride;         /* words between two sequences' entries = pages that a sequence can have */
+    uint32_t pages;                /* pages at d_pages; an entry >= pages is TSP_ERR_INDEX */
+    uint32_t page_tokens;          /* 16, 32, 64, 128 or 256 */
+    uint32_t kv_heads, head_dim;
+    uint32_t type;                 /* TSP_TYPE_Q8_0 or TSP_TYPE_F16 */
+} tsp_kv_cache;
+uint64_t tsp_kv_page_bytes(uint32_t type, uint32_t page_tokens, uint32_t kv_heads, uint32_t head_dim);   /* 0 when unsupported */
+
+/* The rows of one step. Row r of the buffers, d_row_offsets[s] <= r < d_row_offsets[s + 1], is token r - d_row_offsets[s] of sequence s and
+ * has slot d_lengths[s] + r - d_row_offsets[s] of the cache. Both arrays are read on the device, so a captured graph follows them.
+ * Rows from d_row_offsets[sequences] on (a padded batch) are neither read nor written. Offsets that descend or pass `rows`, slots
+ * that the page table does not hold and page entries >= pages raise TSP_ERR_INDEX and leave out what they concern. */
+typedef struct tsp_kv_batch {
+    const uint32_t* d_row_offsets;   /* [sequences + 1], ascending from 0 */
+    const uint32_t* d_lengths;       /* [sequences]: slots of the sequence in the cache before this step */
+    uint32_t sequences;              /* 1 .. TSP_KV_MAX_SEQUENCES */
+    uint32_t rows;                   /* rows that the buffers hold, 1 .. 2^20 */
+} tsp_kv_batch;
+
+/* Norm of every head of the query and key rows, and rotation by the row's position, in one pass:
+ *   y_i = w_i x_i / sqrt(mean_j x_j^2 + eps)    (q_norm / k_norm NULL: y = x)
+ *   the pair (u, v) of index p < rotary_dim / 2 turns by a = position * inv_freq[p] (the product taken and reduced in 64 bits):
+ *   (u, v) -> magnitude (u cos a - v sin a, v cos a + u sin a);
+ *   pairs are (p, p + rotary_dim/2) (TSP_ROPE_HALVES) or (2p, 2p + 1) (TSP_ROPE_PAIRS) of the head's first rotary_dim dims; the others pass.
+ * Sums and rotation in FP32. q_heads or kv_heads may be 0 (those rows are then not touched). Outputs may be the input rows themselves
+ * (the same address, stride and dtype). A head whose result is not finite is written as zeros and raises TSP_ERR_NONFINITE. */
+#define TSP_ROPE_HALVES 0u
+#define TSP_ROPE_PAIRS 1u
+typedef struct tsp_qk_norm_rope_args {
+    const float* d_q_norm;       /* [head_dim] or NULL */
+    const float* d_k_norm;
+    const float* d_inv_freq;     /* [rotary_dim / 2]; may be NULL when rotary_dim is 0 */
+    uint32_t head_dim, rotary_dim;   /* rotary_dim a multiple of 8, <= head_dim */
+    uint32_t style;              /* TSP_ROPE_* */
+    float eps, magnitude;        /* eps >= 0 */
+} tsp_qk_norm_rope_args;
+int tsp_qk_norm_rope(const tsp_qk_norm_rope_args* a, const void* d_q, uint64_t q_stride_bytes, const void* d_k, uint64_t k_stride_bytes, uint32_t in_dtype,
+                     const uint32_t* d_positions, uint32_t rows, uint32_t q_heads, uint32_t kv_heads, void* d_q_out, uint64_t q_out_stride_bytes,
+                     void* d_k_out, uint64_t k_out_stride_bytes, uint32_t out_dtype, uint32_t* d_error, void* stream);
+
+/* K and V rows into the cache slots of the batch, quantised as they are written. Q8_0: per 32 dims d = binary16(max|x| / 127), code =
+ * x / d rounded half to even (of the exact quotient) within +-127; F16: rounded to nearest even. A head whose values are not finite, or
+ * whose scales or binary16 values would not be, is written as zeros and raises TSP_ERR_NONFINITE. No two rows of a step may have the
+ * same slot. tsp_qk_norm_rope_append is tsp_qk_norm_rope whose key rows go into the cache beside the value rows, in one launch (the
+ * key head is computed in 64 bits before it is quantised); d_positions as there, per row. */
+int tsp_kv_cache_append(const tsp_kv_cache* cache, const tsp_kv_batch* batch, const void* d_k, uint64_t k_stride_bytes, const void* d_v,
+                        uint64_t v_stride_bytes, uint32_t dtype, uint32_t* d_error, void* stream);
+int tsp_qk_norm_rope_append(const tsp_qk_norm_rope_args* a, const tsp_kv_cache* cache, const tsp_kv_batch* batch, const void* d_q, uint64_t q_stride_bytes,
+                            const void* d_k, uint64_t k_stride_bytes, const void* d_v, uint64_t v_stride_bytes, uint32_t in_dtype, const uint32_t* d_positions,
+                            uint32_t q_heads, void* d_q_out, uint64_t q_out_stride_bytes, uint32_t out_dtype, uint32_t* d_error, void* stream);
+
+/* The slots of the batch back as rows (code * d, rounded once for binary16): the inverse of an append with the same batch; lengths of
+ * zero and offsets over the sequences' sizes read whole sequences. d_k or d_v may be NULL (left out). */
+int tsp_kv_cache_read(const tsp_kv_cache* cache, const tsp_kv_batch* batch, void* d_k, uint64_t k_stride_bytes, void* d_v, uint64_t v_stride_bytes,
+                      uint32_t dtype, uint32_t* d_error, void* stream);
+
+/* After a verify: the accepted tokens of every sequence move to the front of its draft slots, slot d_lengths[s] + j <- slot d_lengths[s] +
+ * d_accepted[d_row_offsets[s] + j] for j < d_counts[s], bit for bit. The accepted indices of a sequence ascend strictly (a path of the tree from
+ * its root) and stay below the sequence's rows, at most TSP_KV_MAX_DRAFT of them; anything else raises TSP_ERR_INDEX and leaves that
+ * sequence as it was. Slots from d_lengths[s] + d_counts[s] on keep what they held. */
+int tsp_kv_cache_keep(const tsp_kv_cache* cache, const tsp_kv_batch* batch, const uint32_t* d_accepted, const uint32_t* d_counts, uint32_t* d_error,
+                      void* stream);
+
+/* Attention of the drafted tokens of every sequence over its cache: q_heads query heads, kv_heads key / value heads (q_heads a multiple of
+ * them, head h reads kv head h / (q_heads / kv_heads)).
+ *   out = sum_j softmax_j(scale * q.k_j) v_j   over the slots that the row sees: all slots below d_lengths[s], and slot d_lengths[s] + i of its own
+ *   step where bit i of d_tree_mask[row] is set (bits at and above the sequence's rows say nothing). d_tree_mask NULL: a chain, row i of a sequence sees
+ *   tokens 0..i of the step. A row that sees nothing gets zeros. One token per sequence is plain decode.
+ * The step's keys and values have to be in the cache (append first). max_rows: the most rows of a sequence in this batch, 1..TSP_KV_MAX_DRAFT; a
+ * sequence with more raises TSP_ERR_INDEX, as do slots or pages out of range: its rows are then zeros. Slots that a row does not see
+ * never reach its result, whatever they hold; a result that is not finite is written as zeros for that head and raises TSP_ERR_NONFINITE.
+ * q and out rows have one dtype. FP32 rows are computed with FP32 accuracy (products of exact parts, FP32 sums); binary16 rows with
+ * binary16 products and FP32 sums.
+ * d_scratch: tsp_tree_attention_scratch_bytes() (for the current device), 16-byte aligned, zero before its first use; every call leaves what the next one needs.
+ * Calls that share it must be ordered (one stream, or events between): two that overlap need a scratch each. */
+uint64_t tsp_tree_attention_scratch_bytes(void);
+int tsp_tree_attention(const tsp_kv_cache* cache, const tsp_kv_batch* batch, const void* d_q, uint64_t q_stride_bytes, const uint64_t* d_tree_mask,
+                       uint32_t q_heads, uint32_t max_rows, float scale, void* d_out, uint64_t out_stride_bytes, uint32_t dtype, void* d_scratch,
+                       uint64_t scratch_bytes, uint32_t* d_error, void* stream);
 
 /* ---- data preparation (device side) ----------------------------------------------------------------
  * tsp_synth_weights: seeded N(0, sigma) values quantised to GGUF blocks of `type` (Q4_K, Q8_0) or written

@@ -13,12 +13,14 @@ from . import build as _build
 
 LIB_PATH = _build.LIB
 
-TYPE_F32, TYPE_Q8_0, TYPE_Q4_K = 0, 8, 12
+TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_Q4_K = 0, 1, 8, 12
 TYPE_Q5_1, TYPE_Q5_K = 7, 13
 LAYOUT_GGUF, LAYOUT_PLANAR = 0, 1
 ROUTER_SOFTMAX, ROUTER_SIGMOID = 0, 1
 ERR_NONFINITE, ERR_INDEX, ERR_TIMEOUT = 2, 4, 8
 GEMV_TILE = 8
+ROPE_HALVES, ROPE_PAIRS = 0, 1
+KV_MAX_SEQUENCES, KV_MAX_DRAFT = 1024, 64
 E_ARG, E_TYPE, E_CUDA, E_DEVICE = -1, -2, -3, -4
 
 
@@ -56,9 +58,24 @@ class MoeWeights(C.Structure):
                 ("shared_up", MatrixSet), ("shared_down", MatrixSet), ("d_shared_router", C.c_void_p)]
 
 
+class KvCache(C.Structure):
+    _fields_ = [("d_pages", C.c_void_p), ("page_stride_bytes", C.c_uint64), ("d_page_table", C.c_void_p), ("table_stride", C.c_uint32), ("pages", C.c_uint32),
+                ("page_tokens", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("type", C.c_uint32)]
+
+
+class KvBatch(C.Structure):
+    _fields_ = [("d_row_offsets", C.c_void_p), ("d_lengths", C.c_void_p), ("sequences", C.c_uint32), ("rows", C.c_uint32)]
+
+
+class QkNormRope(C.Structure):
+    _fields_ = [("d_q_norm", C.c_void_p), ("d_k_norm", C.c_void_p), ("d_inv_freq", C.c_void_p), ("head_dim", C.c_uint32), ("rotary_dim", C.c_uint32),
+                ("style", C.c_uint32), ("eps", C.c_float), ("magnitude", C.c_float)]
+
+
 # name -> (restype, argtypes); the list is also what the symbol-export test checks against the header
 _vp, _u32, _u64, _i = C.c_void_p, C.c_uint32, C.c_uint64, C.c_int
 _MS = C.POINTER(MatrixSet)
+_KV, _KB, _QK = C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(QkNormRope)
 SIGNATURES = {
     "tsp_last_error": (C.c_char_p, []),
     "tsp_device_info": (_i, [C.POINTER(_i), C.POINTER(_i), C.POINTER(_i)]),
@@ -85,6 +102,14 @@ SIGNATURES = {
     "tsp_router_margin_evaluate": (_i, [_vp, _u32, C.c_float, _vp, C.POINTER(RouterMarginTelemetry), C.POINTER(_i)]),
     "tsp_residual_read": (_i, [_vp, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _vp, _vp]),
     "tsp_residual_write": (_i, [_vp, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _vp]),
+    "tsp_kv_page_bytes": (_u64, [_u32, _u32, _u32, _u32]),
+    "tsp_qk_norm_rope": (_i, [_QK, _vp, _u64, _vp, _u64, _u32, _vp, _u32, _u32, _u32, _vp, _u64, _vp, _u64, _u32, _vp, _vp]),
+    "tsp_kv_cache_append": (_i, [_KV, _KB, _vp, _u64, _vp, _u64, _u32, _vp, _vp]),
+    "tsp_qk_norm_rope_append": (_i, [_QK, _KV, _KB, _vp, _u64, _vp, _u64, _vp, _u64, _u32, _vp, _u32, _vp, _u64, _u32, _vp, _vp]),
+    "tsp_kv_cache_read": (_i, [_KV, _KB, _vp, _u64, _vp, _u64, _u32, _vp, _vp]),
+    "tsp_kv_cache_keep": (_i, [_KV, _KB, _vp, _vp, _vp, _vp]),
+    "tsp_tree_attention_scratch_bytes": (_u64, []),
+    "tsp_tree_attention": (_i, [_KV, _KB, _vp, _u64, _vp, _u32, _u32, C.c_float, _vp, _u64, _u32, _vp, _u64, _vp, _vp]),
     "tsp_rows_f16_to_f32": (_i, [_vp, _u64, _vp, _u64, _u32, _u32, _vp]),
     "tsp_moe_layer_decode": (_i, [C.POINTER(MoeWeights), C.POINTER(MoeScratch), _vp, _u64, _u32, _vp, _u64, _u32, _u32, _u32,
                                   _u32, _u32, _u32, _i, _vp, _u64, _u32, _vp, _vp]),
