@@ -349,7 +349,7 @@ int launch_cache_read(const tsp_kv_cache& cache, const tsp_kv_batch& batch, void
 int launch_cache_keep(const tsp_kv_cache& cache, const tsp_kv_batch& batch, const uint32_t* accepted, const uint32_t* counts, uint32_t* error, cudaStream_t st) {
     const bool q8 = cache.type == TSP_TYPE_Q8_0;
     const size_t smem = TSP_KV_MAX_DRAFT * (q8 ? 2 * (cache.head_dim + cache.head_dim / 16) : 4 * cache.head_dim);
-    static SmemAttrCache attr;
+    static thread_local SmemAttrCache attr;
     TSP_CUDA(ensure_dynamic_smem(cache_keep_kernel, attr, smem));
     TSP_CUDA(launch_pdl(cache_keep_kernel, dim3(batch.sequences, cache.kv_heads), dim3(256), smem, st, cache, batch, accepted, counts, error));
     return TSP_OK;
