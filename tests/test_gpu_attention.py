@@ -439,6 +439,18 @@ def test_large_scores_and_large_values():
                     assert (np.abs(got[j] - want) <= tol).all(), (dtype, type_, at)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("group", [2, 16])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-12])
+def test_scales_of_zero_below_zero_and_close_to_it(dtype, group, scale):
+    s = Step(13, "q8_0", 128, 16, 2, group, [3, 2], [37, 0], dtype, True)
+    s.mask[1] = 0
+    s.scale = scale
+    out, err = s.run()
+    assert err == 0
+    s.check(out)
+
+
 def test_sequences_out_of_range_are_zeros_and_leave_the_others():
     s = Step(9, "q8_0", 128, 16, 2, 4, [3, 9, 4, 2], [50, 20, 70, 8], "f16", False)
     out, err = s.run(most=8)                           # sequence 1 has more rows than the call says

@@ -213,7 +213,7 @@ tree_attention_kernel(const AttnParams p) {
         const uint32_t mine = static_cast<uint32_t>(b - a);
         uint64_t src = 0;              // lane i: source of unit i of the 32 that `issued` is in
         uint32_t issued = 0, gone = 0; // bit st: the unit in stage st has no page
-        auto issue = [&]() {
+        auto issue = [&](uint32_t st) {
             if (issued >= mine) return;
             if (issued % 32 == 0) {
                 src = 0;
@@ -223,7 +223,6 @@ tree_attention_kernel(const AttnParams p) {
                     if (!x.dead) src = reinterpret_cast<uint64_t>(kv_group(p.cache, x.seq, (u - x.start) * kKvGroup, x.head, p.error));
                 }
             }
-            const uint32_t st = issued % P;
             const uint64_t from = __shfl_sync(NONE, src, issued % 32);
             gone = (gone & ~(1u << st)) | (from ? 0u : 1u << st);
             if (elect_one()) {
@@ -233,7 +232,8 @@ tree_attention_kernel(const AttnParams p) {
             __syncwarp();
             ++issued;
         };
-        for (uint32_t i = 0; i < P; ++i) issue();
+        for (uint32_t i = 0; i < P; ++i) issue(i);
+        uint32_t stage = 0, phase = 0;
 
         bool lost = false;   // a wait has run out
         for (uint32_t done = 0; done < mine;) {
@@ -243,14 +243,13 @@ tree_attention_kernel(const AttnParams p) {
             uint32_t qf[F16 ? 1 : 2][D / 16][QR];
             float fa, fb;
             [[maybe_unused]] float start[NB][2];   // Q8_0, binary16 rows: -1152 times the sum of the row's 32 dims
-            uint64_t wa, wb;
+            auto row_of = [&](uint32_t r, uint32_t& node, uint32_t& head) {
+                const uint32_t flat = it.tile * R + r;
+                node = flat / p.group;
+                head = it.head * p.group + flat % p.group;
+            };
             {
-                const float f = fabsf(p.scale) * 1.4426950408889634f;
-                auto row_of = [&](uint32_t r, uint32_t& node, uint32_t& head) {
-                    const uint32_t flat = it.tile * R + r;
-                    node = flat / p.group;
-                    head = it.head * p.group + flat % p.group;
-                };
+                const float f = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-25f);   // not 0: it multiplies minus infinity
                 fa = fb = f;
                 // Q rows of the fragments: g (and g + 8)
 #pragma unroll
@@ -282,7 +281,7 @@ tree_attention_kernel(const AttnParams p) {
                         top = fmaxf(top, __shfl_xor_sync(NONE, top, 1));
                         top = fmaxf(top, __shfl_xor_sync(NONE, top, 2));
                         const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-                        const int shift = top > 0.f && e < 128 ? max(-100, min(100, 14 - e)) : 0;
+                        const int shift = top > 0.f && e < 128 ? max(-115, min(40, 14 - e)) : 0;
                         const float up = __uint_as_float(static_cast<uint32_t>(shift + 127) << 23) * (p.scale < 0.f ? -1.f : 1.f);
                         const float down = f * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);   // of row g (+ 8)
                         if constexpr (R == 8) { fa = __shfl_sync(NONE, down, 8 * t); fb = __shfl_sync(NONE, down, 8 * t + 4); }
@@ -324,11 +323,6 @@ tree_attention_kernel(const AttnParams p) {
                         else { start[k][0] = sum[0]; start[k][1] = sum[R / 8 - 1]; }
                     }
                 }
-                uint32_t node, head;
-                row_of(ra, node, head);
-                wa = ra >= it.rows ? 0 : p.mask ? p.mask[it.row0 + node] : ~0ull >> (63 - min(node, 63u));
-                row_of(rb, node, head);
-                wb = rb >= it.rows ? 0 : p.mask ? p.mask[it.row0 + node] : ~0ull >> (63 - min(node, 63u));
             }
 
             // R = 16: [32 dims][n tile][c]: rows g, g + 8; dims 32 b + 8 i + 2 t, + 1. R = 8: [32 dims][m tile][c]: dims 32 b + 16 i + g, + 8; rows 2 t, + 1
@@ -339,230 +333,244 @@ tree_attention_kernel(const AttnParams p) {
                 for (uint32_t i = 0; i < NI; ++i)
 #pragma unroll
                     for (uint32_t c = 0; c < 4; ++c) o[k][i][c] = 0.f;
-            // A row's weight is 2^(score - ref), ref = m - lift: m, the score that was largest when the reference last moved; lift, Q8_0: the power of two that
-            // keeps weights times value scales below 2^15 (it only falls), else kUp
+            // A row's weight is 2^(score + ref), ref = lift - m: m, the score that was largest when the reference last moved; lift, Q8_0: the power of two
+            // that keeps weights times value scales below 2^15 (it only falls), else kUp
             float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f, lift = Q8 ? 20.f : kUp;
+            float ref_a = 0.f, ref_b = 0.f, limit_a = -INFINITY, limit_b = -INFINITY, limit_v = Q8 ? 0x1p-13f : INFINITY;
             bool dead = false;
 
-            for (; done < stop; ++done) {
-                const uint32_t st = done % P;
-                const uint64_t slot0 = (a + done - it.start) * kKvGroup;
-                if (!lost) lost = !__all_sync(NONE, mbar_wait(&sm.full[warp][st], (done / P) & 1));
-                if (lost) {
-                    if (!dead && lane == 0) raise_error(p.error, TSP_ERR_TIMEOUT);
-                    dead = true;
-                    continue;
-                }
-                if (gone >> st & 1) dead = true;
-                else {
-                    const bool edge = slot0 + kKvGroup > it.length;
-                    const uint8_t* keys = sm.ring[warp] + st * S::kGroupBytes;
-                    const uint8_t* values = keys + S::kHalf;
-                    float s[NS];
+            // One unit; EDGE: it reaches past the context
+            auto unit = [&](auto edge_tag, const uint8_t* keys) {
+                constexpr bool EDGE = decltype(edge_tag)::value;
+                const uint8_t* values = keys + S::kHalf;
+                float s[NS];
 #pragma unroll
-                    for (uint32_t i = 0; i < NS; ++i) s[i] = 0.f;
+                for (uint32_t i = 0; i < NS; ++i) s[i] = 0.f;
 #pragma unroll
-                    for (uint32_t b0 = 0; b0 < NB; b0 += Q8 ? 2 : 1) {
-                        uint4 w[2];   // 16 bytes of slots g and g + 8
+                for (uint32_t b0 = 0; b0 < NB; b0 += Q8 ? 2 : 1) {
+                    uint4 w[2];   // 16 bytes of slots g and g + 8
 #pragma unroll
-                        for (uint32_t n = 0; n < 2; ++n) w[n] = *reinterpret_cast<const uint4*>(keys + ((Q8 ? b0 / 2 : b0) * kKvGroup + 8 * n + g) * 64 + t * 16);
+                    for (uint32_t n = 0; n < 2; ++n) w[n] = *reinterpret_cast<const uint4*>(keys + ((Q8 ? b0 / 2 : b0) * kKvGroup + 8 * n + g) * 64 + t * 16);
 #pragma unroll
-                        for (uint32_t k = b0; k < b0 + (Q8 ? 2 : 1); ++k) {   // 32 dims: two steps under one scale
-                            uint32_t kb[2][4];
+                    for (uint32_t k = b0; k < b0 + (Q8 ? 2 : 1); ++k) {   // 32 dims: two steps under one scale
+                        uint32_t kb[2][4];
 #pragma unroll
-                            for (uint32_t n = 0; n < 2; ++n) {
-                                if constexpr (Q8) {
-                                    const uint32_t x = k & 1 ? w[n].z : w[n].x, y = k & 1 ? w[n].w : w[n].y;
-                                    if constexpr (F16) { biased_halves(x, kb[n][0], kb[n][1]); biased_halves(y, kb[n][2], kb[n][3]); }
-                                    else { codes_to_halves(x, kb[n][0], kb[n][1]); codes_to_halves(y, kb[n][2], kb[n][3]); }
-                                } else { kb[n][0] = w[n].x; kb[n][1] = w[n].y; kb[n][2] = w[n].z; kb[n][3] = w[n].w; }
-                            }
-                            float acc[NS / 4][4];
-#pragma unroll
-                            for (uint32_t n = 0; n < NS / 4; ++n)
-#pragma unroll
-                                for (uint32_t h = 0; h < 2; ++h)
-#pragma unroll
-                                    for (uint32_t part = 0; part < (F16 ? 1 : 2); ++part) {
-                                        const uint32_t (&q)[QR] = qf[part][2 * k + h];
-                                        const bool fresh = h == 0 && part == 0;
-                                        float c0 = 0.f, c1 = 0.f, c2 = 0.f, c3 = 0.f;
-                                        if constexpr (Q8 && F16) { c0 = start[k][0]; c1 = start[k][R == 8]; c2 = start[k][R != 8]; c3 = start[k][1]; }
-                                        if constexpr (R == 8) {
-                                            if (fresh) mma_f16_16816_from(acc[n], kb[0][0], kb[1][0], kb[0][1], kb[1][1], q[0], q[1], c0, c1, c2, c3);
-                                            else mma_f16_16816(acc[n], kb[0][2 * h], kb[1][2 * h], kb[0][2 * h + 1], kb[1][2 * h + 1], q[0], q[1]);
-                                        } else {
-                                            if (fresh) mma_f16_16816_from(acc[n], q[0], q[1], q[2 % QR], q[3 % QR], kb[n][0], kb[n][1], c0, c1, c2, c3);
-                                            else mma_f16_16816(acc[n], q[0], q[1], q[2 % QR], q[3 % QR], kb[n][2 * h], kb[n][2 * h + 1]);
-                                        }
-                                    }
+                        for (uint32_t n = 0; n < 2; ++n) {
                             if constexpr (Q8) {
-                                const uint8_t* scales = keys + kKvGroup * D + k * kKvGroup * 2;
-                                if constexpr (R == 8) {
-                                    const float d0 = __half2float(*reinterpret_cast<const __half*>(scales + g * 2)), d1 = __half2float(*reinterpret_cast<const __half*>(scales + g * 2 + 16));
-                                    s[0] = fmaf(acc[0][0], d0, s[0]); s[1] = fmaf(acc[0][1], d0, s[1]);
-                                    s[2] = fmaf(acc[0][2], d1, s[2]); s[3] = fmaf(acc[0][3], d1, s[3]);
-                                } else {
+                                const uint32_t x = k & 1 ? w[n].z : w[n].x, y = k & 1 ? w[n].w : w[n].y;
+                                if constexpr (F16) { biased_halves(x, kb[n][0], kb[n][1]); biased_halves(y, kb[n][2], kb[n][3]); }
+                                else { codes_to_halves(x, kb[n][0], kb[n][1]); codes_to_halves(y, kb[n][2], kb[n][3]); }
+                            } else { kb[n][0] = w[n].x; kb[n][1] = w[n].y; kb[n][2] = w[n].z; kb[n][3] = w[n].w; }
+                        }
+                        float acc[NS / 4][4];
 #pragma unroll
-                                    for (uint32_t n = 0; n < NS / 4; ++n) {
-                                        const float2 d = __half22float2(*reinterpret_cast<const __half2*>(scales + (8 * n + 2 * t) * 2));
+                        for (uint32_t n = 0; n < NS / 4; ++n)
 #pragma unroll
-                                        for (uint32_t c = 0; c < 4; ++c) s[4 * n + c] = fmaf(acc[n][c], c & 1 ? d.y : d.x, s[4 * n + c]);
+                            for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                                for (uint32_t part = 0; part < (F16 ? 1 : 2); ++part) {
+                                    const uint32_t (&q)[QR] = qf[part][2 * k + h];
+                                    const bool fresh = h == 0 && part == 0;
+                                    float c0 = 0.f, c1 = 0.f, c2 = 0.f, c3 = 0.f;
+                                    if constexpr (Q8 && F16) { c0 = start[k][0]; c1 = start[k][R == 8]; c2 = start[k][R != 8]; c3 = start[k][1]; }
+                                    if constexpr (R == 8) {
+                                        if (fresh) mma_f16_16816_from(acc[n], kb[0][0], kb[1][0], kb[0][1], kb[1][1], q[0], q[1], c0, c1, c2, c3);
+                                        else mma_f16_16816(acc[n], kb[0][2 * h], kb[1][2 * h], kb[0][2 * h + 1], kb[1][2 * h + 1], q[0], q[1]);
+                                    } else {
+                                        if (fresh) mma_f16_16816_from(acc[n], q[0], q[1], q[2 % QR], q[3 % QR], kb[n][0], kb[n][1], c0, c1, c2, c3);
+                                        else mma_f16_16816(acc[n], q[0], q[1], q[2 % QR], q[3 % QR], kb[n][2 * h], kb[n][2 * h + 1]);
                                     }
                                 }
-                            } else {
-#pragma unroll
-                                for (uint32_t i = 0; i < NS; ++i) s[i] += acc[i / 4][i % 4];
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (uint32_t i = 0; i < NS; ++i) s[i] *= second(i) ? fb : fa;
-                    // At the end of the context: what a row does not see gets no weight. Drafted slots whose values are not finite give the rows that see
-                    // them NaN through the weight, and count as zero themselves; slots behind the last count as zero, whatever they hold.
-                    uint32_t drop = 0;   // bit i: slot i of the unit
-                    if (edge) {
-                        uint32_t odd = 0;
-                        const uint32_t there = it.total - slot0 >= kKvGroup ? 0xffffu : (1u << static_cast<uint32_t>(it.total - slot0)) - 1;
-                        const uint32_t drafted = slot0 >= it.length ? 0xffffu : 0xffffu << static_cast<uint32_t>(it.length - slot0);
                         if constexpr (Q8) {
-                            for (uint32_t i = lane; i < NB * kKvGroup; i += 32)
-                                odd |= static_cast<uint32_t>(odd_half(*reinterpret_cast<const uint16_t*>(values + kKvGroup * D + i * 2))) << i % kKvGroup;
-                        } else {
-                            for (uint32_t i = 0; i < D / 8; ++i)   // 16 dims, half of them: eight bytes of four slots a lane
-#pragma unroll
-                                for (uint32_t e = 0; e < 4; ++e)
-                                    odd |= static_cast<uint32_t>(odd_half(*reinterpret_cast<const uint16_t*>(values + (i / 2 * 32 + lane) * 16 + i % 2 * 8 + e * 2))) << (2 * t + (e & 1) + 8 * (e >> 1));
-                        }
-                        odd = __reduce_or_sync(NONE, odd) & drafted & there;
-                        drop = odd | (~there & 0xffffu);
-#pragma unroll
-                        for (uint32_t i = 0; i < NS; ++i) {
-                            const uint32_t x = slot_in(i);
-                            const bool seen = there >> x & 1 && (!(drafted >> x & 1) || ((second(i) ? wb : wa) >> (slot0 + x - it.length) & 1));
-                            if (!seen) s[i] = -INFINITY;
-                            else if (odd >> x & 1) s[i] = NAN;
-                        }
-                    }
-                    float xa = -INFINITY, xb = -INFINITY;
-#pragma unroll
-                    for (uint32_t i = 0; i < NS; ++i) { if (second(i)) xb = fmaxf(xb, s[i]); else xa = fmaxf(xa, s[i]); }
-                    bool move = xa > ma + kSlack || xb > mb + kSlack;
-                    [[maybe_unused]] uint32_t exponent = 0;
-                    if constexpr (Q8) {   // largest value scale of the unit: the lanes have a part each. It is below 2^(exponent - 14)
-                        uint32_t top = 0;
-                        for (uint32_t i = lane; i < NB * kKvGroup / 2; i += 32) {
-                            uint32_t d = *reinterpret_cast<const uint32_t*>(values + kKvGroup * D + i * 4) & 0x7fff7fffu;
-                            if (edge) {
-                                const uint32_t out = drop >> (i * 2 % kKvGroup);
-                                if (out & 1) d &= 0xffff0000u;
-                                if (out & 2) d &= 0x0000ffffu;
-                            }
-                            top = max(top, max(d & 0xffffu, d >> 16));
-                        }
-                        exponent = min(max(top >> 10, 1u), 31u);
-                        move |= lift > 21.f - static_cast<float>(exponent);
-                    }
-                    if (__any_sync(NONE, move)) {
-#pragma unroll
-                        for (uint32_t x = R == 8 ? 4 : 1; x < (R == 8 ? 32 : 4); x *= 2) { xa = fmaxf(xa, __shfl_xor_sync(NONE, xa, x)); xb = fmaxf(xb, __shfl_xor_sync(NONE, xb, x)); }
-                        xa = fmaxf(xa, ma); xb = fmaxf(xb, mb);
-                        float fall = 0.f;
-                        if constexpr (Q8) {
-                            const float now = fminf(lift, 21.f - static_cast<float>(__reduce_max_sync(NONE, exponent)));
-                            fall = now - lift;
-                            lift = now;
-                        }
-                        const float r0 = ma == -INFINITY ? 0.f : exp2_approx(ma - xa + fall), r1 = mb == -INFINITY ? 0.f : exp2_approx(mb - xb + fall);
-                        la *= ma == -INFINITY ? 1.f : r0; lb *= mb == -INFINITY ? 1.f : r1;   // a NaN stays
-                        ma = xa; mb = xb;
-#pragma unroll
-                        for (uint32_t k = 0; k < NB; ++k)
-#pragma unroll
-                            for (uint32_t i = 0; i < NI; ++i)
-#pragma unroll
-                                for (uint32_t c = 0; c < 4; ++c) o[k][i][c] *= second(c) ? r1 : r0;
-                    }
-                    const float ba = ma == -INFINITY ? 0.f : ma - lift, bb = mb == -INFINITY ? 0.f : mb - lift;
-                    float pr[NS];
-#pragma unroll
-                    for (uint32_t i = 0; i < NS; ++i) {
-                        pr[i] = exp2_approx(s[i] - (second(i) ? bb : ba));
-                        if (second(i)) lb += pr[i]; else la += pr[i];
-                    }
-                    uint32_t keep[2] = {NONE, NONE};   // values of slots 2t, 2t + 1 and 8 more
-                    if (edge) {
-#pragma unroll
-                        for (uint32_t n = 0; n < 2; ++n)
-                            keep[n] = (drop >> (8 * n + 2 * t) & 1 ? 0u : 0x0000ffffu) | (drop >> (8 * n + 2 * t) & 2 ? 0u : 0xffff0000u);
-                    }
-                    uint32_t wf[QR], wl[QR];
-                    auto split = [&](const float (&w)[NS]) {   // R = 16: A fragment (rows g, g + 8; slots 2t.., 8 more); R = 8: B fragment, slots 2t.., 8 more, row g
-#pragma unroll
-                        for (uint32_t r = 0; r < QR; ++r) {
-                            wf[r] = h2_bits(__floats2half2_rn(w[2 * r], w[2 * r + 1]));
-                            if constexpr (!F16) wl[r] = pack_low(w[2 * r], w[2 * r + 1], wf[r]);
+                            const uint8_t* scales = keys + kKvGroup * D + k * kKvGroup * 2;
                             if constexpr (R == 8) {
-                                wf[r] = transposed(wf[r]);
-                                if constexpr (!F16) wl[r] = transposed(wl[r]);
-                            }
-                        }
-                    };
-                    if constexpr (!Q8) split(pr);
-#pragma unroll
-                    for (uint32_t k = 0; k < NB; ++k) {
-                        uint32_t vb[8];   // dims 8 i + g: slots 2t, 2t + 1 in vb[2 i], 8 further in vb[2 i + 1]
-                        if constexpr (Q8) {
-                            const uint4 w = *reinterpret_cast<const uint4*>(values + k * 512 + lane * 16);
-                            codes_to_halves(w.x, vb[0], vb[1]); codes_to_halves(w.y, vb[2], vb[3]);
-                            codes_to_halves(w.z, vb[4], vb[5]); codes_to_halves(w.w, vb[6], vb[7]);
-                            const uint8_t* scales = values + kKvGroup * D + k * kKvGroup * 2;
-                            float w4[NS];
-                            if constexpr (R == 8) {
-                                float d0 = __half2float(*reinterpret_cast<const __half*>(scales + g * 2)), d1 = __half2float(*reinterpret_cast<const __half*>(scales + g * 2 + 16));
-                                if (edge) { if (drop >> g & 1) d0 = 0.f; if (drop >> (g + 8) & 1) d1 = 0.f; }
-                                w4[0] = pr[0] * d0; w4[1] = pr[1] * d0; w4[2] = pr[2] * d1; w4[3] = pr[3] * d1;
+                                const float d0 = __half2float(*reinterpret_cast<const __half*>(scales + g * 2)), d1 = __half2float(*reinterpret_cast<const __half*>(scales + g * 2 + 16));
+                                s[0] = fmaf(acc[0][0], d0, s[0]); s[1] = fmaf(acc[0][1], d0, s[1]);
+                                s[2] = fmaf(acc[0][2], d1, s[2]); s[3] = fmaf(acc[0][3], d1, s[3]);
                             } else {
 #pragma unroll
                                 for (uint32_t n = 0; n < NS / 4; ++n) {
-                                    const float2 f = __half22float2(bits_h2(*reinterpret_cast<const uint32_t*>(scales + (8 * n + 2 * t) * 2) & keep[n]));
+                                    const float2 d = __half22float2(*reinterpret_cast<const __half2*>(scales + (8 * n + 2 * t) * 2));
 #pragma unroll
-                                    for (uint32_t c = 0; c < 4; ++c) w4[4 * n + c] = pr[4 * n + c] * (c & 1 ? f.y : f.x);
+                                    for (uint32_t c = 0; c < 4; ++c) s[4 * n + c] = fmaf(acc[n][c], c & 1 ? d.y : d.x, s[4 * n + c]);
                                 }
                             }
-                            split(w4);
                         } else {
-                            const uint4 w = *reinterpret_cast<const uint4*>(values + k * 1024 + lane * 16), x = *reinterpret_cast<const uint4*>(values + k * 1024 + 512 + lane * 16);
-                            vb[0] = w.x; vb[1] = w.y; vb[2] = w.z; vb[3] = w.w; vb[4] = x.x; vb[5] = x.y; vb[6] = x.z; vb[7] = x.w;
-                            if (edge) {
 #pragma unroll
-                                for (uint32_t i = 0; i < 8; ++i) vb[i] &= keep[i & 1];
-                            }
-                        }
-#pragma unroll
-                        for (uint32_t i = 0; i < NI; ++i) {
-                            auto product = [&](float (&acc)[4], const uint32_t (&w)[QR], bool fresh) {
-                                if constexpr (R == 8) {
-                                    if (fresh) mma_f16_16816_zero(acc, vb[4 * i % 8], vb[(4 * i + 2) % 8], vb[(4 * i + 1) % 8], vb[(4 * i + 3) % 8], w[0], w[1]);
-                                    else mma_f16_16816(acc, vb[4 * i % 8], vb[(4 * i + 2) % 8], vb[(4 * i + 1) % 8], vb[(4 * i + 3) % 8], w[0], w[1]);
-                                } else {
-                                    if (fresh) mma_f16_16816_zero(acc, w[0], w[1], w[2 % QR], w[3 % QR], vb[2 * i], vb[2 * i + 1]);
-                                    else mma_f16_16816(acc, w[0], w[1], w[2 % QR], w[3 % QR], vb[2 * i], vb[2 * i + 1]);
-                                }
-                            };
-                            if constexpr (F16) product(o[k][i], wf, false);
-                            else {   // the tensor core cuts its sums off: a chain of two products, added up rounded
-                                float acc[4];
-                                product(acc, wf, true);
-                                product(acc, wl, false);
-#pragma unroll
-                                for (uint32_t c = 0; c < 4; ++c) o[k][i][c] += acc[c];
-                            }
+                            for (uint32_t i = 0; i < NS; ++i) s[i] += acc[i / 4][i % 4];
                         }
                     }
                 }
+                // At the end of the context: what a row does not see gets no weight. Drafted slots whose values are not finite give the rows that see
+                // them NaN through the weight, and count as zero themselves; slots behind the last count as zero, whatever they hold.
+                uint32_t keep[2] = {NONE, NONE};   // values of slots 2t, 2t + 1 and 8 more
+                uint32_t drop = 0;                 // bit i: slot i of the unit
+                if constexpr (EDGE) {
+                    const uint64_t slot0 = (a + done - it.start) * kKvGroup;
+                    uint32_t odd = 0;
+                    const uint32_t there = it.total - slot0 >= kKvGroup ? 0xffffu : (1u << static_cast<uint32_t>(it.total - slot0)) - 1;
+                    const uint32_t drafted = slot0 >= it.length ? 0xffffu : 0xffffu << static_cast<uint32_t>(it.length - slot0);
+                    if constexpr (Q8) {
+                        for (uint32_t i = lane; i < NB * kKvGroup; i += 32)
+                            odd |= static_cast<uint32_t>(odd_half(*reinterpret_cast<const uint16_t*>(values + kKvGroup * D + i * 2))) << i % kKvGroup;
+                    } else {
+                        for (uint32_t i = 0; i < D / 8; ++i)   // 16 dims, half of them: eight bytes of four slots a lane
+#pragma unroll
+                            for (uint32_t e = 0; e < 4; ++e)
+                                odd |= static_cast<uint32_t>(odd_half(*reinterpret_cast<const uint16_t*>(values + (i / 2 * 32 + lane) * 16 + i % 2 * 8 + e * 2))) << (2 * t + (e & 1) + 8 * (e >> 1));
+                    }
+                    odd = __reduce_or_sync(NONE, odd) & drafted & there;
+                    drop = odd | (~there & 0xffffu);
+                    uint64_t wa, wb;
+                    {
+                        uint32_t node, head;
+                        row_of(ra, node, head);
+                        wa = ra >= it.rows ? 0 : p.mask ? p.mask[it.row0 + node] : ~0ull >> (63 - min(node, 63u));
+                        row_of(rb, node, head);
+                        wb = rb >= it.rows ? 0 : p.mask ? p.mask[it.row0 + node] : ~0ull >> (63 - min(node, 63u));
+                    }
+#pragma unroll
+                    for (uint32_t i = 0; i < NS; ++i) {
+                        const uint32_t x = slot_in(i);
+                        const bool seen = there >> x & 1 && (!(drafted >> x & 1) || ((second(i) ? wb : wa) >> (slot0 + x - it.length) & 1));
+                        if (!seen) s[i] = -INFINITY;
+                        else if (odd >> x & 1) s[i] = NAN;
+                    }
+#pragma unroll
+                    for (uint32_t n = 0; n < 2; ++n)
+                        keep[n] = (drop >> (8 * n + 2 * t) & 1 ? 0u : 0x0000ffffu) | (drop >> (8 * n + 2 * t) & 2 ? 0u : 0xffff0000u);
+                }
+                // value scales: R = 8, of slots g, g + 8; R = 16, of slots 2t, 2t + 1, 8 more
+                [[maybe_unused]] float dv[Q8 ? NB : 1][QR];
+                float widest = 0.f;
+                if constexpr (Q8) {
+#pragma unroll
+                    for (uint32_t k = 0; k < NB; ++k) {
+                        const uint8_t* scales = values + kKvGroup * D + k * kKvGroup * 2;
+                        if constexpr (R == 8) {
+                            dv[k][0] = __half2float(*reinterpret_cast<const __half*>(scales + g * 2));
+                            dv[k][1] = __half2float(*reinterpret_cast<const __half*>(scales + g * 2 + 16));
+                            if constexpr (EDGE) { if (drop >> g & 1) dv[k][0] = 0.f; if (drop >> (g + 8) & 1) dv[k][1] = 0.f; }
+                        } else {
+#pragma unroll
+                            for (uint32_t n = 0; n < 2; ++n) {
+                                const float2 f = __half22float2(bits_h2(*reinterpret_cast<const uint32_t*>(scales + (8 * n + 2 * t) * 2) & keep[n]));
+                                dv[k][2 * n % QR] = f.x; dv[k][(2 * n + 1) % QR] = f.y;
+                            }
+                        }
+#pragma unroll
+                        for (uint32_t i = 0; i < QR; ++i) widest = fmaxf(widest, fabsf(dv[k][i]));
+                    }
+                }
+                float xa = -INFINITY, xb = -INFINITY;
+#pragma unroll
+                for (uint32_t i = 0; i < NS; ++i) { if (second(i)) xb = fmaxf(xb, s[i]); else xa = fmaxf(xa, s[i]); }
+                xa *= fa; xb *= fb;
+                if (__any_sync(NONE, xa > limit_a || xb > limit_b || widest > limit_v)) {
+#pragma unroll
+                    for (uint32_t x = R == 8 ? 4 : 1; x < (R == 8 ? 32 : 4); x *= 2) { xa = fmaxf(xa, __shfl_xor_sync(NONE, xa, x)); xb = fmaxf(xb, __shfl_xor_sync(NONE, xb, x)); }
+                    xa = fmaxf(xa, ma); xb = fmaxf(xb, mb);
+                    float fall = 0.f;
+                    if constexpr (Q8) {   // widest < 2^(e + 1): weights up to 2^kSlack times it times 2^lift stay below 2^15
+                        const uint32_t bits = __reduce_max_sync(NONE, __float_as_uint(widest));
+                        const float now = fminf(lift, 6.f - static_cast<float>(static_cast<int>(min(bits >> 23, 143u)) - 127));
+                        fall = now - lift;
+                        lift = now;
+                        limit_v = exp2f(7.f - lift);
+                    }
+                    const float r0 = ma == -INFINITY ? 0.f : exp2_approx(ma - xa + fall), r1 = mb == -INFINITY ? 0.f : exp2_approx(mb - xb + fall);
+                    la *= ma == -INFINITY ? 1.f : r0; lb *= mb == -INFINITY ? 1.f : r1;   // a NaN stays
+                    ma = xa; mb = xb;
+                    limit_a = ma + kSlack; limit_b = mb + kSlack;
+                    ref_a = ma == -INFINITY ? 0.f : lift - ma; ref_b = mb == -INFINITY ? 0.f : lift - mb;
+#pragma unroll
+                    for (uint32_t k = 0; k < NB; ++k)
+#pragma unroll
+                        for (uint32_t i = 0; i < NI; ++i)
+#pragma unroll
+                            for (uint32_t c = 0; c < 4; ++c) o[k][i][c] *= second(c) ? r1 : r0;
+                }
+                float pr[NS];
+#pragma unroll
+                for (uint32_t i = 0; i < NS; ++i) {
+                    pr[i] = exp2_approx(fmaf(s[i], second(i) ? fb : fa, second(i) ? ref_b : ref_a));
+                    if (second(i)) lb += pr[i]; else la += pr[i];
+                }
+                uint32_t wf[QR];
+                [[maybe_unused]] uint32_t wl[QR];
+                auto split = [&](const float (&w)[NS]) {   // R = 16: A fragment (rows g, g + 8; slots 2t.., 8 more); R = 8: B fragment, slots 2t.., 8 more, row g
+#pragma unroll
+                    for (uint32_t r = 0; r < QR; ++r) {
+                        wf[r] = h2_bits(__floats2half2_rn(w[2 * r], w[2 * r + 1]));
+                        if constexpr (!F16) wl[r] = pack_low(w[2 * r], w[2 * r + 1], wf[r]);
+                        if constexpr (R == 8) {
+                            wf[r] = transposed(wf[r]);
+                            if constexpr (!F16) wl[r] = transposed(wl[r]);
+                        }
+                    }
+                };
+                if constexpr (!Q8) split(pr);
+#pragma unroll
+                for (uint32_t k = 0; k < NB; ++k) {
+                    uint32_t vb[8];   // dims 8 i + g: slots 2t, 2t + 1 in vb[2 i], 8 further in vb[2 i + 1]
+                    if constexpr (Q8) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(values + k * 512 + lane * 16);
+                        codes_to_halves(w.x, vb[0], vb[1]); codes_to_halves(w.y, vb[2], vb[3]);
+                        codes_to_halves(w.z, vb[4], vb[5]); codes_to_halves(w.w, vb[6], vb[7]);
+                        float w4[NS];
+#pragma unroll
+                        for (uint32_t i = 0; i < NS; ++i) w4[i] = pr[i] * dv[k][R == 8 ? i / 2 : i / 4 * 2 + i % 2];
+                        split(w4);
+                    } else {
+                        const uint4 w = *reinterpret_cast<const uint4*>(values + k * 1024 + lane * 16), x = *reinterpret_cast<const uint4*>(values + k * 1024 + 512 + lane * 16);
+                        vb[0] = w.x; vb[1] = w.y; vb[2] = w.z; vb[3] = w.w; vb[4] = x.x; vb[5] = x.y; vb[6] = x.z; vb[7] = x.w;
+                        if constexpr (EDGE) {
+#pragma unroll
+                            for (uint32_t i = 0; i < 8; ++i) vb[i] &= keep[i & 1];
+                        }
+                    }
+#pragma unroll
+                    for (uint32_t i = 0; i < NI; ++i) {
+                        auto product = [&](float (&acc)[4], const uint32_t (&w)[QR], bool fresh) {
+                            if constexpr (R == 8) {
+                                if (fresh) mma_f16_16816_zero(acc, vb[4 * i % 8], vb[(4 * i + 2) % 8], vb[(4 * i + 1) % 8], vb[(4 * i + 3) % 8], w[0], w[1]);
+                                else mma_f16_16816(acc, vb[4 * i % 8], vb[(4 * i + 2) % 8], vb[(4 * i + 1) % 8], vb[(4 * i + 3) % 8], w[0], w[1]);
+                            } else {
+                                if (fresh) mma_f16_16816_zero(acc, w[0], w[1], w[2 % QR], w[3 % QR], vb[2 * i], vb[2 * i + 1]);
+                                else mma_f16_16816(acc, w[0], w[1], w[2 % QR], w[3 % QR], vb[2 * i], vb[2 * i + 1]);
+                            }
+                        };
+                        if constexpr (F16) product(o[k][i], wf, false);
+                        else {   // the tensor core cuts its sums off: a chain of two products, added up rounded
+                            float acc[4];
+                            product(acc, wf, true);
+                            product(acc, wl, false);
+#pragma unroll
+                            for (uint32_t c = 0; c < 4; ++c) o[k][i][c] += acc[c];
+                        }
+                    }
+                }
+            };
+            const uint64_t plain = it.start + it.length / kKvGroup;   // units before this one lie in the context
+            const uint32_t inner = plain <= a ? 0u : static_cast<uint32_t>(min(plain - a, static_cast<uint64_t>(stop)));
+            // false: the wait has run out, and no wait is tried again
+            auto arrived = [&](uint32_t st) { return !lost && (mbar_try_wait(&sm.full[warp][st], phase) || mbar_wait(&sm.full[warp][st], phase)); };
+            auto step = [&](uint32_t st, auto edge_tag) {
+                if (!__all_sync(NONE, arrived(st))) {
+                    if (!lost && lane == 0) raise_error(p.error, TSP_ERR_TIMEOUT);
+                    lost = dead = true;
+                } else if (gone >> st & 1) dead = true;
+                else unit(edge_tag, sm.ring[warp] + st * S::kGroupBytes);
                 __syncwarp();
-                issue();   // into the stage that was just read
+                if (!lost) issue(st);   // into the stage that was just read
+            };
+            for (; done < inner; ++done) {
+                step(stage, std::false_type{});
+                if (++stage == P) { stage = 0; phase ^= 1; }
+            }
+            for (; done < stop; ++done) {
+                step(stage, std::true_type{});
+                if (++stage == P) { stage = 0; phase ^= 1; }
             }
 
             // ---- end of the item or of the run
