@@ -51,7 +51,13 @@ struct AttnShape {
     static constexpr uint32_t kWarps = R == 8 && 16 * 3 * kGroupBytes <= 212992 ? 16 : 8 * 3 * kGroupBytes <= 212992 ? 8 : 4, kThreads = 32 * kWarps;
     static constexpr uint32_t kStages = 212992 / (kWarps * kGroupBytes) < 6 ? 212992 / (kWarps * kGroupBytes) : 6;
     static constexpr uint32_t kRing = kStages * kGroupBytes;   // a warp's
-    static_assert(kStages >= 3 && kRing >= R * D * 4 && R * D <= 2048, "a warp's last piece lies in its ring");
+    static_assert(kStages >= 3 && kRing >= (R * D + kPartHead) * 4 && R * D <= 2048, "a warp's last piece lies in its ring");
+};
+struct AttnItem {
+    uint64_t start, end;     // units of the item
+    uint64_t length, total;  // slots of the context, and with the step's own
+    uint32_t seq, head, tile, row0, drafted, rows;   // rows: of this tile
+    bool dead;               // out of range: zeros
 };
 template <uint32_t D, bool Q8, bool F16, uint32_t R>
 struct AttnSmem {
@@ -61,9 +67,10 @@ struct AttnSmem {
     uint64_t cum[TSP_KV_MAX_SEQUENCES + 1];
     uint64_t warp_sums[S::kWarps];
     uint64_t key[S::kWarps][2];              // first unit of the item that a piece belongs to, ~0: none
-    float m[S::kWarps][2][R], l[S::kWarps][2][R];
-    uint32_t dead[S::kWarps][2];
-    uint32_t last[2];
+    alignas(16) float meet[S::kWarps * D];
+    AttnItem item[S::kWarps][2];             // and the item itself
+    AttnItem edge[2];                        // items of the run's first and last unit
+    uint32_t last[2], span[2][2];            // whether the block joins its first / last item; the item's blocks
 };
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -71,6 +78,18 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Pieces lie in shared memory or were written by other blocks: generic addresses, past the L1
+__device__ __forceinline__ float load_piece(const float* p) {
+    float v;
+    asm volatile("ld.relaxed.gpu.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 load_piece4(const float* p) {
+    float4 v;
+    asm volatile("ld.relaxed.gpu.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+    return v;
+}
+template <bool F16> __device__ __forceinline__ bool in_range(float v) { return F16 ? fabsf(v) < 65520.f : finite_f32(v); }
 __device__ __forceinline__ float weight_of(float m, float top) { return m == -INFINITY ? 0.f : exp2_approx(m - top); }
 __device__ __forceinline__ uint32_t h2_bits(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
@@ -102,12 +121,6 @@ __device__ __forceinline__ uint32_t pack_low(float u, float v, uint32_t high) { 
 }
 __device__ __forceinline__ bool odd_half(uint32_t bits) { return (bits & 0x7c00u) == 0x7c00u; }
 
-struct AttnItem {
-    uint64_t start, end;     // units of the item
-    uint64_t length, total;  // slots of the context, and with the step's own
-    uint32_t seq, head, tile, row0, drafted, rows;   // rows: of this tile
-    bool dead;               // out of range: zeros
-};
 
 // Geometry of a sequence: units of an item, row tiles
 template <uint32_t R>
@@ -183,7 +196,7 @@ tree_attention_kernel(const AttnParams p) {
             if (lane >= o) run += below;
         }
         if (lane == 31) sm.warp_sums[warp] = run;
-        if (lane < 2) { sm.key[warp][lane] = ~0ull; sm.dead[warp][lane] = 0; }
+        if (lane < 2) sm.key[warp][lane] = ~0ull;
         __syncthreads();
         uint64_t base = run - sum;
         for (uint32_t w = 0; w < warp; ++w) base += sm.warp_sums[w];
@@ -209,8 +222,9 @@ tree_attention_kernel(const AttnParams p) {
     auto slot_in = [&](uint32_t i) { return R == 8 ? g + 8 * (i / 2) : 8 * (i / 4) + 2 * t + i % 2; };
     float* const warp_part = p.parts + (2ull * kAttnMaxBlocks + blockIdx.x * kMaxWarps + warp) * part_floats();
     {
-        const uint64_t n = u1 - u0, a = u0 + n * warp / W, b = u0 + n * (warp + 1) / W;
-        const uint32_t mine = static_cast<uint32_t>(b - a);
+        // warps without a unit are the last ones: the pieces of an item lie in neighbouring rings
+        const uint32_t n = static_cast<uint32_t>(u1 - u0), mine = n / W + (warp < n % W);
+        const uint64_t a = u0 + warp * (n / W) + min(warp, n % W), b = a + mine;
         uint64_t src = 0;              // lane i: source of unit i of the 32 that `issued` is in
         uint32_t issued = 0, gone = 0; // bit st: the unit in stage st has no page
         auto issue = [&](uint32_t st) {
@@ -239,6 +253,7 @@ tree_attention_kernel(const AttnParams p) {
         for (uint32_t done = 0; done < mine;) {
             const AttnItem it = item_of<R>(p, sm.cum, a + done);
             const uint32_t stop = static_cast<uint32_t>(min(it.end, b) - a);
+            if (lane == 0) { if (a + done == u0) sm.edge[0] = it; if (a + stop == u1) sm.edge[1] = it; }
             // ---- the item's rows as fragments: step 2 b + h holds, in lane (row % 8, t), dims 32 b + 8 t + 4 h + 0..3, the order of a lane's keys
             uint32_t qf[F16 ? 1 : 2][D / 16][QR];
             float fa, fb;
@@ -613,12 +628,12 @@ tree_attention_kernel(const AttnParams p) {
                 }
             } else {
                 const uint32_t which = stop == mine ? 1 : 0;   // 1: the run's last item, into the ring, where no copy is under way any more
-                float* rows = which ? reinterpret_cast<float*>(sm.ring[warp]) : warp_part;
+                float* part = which ? reinterpret_cast<float*>(sm.ring[warp]) : warp_part;
                 if (R == 8 ? g == 0 : t == 0) {
-                    sm.m[warp][which][ra] = ma == -INFINITY ? ma : ma - lift; sm.m[warp][which][rb] = mb == -INFINITY ? mb : mb - lift;
-                    sm.l[warp][which][ra] = la; sm.l[warp][which][rb] = lb;
+                    part[ra] = ma == -INFINITY ? ma : -ref_a; part[rb] = mb == -INFINITY ? mb : -ref_b;
+                    part[16 + ra] = la; part[16 + rb] = lb;
                 }
-                if (lane == 0) { sm.key[warp][which] = it.start; sm.dead[warp][which] = dead; }
+                if (lane == 0) { sm.key[warp][which] = it.start; sm.item[warp][which] = it; part[32] = dead ? 1.f : 0.f; }
 #pragma unroll
                 for (uint32_t k = 0; k < NB; ++k)
 #pragma unroll
@@ -626,179 +641,172 @@ tree_attention_kernel(const AttnParams p) {
 #pragma unroll
                         for (uint32_t c = 0; c < 4; ++c) {
                             const uint32_t r = second(c) ? rb : ra;
-                            if (r < it.rows) rows[r * D + dim_of(k, i, c)] = o[k][i][c];
+                            if (r < it.rows) part[kPartHead + r * D + dim_of(k, i, c)] = o[k][i][c];
                         }
             }
         }
     }
     __syncthreads();
 
-    // ---- the warps' pieces meet. Piece j (lane j): warp j / 2, its first or last item; consecutive pieces of one item are a group; a warp takes a row of one
+    // ---- pieces of an item meet: first those of the block's warps, one item after another, then, where this block is the last of an item's to arrive,
+    // those of its blocks. All of it is one loop: what runs once per launch waits for its instructions more than for anything else (unrolled
+    // code of their own took the two joins 10 us of a call of 22).
     constexpr uint32_t LANES = D / 4 < 32 ? D / 4 : 32, V = D / 4 / LANES;   // lanes of a row, float4s a lane
-    const uint64_t key = lane < 2 * W ? sm.key[lane / 2][lane % 2] : ~0ull;
-    const uint32_t there = __ballot_sync(NONE, key != ~0ull);
-    uint32_t heads;
-    {
-        const uint32_t below = there & ((1u << lane) - 1);
-        const uint64_t before = __shfl_sync(NONE, key, below ? 31 - __clz(below) : 0);
-        heads = __ballot_sync(NONE, key != ~0ull && (!below || before != key));
-    }
-    auto finish_row = [&](const AttnItem& it, uint32_t r, float4 (&y)[V], float sum, bool dead) {   // by a whole warp
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        bool ok = sum == sum;
-#pragma unroll
-        for (uint32_t k = 0; k < V; ++k) {
-            float* v = &y[k].x;
-#pragma unroll
-            for (uint32_t c = 0; c < 4; ++c) { v[c] *= inv; ok &= F16 ? fabsf(v[c]) < 65520.f : finite_f32(v[c]); }
-        }
-        ok = __all_sync(NONE, ok || lane >= LANES);
-        if (!ok && !dead && lane == 0) raise_error(p.error, TSP_ERR_NONFINITE);
-        const uint32_t flat = it.tile * R + r, node = flat / p.group, head = it.head * p.group + flat % p.group;
-        uint8_t* dst = p.out + static_cast<uint64_t>(it.row0 + node) * p.out_stride + head * D * (F16 ? 2u : 4u);
-        if (lane < LANES)
-#pragma unroll
-            for (uint32_t k = 0; k < V; ++k) {
-                if (!ok || dead) y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                const uint32_t x = k * LANES + lane;
-                if constexpr (F16) reinterpret_cast<uint2*>(dst)[x] = make_uint2(h2_bits(__floats2half2_rn(y[k].x, y[k].y)), h2_bits(__floats2half2_rn(y[k].z, y[k].w)));
-                else reinterpret_cast<float4*>(dst)[x] = y[k];
-            }
-    };
-    auto add = [](float4& y, const float4& v, float f) { y.x = fmaf(v.x, f, y.x); y.y = fmaf(v.y, f, y.y); y.z = fmaf(v.z, f, y.z); y.w = fmaf(v.w, f, y.w); };
+    const bool has_row = lane < LANES;
     auto block_part = [&](uint64_t block, bool at_start) { return p.parts + (2 * block + (at_start ? 0 : 1)) * part_floats(); };
-    uint32_t task = 0;
-    for (uint32_t left = heads; left; left &= left - 1) {
-        const uint32_t head = __ffs(left) - 1, next = left & (left - 1);
-        const uint32_t members = there & ~((1u << head) - 1) & (next ? (1u << (__ffs(next) - 1)) - 1 : NONE);
-        const AttnItem it = item_of<R>(p, sm.cum, __shfl_sync(NONE, key, head));
-        const bool complete = it.start >= u0 && it.end <= u1, mine = members >> lane & 1;
-        const bool dead = __any_sync(NONE, mine && sm.dead[lane / 2 % W][lane % 2]);
-        float* part = block_part(blockIdx.x, it.start <= u0);
-        for (uint32_t r = 0; r < it.rows; ++r, ++task) {
-            if (task % W != warp) continue;
-            const float m = mine ? sm.m[lane / 2 % W][lane % 2][r] : -INFINITY, l = mine ? sm.l[lane / 2 % W][lane % 2][r] : 0.f;
-            float top = m;
-#pragma unroll
-            for (uint32_t x = 16; x; x /= 2) top = fmaxf(top, __shfl_xor_sync(NONE, top, x));
-            const float f = weight_of(m, top);
-            float sum = m == -INFINITY ? l : l * f;   // a row of NaN alone has a sum of NaN and no reference
-#pragma unroll
-            for (uint32_t x = 16; x; x /= 2) sum += __shfl_xor_sync(NONE, sum, x);
-            float4 y[V];
-#pragma unroll
-            for (uint32_t k = 0; k < V; ++k) y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (uint32_t rest = members; rest; rest &= rest - 1) {
-                const uint32_t j = __ffs(rest) - 1;
-                const float fj = __shfl_sync(NONE, f, j);
-                if (fj == 0.f) continue;
-                const float* rows = j % 2 ? reinterpret_cast<const float*>(sm.ring[j / 2]) : p.parts + (2ull * kAttnMaxBlocks + blockIdx.x * kMaxWarps + j / 2) * part_floats();
-#pragma unroll
-                for (uint32_t k = 0; k < V; ++k)
-                    if (lane < LANES) add(y[k], reinterpret_cast<const float4*>(rows + r * D)[k * LANES + lane], fj);
-            }
-            if (complete) finish_row(it, r, y, sum, dead);
-            else {
-#pragma unroll
-                for (uint32_t k = 0; k < V; ++k)
-                    if (lane < LANES) __stcg(reinterpret_cast<float4*>(part + kPartHead + r * D) + k * LANES + lane, y[k]);
-                if (lane == 0) { __stcg(part + r, top); __stcg(part + 16 + r, sum); __stcg(part + 32, dead ? 1.f : 0.f); }
-            }
-        }
-    }
-    // ---- pieces of the block: of the item at its start, and of another at its end
-    const AttnItem first = item_of<R>(p, sm.cum, u0), last = item_of<R>(p, sm.cum, u1 - 1);
+    // Piece j (lane j) is warp j / 2's first or last item; consecutive pieces of one item are a group
+    const uint64_t key = lane < 2 * W ? sm.key[lane / 2][lane % 2] : ~0ull;
+    const uint32_t there = __ballot_sync(NONE, key != ~0ull), below = there & ((1u << lane) - 1);
+    const uint64_t before = __shfl_sync(NONE, key, below ? 31 - __clz(below) : 0);
+    uint32_t heads = __ballot_sync(NONE, key != ~0ull && (!below || before != key));
+    const AttnItem &first = sm.edge[0], &last = sm.edge[1];
     const bool open0 = first.start < u0 || first.end > u1, open1 = last.start != first.start && last.end > u1;
-    if (!open0 && !open1) return;
-    __threadfence();
-    __syncthreads();
-    if (tid < 2) {
-        const AttnItem& it = tid ? last : first;
-        sm.last[tid] = 0;
-        if (tid ? open1 : open0) {
-            const uint32_t c0 = static_cast<uint32_t>(it.start / quota), c1 = static_cast<uint32_t>((it.end - 1) / quota);
-            if (atomicAdd(p.counters + c0, 1u) == c1 - c0) { sm.last[tid] = 1; p.counters[c0] = 0; }
+    float4* const meet = reinterpret_cast<float4*>(sm.meet);
+    uint32_t task = warp;   // inside the block every warp takes every W-th row of all items' together
+#pragma unroll 1
+    for (uint32_t side = 0; side < 2;) {
+        // n pieces: at p0, then p1 + stride (i - 1), the last of them at pl
+        const AttnItem* item;
+        const float *p0, *p1, *pl;
+        uint32_t n, stride;
+        const bool inside = heads != 0;
+        if (inside) {
+            const uint32_t head = __ffs(heads) - 1, next = heads & (heads - 1);
+            const uint32_t members = there & ~((1u << head) - 1) & (next ? (1u << (__ffs(next) - 1)) - 1 : NONE), tail = 31 - __clz(members);
+            auto piece = [&](uint32_t j) { return j % 2 ? reinterpret_cast<const float*>(sm.ring[j / 2]) : p.parts + (2ull * kAttnMaxBlocks + blockIdx.x * kMaxWarps + j / 2) * part_floats(); };
+            item = &sm.item[head / 2][head % 2];
+            n = __popc(members);
+            p0 = piece(head); pl = piece(tail);
+            p1 = reinterpret_cast<const float*>(sm.ring[head / 2 + (n > 1)]);
+            stride = S::kRing / 4;
+            heads = next;
+        } else {
+            if (side == 0) {   // the block's own pieces are written: count it in
+                if (!open0 && !open1) return;
+                __syncthreads();
+                if (tid < 2) {
+                    __threadfence();   // they go before the count
+                    const AttnItem& it = tid ? last : first;
+                    uint32_t joins = 0;
+                    if (tid ? open1 : open0) {
+                        const uint32_t c0 = static_cast<uint32_t>(it.start / quota), c1 = static_cast<uint32_t>((it.end - 1) / quota);
+                        joins = atomicAdd(p.counters + c0, 1u) == c1 - c0;
+                        if (joins) p.counters[c0] = 0;
+                        sm.span[tid][0] = c0; sm.span[tid][1] = c1 - c0 + 1;
+                    }
+                    sm.last[tid] = joins;
+                    __threadfence();
+                }
+                __syncthreads();
+            }
+            const uint32_t mine = side++;
+            if (!sm.last[mine]) continue;
+            item = mine ? &last : &first;
+            const uint32_t c0 = sm.span[mine][0];
+            n = sm.span[mine][1];
+            p0 = block_part(c0, item->start == c0 * quota);
+            p1 = block_part(c0 + 1, true);
+            stride = 2 * static_cast<uint32_t>(part_floats());
+            pl = n > 1 ? p1 + static_cast<uint64_t>(n - 2) * stride : p0;
         }
-    }
-    __syncthreads();
-    for (uint32_t side = 0; side < 2; ++side) {
-        if (!sm.last[side]) continue;
-        __threadfence();
-        const AttnItem& it = side ? last : first;
-        const uint32_t c0 = static_cast<uint32_t>(it.start / quota), n = static_cast<uint32_t>((it.end - 1) / quota) - c0 + 1;
-        const float* part0 = block_part(c0, it.start == c0 * quota);
-        const float* part1 = block_part(c0 + 1, true);
-        auto part_of = [&](uint32_t i) { return i == 0 ? part0 : part1 + 2ull * (i - 1) * part_floats(); };
-        // a row by `ways` warps, each every ways-th piece; they meet in the rings
-        const uint32_t ways = it.rows < W ? W / it.rows : 1;
-        float4* meet = reinterpret_cast<float4*>(sm.ring);
-        for (uint32_t r0 = 0; r0 < it.rows; r0 += W) {
-            const uint32_t r = r0 + warp % min(W, it.rows), way = warp / min(W, it.rows);
-            const bool on = way < ways && r < it.rows;
+        auto part_of = [&](uint32_t i) { return i == 0 ? p0 : i == n - 1 ? pl : p1 + static_cast<uint64_t>(i - 1) * stride; };
+        // a row by `ways` warps, each every ways-th piece of every 32; the references of all of them go by all the warps, so that theirs is the same
+        const uint32_t rows = item->rows, wide = min(W, rows), ways = inside ? 1 : W / wide, way = inside ? 0 : warp / wide;
+        uint32_t r = inside ? task : warp % wide;
+#pragma unroll 1
+        for (; inside ? r < rows : r < (rows + wide - 1) / wide * wide; r += inside ? W : wide) {
+            const bool on = way < ways && r < rows;
             float4 y[V];
-            float sum = 0.f;
-            bool dead = false;
 #pragma unroll
             for (uint32_t k = 0; k < V; ++k) y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            float top = -INFINITY, sum = 0.f;
+            bool dead = false;
             if (on) {
-                constexpr uint32_t LOADS = kAttnMaxBlocks / 32;
-                float m[LOADS], top = -INFINITY;
+#pragma unroll 1
+                for (uint32_t i0 = 0; i0 < n; i0 += 32) {
+                    const uint32_t i = i0 + lane, count = min(32u, n - i0);
+                    const float* head = part_of(min(i, n - 1));
+                    float m = load_piece(head + r), l = load_piece(head + 16 + r);
+                    dead |= load_piece(head + 32) != 0.f;
+                    if (i >= n) { m = -INFINITY; l = 0.f; }
+                    float now = m;
 #pragma unroll
-                for (uint32_t k = 0; k < LOADS; ++k) {
-                    const uint32_t i = k * 32 + lane;
-                    m[k] = -INFINITY;
-                    if (i < n) { m[k] = __ldcg(part_of(i) + r); dead |= __ldcg(part_of(i) + 32) != 0.f; }
-                    top = fmaxf(top, m[k]);
-                }
+                    for (uint32_t x = 16; x; x /= 2) now = fmaxf(now, __shfl_xor_sync(NONE, now, x));
+                    now = fmaxf(now, top);
+                    const float f = weight_of(m, now), old = weight_of(top, now);
+                    sum = (top == -INFINITY ? sum : sum * old) + (m == -INFINITY ? l : l * f);   // a row of NaN alone has a sum of NaN and no reference
 #pragma unroll
-                for (uint32_t x = 16; x; x /= 2) top = fmaxf(top, __shfl_xor_sync(NONE, top, x));
+                    for (uint32_t k = 0; k < V; ++k) { y[k].x *= old; y[k].y *= old; y[k].z *= old; y[k].w *= old; }
+                    top = now;
+#pragma unroll 1
+                    for (uint32_t j0 = way; j0 < count; j0 += 4 * ways) {
+                        float4 v[4][V];
+                        float fj[4];
 #pragma unroll
-                for (uint32_t k = 0; k < LOADS; ++k) {
-                    const uint32_t i = k * 32 + lane;
-                    const float l = i < n ? __ldcg(part_of(i) + 16 + r) : 0.f, f = weight_of(m[k], top);
-                    sum += m[k] == -INFINITY ? l : l * f;
-                    m[k] = f;
+                        for (uint32_t j = 0; j < 4; ++j) {
+                            const uint32_t at = min(j0 + j * ways, count - 1);
+                            fj[j] = __shfl_sync(NONE, f, at);
+                            if (j0 + j * ways >= count) fj[j] = 0.f;
+#pragma unroll
+                            for (uint32_t x = 0; x < V; ++x) v[j][x] = load_piece4(part_of(i0 + at) + kPartHead + r * D + (x * LANES + lane % LANES) * 4);
+                        }
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; ++j)
+                            if (fj[j] != 0.f)
+#pragma unroll
+                                for (uint32_t x = 0; x < V; ++x) {
+                                    y[x].x = fmaf(v[j][x].x, fj[j], y[x].x); y[x].y = fmaf(v[j][x].y, fj[j], y[x].y);
+                                    y[x].z = fmaf(v[j][x].z, fj[j], y[x].z); y[x].w = fmaf(v[j][x].w, fj[j], y[x].w);
+                                }
+                    }
                 }
 #pragma unroll
                 for (uint32_t x = 16; x; x /= 2) sum += __shfl_xor_sync(NONE, sum, x);
                 dead = __any_sync(NONE, dead);
-#pragma unroll
-                for (uint32_t k = 0; k < LOADS; ++k) {
-                    const uint32_t end = min(n, k * 32 + 32);
-                    for (uint32_t i0 = k * 32 + (way + ways - k * 32 % ways) % ways; i0 < end; i0 += 8 * ways) {
-                        float4 v[8][V];
-                        float f[8];
-#pragma unroll
-                        for (uint32_t j = 0; j < 8; ++j) {
-                            const uint32_t i = i0 + j * ways;
-                            f[j] = __shfl_sync(NONE, m[k], i % 32);
-                            if (i >= end) f[j] = 0.f;
-#pragma unroll
-                            for (uint32_t x = 0; x < V; ++x)
-                                if (f[j] != 0.f && lane < LANES) v[j][x] = __ldcg(reinterpret_cast<const float4*>(part_of(i) + kPartHead + r * D) + x * LANES + lane);
-                        }
-#pragma unroll
-                        for (uint32_t j = 0; j < 8; ++j)
-#pragma unroll
-                            for (uint32_t x = 0; x < V; ++x)
-                                if (f[j] != 0.f && lane < LANES) add(y[x], v[j][x], f[j]);
-                    }
-                }
-            }
-            if (ways > 1) {
-                if (on && way && lane < LANES)
+                if (way && has_row)
 #pragma unroll
                     for (uint32_t k = 0; k < V; ++k) meet[(warp * V + k) * LANES + lane] = y[k];
-                __syncthreads();
-                if (on && !way)
-                    for (uint32_t x = 1; x < ways; ++x)
-                        if (lane < LANES)
-#pragma unroll
-                            for (uint32_t k = 0; k < V; ++k) add(y[k], meet[((warp + x * it.rows) * V + k) * LANES + lane], 1.f);
-                __syncthreads();
             }
-            if (on && !way) finish_row(it, r, y, sum, dead);
+            if (ways > 1) __syncthreads();
+            if (on && !way) {
+#pragma unroll 1
+                for (uint32_t x = 1; x < ways; ++x)
+#pragma unroll
+                    for (uint32_t k = 0; k < V; ++k) {
+                        const float4 v = meet[((warp + x * wide) * V + k) * LANES + lane % LANES];
+                        y[k].x += v.x; y[k].y += v.y; y[k].z += v.z; y[k].w += v.w;
+                    }
+                if (inside && (item->start < u0 || item->end > u1)) {   // still a piece
+                    float* part = block_part(blockIdx.x, item->start <= u0);
+                    if (has_row)
+#pragma unroll
+                        for (uint32_t k = 0; k < V; ++k) __stcg(reinterpret_cast<float4*>(part + kPartHead + r * D) + k * LANES + lane, y[k]);
+                    if (lane == 0) { __stcg(part + r, top); __stcg(part + 16 + r, sum); __stcg(part + 32, dead ? 1.f : 0.f); }
+                } else {
+                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                    bool ok = sum == sum;
+#pragma unroll
+                    for (uint32_t k = 0; k < V; ++k) {
+                        y[k].x *= inv; y[k].y *= inv; y[k].z *= inv; y[k].w *= inv;
+                        ok &= in_range<F16>(y[k].x) && in_range<F16>(y[k].y) && in_range<F16>(y[k].z) && in_range<F16>(y[k].w);
+                    }
+                    ok = __all_sync(NONE, ok);
+                    if (!ok && !dead && lane == 0) raise_error(p.error, TSP_ERR_NONFINITE);
+                    const uint32_t flat = item->tile * R + r, node = flat / p.group, head = item->head * p.group + flat % p.group;
+                    uint8_t* dst = p.out + static_cast<uint64_t>(item->row0 + node) * p.out_stride + head * D * (F16 ? 2u : 4u);
+                    if (has_row)
+#pragma unroll
+                        for (uint32_t k = 0; k < V; ++k) {
+                            if (!ok || dead) y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            const uint32_t x = k * LANES + lane;
+                            if constexpr (F16) reinterpret_cast<uint2*>(dst)[x] = make_uint2(h2_bits(__floats2half2_rn(y[k].x, y[k].y)), h2_bits(__floats2half2_rn(y[k].z, y[k].w)));
+                            else reinterpret_cast<float4*>(dst)[x] = y[k];
+                        }
+                }
+            }
+            if (ways > 1) __syncthreads();
         }
+        if (inside) task = r - rows;
     }
 }
 
