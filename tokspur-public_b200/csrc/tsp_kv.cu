@@ -11,6 +11,10 @@ template <bool F16> __device__ __forceinline__ float load1(const uint8_t* p, uin
     if constexpr (F16) return __half2float(reinterpret_cast<const __half*>(p)[i]);
     else return reinterpret_cast<const float*>(p)[i];
 }
+template <bool F16> __device__ __forceinline__ float2 load2(const uint8_t* p, uint32_t i) {
+    if constexpr (F16) return __half22float2(*reinterpret_cast<const __half2*>(p + i * 2));
+    else return *reinterpret_cast<const float2*>(p + i * 4);
+}
 template <bool F16> __device__ __forceinline__ void load4(const uint8_t* p, uint32_t i, float (&v)[4]) {
     if constexpr (F16) {
         const uint2 u = *reinterpret_cast<const uint2*>(p + i * 2);
@@ -39,36 +43,31 @@ template <typename T> __device__ __forceinline__ int code_of(T y, T d, T inv) {
     return max(-127, min(127, r));
 }
 
-// One head of K or V (a warp, lane l holds dims l NV .. l NV + NV - 1) into its slot. Returns false where it wrote zeros for it.
-template <uint32_t D, typename T>
-__device__ __forceinline__ bool put_head(uint8_t* half, uint32_t t, bool is_v, bool q8, uint32_t lane, T (&y)[D / 32]) {
+// One head of K (a warp, lane l holds dims l NV .. l NV + NV - 1) into its slot. Returns false where it wrote zeros for it.
+template <uint32_t D>
+__device__ __forceinline__ bool put_keys(uint8_t* half, uint32_t t, bool q8, uint32_t lane, double (&y)[D / 32]) {
     constexpr uint32_t NV = D / 32;
     const uint32_t x0 = lane * NV;
     bool ok = true;
     if (q8) {
-        T top = 0;
+        double top = 0;
 #pragma unroll
         for (uint32_t i = 0; i < NV; ++i) { ok &= finite_f32(static_cast<float>(y[i])); top = fmax(top, fabs(y[i])); }
 #pragma unroll
         for (uint32_t o = 1; o < 32 / NV; o *= 2) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const __half d16 = __float2half_rn(static_cast<float>(static_cast<double>(top) / 127.0));
+        const __half d16 = __float2half_rn(static_cast<float>(top / 127.0));
         ok &= !__hisinf(d16);
         ok = __all_sync(0xffffffffu, ok);
-        const T d = ok ? static_cast<T>(__half2float(d16)) : static_cast<T>(0), inv = d > 0 ? 1 / d : 0;
+        const double d = ok ? static_cast<double>(__half2float(d16)) : 0, inv = d > 0 ? 1 / d : 0;
         uint8_t code[NV];
 #pragma unroll
-        for (uint32_t i = 0; i < NV; ++i) code[i] = static_cast<uint8_t>(d > 0 ? code_of<T>(y[i], d, inv) + 128 : 128);
-        if (is_v) {
+        for (uint32_t i = 0; i < NV; ++i) code[i] = static_cast<uint8_t>(d > 0 ? code_of<double>(y[i], d, inv) + 128 : 128);
+        uint8_t* p = half + kv_k_byte(x0, t, true);
+        if constexpr (NV == 2) *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(code[0] | code[1] << 8);
+        else {
 #pragma unroll
-            for (uint32_t i = 0; i < NV; ++i) half[kv_v_byte(x0 + i, t, true)] = code[i];
-        } else {
-            uint8_t* p = half + kv_k_byte(x0, t, true);
-            if constexpr (NV == 2) *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(code[0] | code[1] << 8);
-            else {
-#pragma unroll
-                for (uint32_t i = 0; i < NV; i += 4)
-                    *reinterpret_cast<uint32_t*>(p + i) = code[i] | code[i + 1] << 8 | code[i + 2] << 16 | static_cast<uint32_t>(code[i + 3]) << 24;
-            }
+            for (uint32_t i = 0; i < NV; i += 4)
+                *reinterpret_cast<uint32_t*>(p + i) = code[i] | code[i + 1] << 8 | code[i + 2] << 16 | static_cast<uint32_t>(code[i + 3]) << 24;
         }
         if (x0 % 32 == 0) *reinterpret_cast<__half*>(half + kv_scale_byte(x0, t, D)) = ok ? d16 : __ushort_as_half(0);
     } else {
@@ -76,12 +75,128 @@ __device__ __forceinline__ bool put_head(uint8_t* half, uint32_t t, bool is_v, b
         for (uint32_t i = 0; i < NV; ++i) ok &= fits<true>(static_cast<float>(y[i]));
         ok = __all_sync(0xffffffffu, ok);
 #pragma unroll
-        for (uint32_t i = 0; i < NV; ++i) {
-            const __half v = ok ? __float2half_rn(static_cast<float>(y[i])) : __ushort_as_half(0);
-            *reinterpret_cast<__half*>(half + (is_v ? kv_v_byte(x0 + i, t, false) : kv_k_byte(x0 + i, t, false))) = v;
-        }
+        for (uint32_t i = 0; i < NV; i += 2)
+            *reinterpret_cast<__half2*>(half + kv_k_byte(x0 + i, t, false)) = ok ? __floats2half2_rn(static_cast<float>(y[i]), static_cast<float>(y[i + 1])) : __half2half2(__ushort_as_half(0));
     }
     return ok;
+}
+
+// 16 slots of a head's values, a warp: lane (g, t) takes dims 8 i + 2 t, + 1 of slots g and g + 8, in the order of an MMA fragment, and a transposing
+// move of 8 x 8 matrices puts four slots beside each other as the cache holds them: whole 512-byte rows go out. `rows`: slots of the group that are
+// written (bit i: slot i), `at(slot)`: a slot's values. (A warp per row and head, byte by byte: three prompts of 3000 rows 100 us, now 38.)
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <uint32_t D, bool IN16, typename At>
+__device__ __forceinline__ bool put_values(uint8_t* half, uint32_t rows, bool q8, uint32_t lane, At&& at) {
+    const uint32_t g = lane / 4, t = lane % 4;
+    bool fine = true;
+    const bool on[2] = {(rows >> g & 1) != 0, (rows >> (g + 8) & 1) != 0};
+    const uint8_t* src[2] = {on[0] ? at(g) : nullptr, on[1] ? at(g + 8) : nullptr};
+    // a head whose values are not finite is zeros as a whole: look at all of it first (the second read comes from the L1)
+    bool ok[2] = {true, true};
+#pragma unroll
+    for (uint32_t n = 0; n < 2; ++n) {
+        if (on[n]) {
+#pragma unroll
+            for (uint32_t b = 0; b < D / 32; ++b)
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const float2 v = load2<IN16>(src[n], 32 * b + 8 * i + 2 * t);
+                    // a block's scale is finite in binary16 when its largest value over 127 rounds below infinity
+                    ok[n] &= q8 ? fabsf(v.x) < 127.f * 65520.f && fabsf(v.y) < 127.f * 65520.f : fits<true>(v.x) && fits<true>(v.y);
+                }
+        }
+        uint32_t v = ok[n];
+        v &= __shfl_xor_sync(0xffffffffu, v, 1);
+        v &= __shfl_xor_sync(0xffffffffu, v, 2);
+        ok[n] = v != 0;
+        fine &= ok[n];
+    }
+#pragma unroll
+    for (uint32_t b = 0; b < D / 32; ++b) {
+        float v[2][8];
+        uint32_t out[4][2];   // [i][slots 2t, 2t + 1 | 8 more]: binary16 values, or codes
+#pragma unroll
+        for (uint32_t n = 0; n < 2; ++n) {
+            float top = 0.f;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const float2 x = on[n] && ok[n] ? load2<IN16>(src[n], 32 * b + 8 * i + 2 * t) : make_float2(0.f, 0.f);
+                v[n][2 * i] = x.x; v[n][2 * i + 1] = x.y;
+                top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
+            }
+            if (q8) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const __half d16 = __float2half_rn(static_cast<float>(static_cast<double>(top) / 127.0));
+                const float d = __half2float(d16), inv = d > 0.f ? 1.f / d : 0.f;
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) v[n][i] = d > 0.f ? static_cast<float>(code_of<float>(v[n][i], d, inv)) : 0.f;
+                if (on[n] && t == 0) *reinterpret_cast<__half*>(half + kv_scale_byte(32 * b, g + 8 * n, D)) = d16;
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) out[i][n] = transposed(half2_bits(v[n][2 * i], v[n][2 * i + 1]));
+        }
+        const bool whole = rows == 0xffffu;
+        if (q8) {
+            uint32_t word[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {   // code + 128 as the low byte of 1152 + code
+                const __half2 bias = __half2half2(__ushort_as_half(0x6480));
+                const __half2 x = __hadd2(*reinterpret_cast<const __half2*>(&out[i][0]), bias), y = __hadd2(*reinterpret_cast<const __half2*>(&out[i][1]), bias);
+                word[i] = __byte_perm(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y), 0x6420);
+            }
+            uint8_t* dst = half + b * 512 + lane * 16;
+            if (whole) *reinterpret_cast<uint4*>(dst) = make_uint4(word[0], word[1], word[2], word[3]);
+            else {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e)
+                    if (rows >> (2 * t + (e & 1) + 8 * (e >> 1)) & 1)
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i) dst[i * 4 + e] = static_cast<uint8_t>(word[i] >> (8 * e));
+            }
+        } else {
+#pragma unroll
+            for (uint32_t m = 0; m < 2; ++m) {
+                uint8_t* dst = half + (b * 2 + m) * 512 + lane * 16;
+                if (whole) *reinterpret_cast<uint4*>(dst) = make_uint4(out[2 * m][0], out[2 * m][1], out[2 * m + 1][0], out[2 * m + 1][1]);
+                else {
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e)
+                        if (rows >> (2 * t + (e & 1) + 8 * (e >> 1)) & 1)
+#pragma unroll
+                            for (uint32_t i = 0; i < 2; ++i) reinterpret_cast<uint16_t*>(dst)[i * 4 + e] = static_cast<uint16_t>(out[2 * m + i][e >> 1] >> (16 * (e & 1)));
+                }
+            }
+        }
+    }
+    return fine;
+}
+
+// Groups of 16 slots that a step touches, without a scan: sequence s gets the places from d_row_offsets[s] / 16 + 2 s on. T rows touch (T + 30) / 16 groups at
+// most, and the next sequence's places start T / 16 + 2 later at least. False: a place without slots.
+__host__ __device__ constexpr uint32_t kv_group_places(uint32_t rows, uint32_t sequences) { return rows / 16 + 2 * sequences; }
+__device__ __forceinline__ bool kv_group_of_place(const tsp_kv_batch& b, uint32_t place, uint32_t lane, uint32_t& seq, uint64_t& slot0, uint32_t& row0, uint32_t& mask) {
+    auto before = [&](uint32_t s) { return b.d_row_offsets[s] / 16 + 2 * s <= place; };
+    const uint32_t step = (b.sequences + 31) / 32;
+    const uint32_t a = __popc(__ballot_sync(0xffffffffu, (lane + 1) * step < b.sequences && before(min((lane + 1) * step, b.sequences)))) * step;
+    seq = a + __popc(__ballot_sync(0xffffffffu, lane + 1 < step && a + lane + 1 < b.sequences && before(min(a + lane + 1, b.sequences))));
+    const uint32_t first = b.d_row_offsets[seq], end = b.d_row_offsets[seq + 1];
+    if (end < first || end > b.rows) return false;
+    const uint64_t length = b.d_lengths[seq], total = length + (end - first), start = length / 16 * 16 + 16ull * (place - (first / 16 + 2 * seq));
+    if (start >= total) return false;
+    slot0 = start;
+    mask = total - start >= 16 ? 0xffffu : (1u << static_cast<uint32_t>(total - start)) - 1;
+    if (start < length) mask &= 0xffffu << static_cast<uint32_t>(length - start);
+    row0 = static_cast<uint32_t>(first + start - length);   // row of the group's slot 0, modulo 2^32: that slot may lie in front of the step's first
+    return mask != 0;
 }
 
 struct HeadRows {
@@ -96,7 +211,7 @@ struct HeadRows {
 // A block per row. Angles once per row; then eight lanes' worth of pairs per group of D / 8 lanes for the rows that go out as rows, a warp per
 // head for those that go into the cache.
 template <uint32_t D, bool IN16, bool OUT16, bool CACHE>
-__global__ void __launch_bounds__(kHeadThreads)
+__global__ void __launch_bounds__(CACHE ? kHeadThreads : 512)
 head_rows_kernel(const tsp_qk_norm_rope_args a, const HeadRows r, const tsp_kv_cache cache, const tsp_kv_batch batch, uint32_t* error) {
     __shared__ float cs[D / 2], sn[D / 2];
     __shared__ double cs64[CACHE ? D / 2 : 1], sn64[CACHE ? D / 2 : 1];
@@ -107,37 +222,62 @@ head_rows_kernel(const tsp_qk_norm_rope_args a, const HeadRows r, const tsp_kv_c
     uint32_t seq = 0, node = 0;
     if constexpr (CACHE) {
         if (row == 0) kv_check_offsets(batch, error);
+        if (row >= batch.rows) {   // the blocks behind the rows': values, a warp per group of slots and head
+            const uint32_t task = (row - batch.rows) * (kHeadThreads / 32) + warp, place = task / cache.kv_heads, head = task % cache.kv_heads;
+            uint64_t slot0;
+            uint32_t row0, mask;
+            if (place >= kv_group_places(batch.rows, batch.sequences) || !kv_group_of_place(batch, place, lane, seq, slot0, row0, mask)) return;
+            const bool q8 = cache.type == TSP_TYPE_Q8_0;
+            uint8_t* group = kv_group(cache, seq, slot0, head, error);
+            if (!group) return;
+            const bool fine = put_values<D, IN16>(group + kv_half_bytes(D, q8), mask, q8, lane,
+                                                  [&](uint32_t t) { return r.v + static_cast<uint64_t>(row0 + t) * r.v_stride + head * D * (IN16 ? 2u : 4u); });
+            if (!fine) raise_error(error, TSP_ERR_NONFINITE);
+            return;
+        }
         if (!kv_row(batch, row, lane, seq, node)) return;
     }
     const uint32_t half = a.rotary_dim / 2;
+    constexpr uint32_t LANES = D / 8;   // lanes of a head
+    const uint32_t per = blockDim.x / LANES, out_heads = r.q_heads + (CACHE ? 0 : r.kv_heads), passes = (out_heads + per - 1) / per, l = tid % LANES;
+    // four pairs a lane: (u, v) at dims xu.., xv.., or interleaved in eight dims from xu on; the dims behind the rotated ones pair up as halves
+    const uint32_t p0 = 4 * l, rest = p0 - half;
+    const bool turned = p0 < half, pairs = turned && a.style == TSP_ROPE_PAIRS;
+    const uint32_t xu = turned ? (pairs ? 2 * p0 : p0) : a.rotary_dim + rest, xv = turned ? (pairs ? xu + 4 : p0 + half) : xu + (D - a.rotary_dim) / 2;
+    float u[4], v[4];
+    auto load = [&](uint32_t pass) {   // whole warps stay together for the shuffles: a lane behind the last head takes that one again
+        const uint32_t h = min(pass * per + tid / LANES, out_heads - 1);
+        const uint8_t* in = h >= r.q_heads ? r.k + row * r.k_stride + (h - r.q_heads) * D * (IN16 ? 2 : 4) : r.q + row * r.q_stride + h * D * (IN16 ? 2 : 4);
+        load4<IN16>(in, xu, u);
+        load4<IN16>(in, xv, v);
+    };
+    if (passes) load(0);   // under way while the angles are computed
     if (half) {
         const double pos = r.positions[row];
-        for (uint32_t p = tid; p < half; p += kHeadThreads) {
+        for (uint32_t p = tid; p < half; p += blockDim.x) {
             const double angle = pos * static_cast<double>(a.d_inv_freq[p]);
-            double s, c;
-            sincos(angle, &s, &c);
-            c *= a.magnitude; s *= a.magnitude;
-            cs[p] = static_cast<float>(c); sn[p] = static_cast<float>(s);
-            if constexpr (CACHE) { cs64[p] = c; sn64[p] = s; }
+            if constexpr (CACHE) {
+                double s, c;
+                sincos(angle, &s, &c);
+                c *= a.magnitude; s *= a.magnitude;
+                cs[p] = static_cast<float>(c); sn[p] = static_cast<float>(s);
+                cs64[p] = c; sn64[p] = s;
+            } else {   // turns, reduced in 64 bits
+                const double turns = angle * 0.15915494309189535;
+                float s, c;
+                sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &c);
+                cs[p] = c * a.magnitude; sn[p] = s * a.magnitude;
+            }
         }
         __syncthreads();
     }
     bool bad = false;
-    constexpr uint32_t LANES = D / 8, PER = kHeadThreads / LANES;   // lanes of a head, heads in flight
-    const uint32_t out_heads = r.q_heads + (CACHE ? 0 : r.kv_heads);
-    for (uint32_t h0 = tid / LANES; h0 < (out_heads + PER - 1) / PER * PER; h0 += PER) {   // whole warps stay together for the shuffles
-        const uint32_t h = min(h0, out_heads - 1), l = tid % LANES;
+    for (uint32_t pass = 0; pass < passes; ++pass) {
+        const uint32_t h0 = pass * per + tid / LANES, h = min(h0, out_heads - 1);
+        if (pass) load(pass);
         const bool is_k = h >= r.q_heads;
-        const uint8_t* in = is_k ? r.k + row * r.k_stride + (h - r.q_heads) * D * (IN16 ? 2 : 4) : r.q + row * r.q_stride + h * D * (IN16 ? 2 : 4);
         uint8_t* out = is_k ? r.k_out + row * r.k_out_stride + (h - r.q_heads) * D * (OUT16 ? 2 : 4) : r.q_out + row * r.q_out_stride + h * D * (OUT16 ? 2 : 4);
         const float* w = is_k ? a.d_k_norm : a.d_q_norm;
-        // four pairs a lane: (u, v) at dims xu.., xv.., or interleaved in eight dims from xu on; the dims behind the rotated ones pair up as halves
-        const uint32_t p0 = 4 * l, rest = p0 - half;
-        const bool turned = p0 < half, pairs = turned && a.style == TSP_ROPE_PAIRS;
-        const uint32_t xu = turned ? (pairs ? 2 * p0 : p0) : a.rotary_dim + rest, xv = turned ? (pairs ? xu + 4 : p0 + half) : xu + (D - a.rotary_dim) / 2;
-        float u[4], v[4];
-        load4<IN16>(in, xu, u);
-        load4<IN16>(in, xv, v);
         float wu[4] = {1.f, 1.f, 1.f, 1.f}, wv[4] = {1.f, 1.f, 1.f, 1.f};
         if (w) {
             float ss = 0.f;
@@ -179,19 +319,12 @@ head_rows_kernel(const tsp_qk_norm_rope_args a, const HeadRows r, const tsp_kv_c
         constexpr uint32_t NV = D / 32;
         const bool q8 = cache.type == TSP_TYPE_Q8_0;
         const uint64_t slot = static_cast<uint64_t>(batch.d_lengths[seq]) + node;
-        const uint32_t t = slot % kKvGroup, hb = kv_half_bytes(D, q8);
-        for (uint32_t h = warp; h < 2 * cache.kv_heads; h += kHeadThreads / 32) {
-            const bool is_v = h >= cache.kv_heads;
-            const uint32_t head = is_v ? h - cache.kv_heads : h;
-            uint8_t* group = kv_group(cache, seq, slot, head, error);
+        const uint32_t t = slot % kKvGroup;
+        for (uint32_t h = warp; h < cache.kv_heads; h += kHeadThreads / 32) {
+            uint8_t* group = kv_group(cache, seq, slot, h, error);
             if (!group) continue;
-            const uint8_t* in = is_v ? r.v + row * r.v_stride + head * D * (IN16 ? 2 : 4) : r.k + row * r.k_stride + head * D * (IN16 ? 2 : 4);
-            if (is_v) {
-                float y[NV];
-#pragma unroll
-                for (uint32_t i = 0; i < NV; ++i) y[i] = load1<IN16>(in, lane * NV + i);
-                bad |= !put_head<D, float>(group + hb, t, true, q8, lane, y);
-            } else {
+            const uint8_t* in = r.k + row * r.k_stride + h * D * (IN16 ? 2 : 4);
+            {
                 double y[NV];
 #pragma unroll
                 for (uint32_t i = 0; i < NV; ++i) y[i] = load1<IN16>(in, lane * NV + i);
@@ -221,42 +354,120 @@ head_rows_kernel(const tsp_qk_norm_rope_args a, const HeadRows r, const tsp_kv_c
                         }
                     }
                 }
-                bad |= !put_head<D, double>(group, t, false, q8, lane, y);
+                bad |= !put_keys<D>(group, t, q8, lane, y);
             }
         }
     }
     if (bad) raise_error(error, TSP_ERR_NONFINITE);
 }
 
+// A warp per group of 16 slots and head: every load is a whole 512-byte row of the group, all of them under way at once; K leaves in the order it lies in,
+// V through transposing moves as it came. (A warp per row and head, byte by byte: 60000 rows of 8 heads 238 us, now 63.)
 template <uint32_t D, bool OUT16>
+__device__ __forceinline__ void store8(uint8_t* row, uint32_t x, const float (&v)[8]) {   // eight dims from x on
+    if constexpr (OUT16) *reinterpret_cast<uint4*>(row + x * 2) = make_uint4(half2_bits(v[0], v[1]), half2_bits(v[2], v[3]), half2_bits(v[4], v[5]), half2_bits(v[6], v[7]));
+    else {
+        reinterpret_cast<float4*>(row + x * 4)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(row + x * 4)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+}
+// two words of codes + 128 -> eight values
+__device__ __forceinline__ void values_of(uint32_t a, uint32_t b, float d, float (&v)[8]) {
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) v[i] = static_cast<float>(static_cast<int>((i < 4 ? a : b) >> (8 * (i % 4)) & 0xffu) - 128) * d;
+}
+template <uint32_t D, bool OUT16, bool Q8>
 __global__ void __launch_bounds__(256)
 cache_read_kernel(const tsp_kv_cache cache, const tsp_kv_batch batch, uint8_t* k, uint64_t k_stride, uint8_t* v, uint64_t v_stride, uint32_t* error) {
     pdl_launch_dependents();
     pdl_wait();
-    constexpr uint32_t NV = D / 32;
-    const uint32_t row = blockIdx.x, lane = threadIdx.x % 32;
-    if (row == 0) kv_check_offsets(batch, error);
-    uint32_t seq, node;
-    if (!kv_row(batch, row, lane, seq, node)) return;
-    const bool q8 = cache.type == TSP_TYPE_Q8_0;
-    const uint64_t slot = static_cast<uint64_t>(batch.d_lengths[seq]) + node;
-    const uint32_t t = slot % kKvGroup, hb = kv_half_bytes(D, q8), x0 = lane * NV;
-    for (uint32_t h = threadIdx.x / 32; h < 2 * cache.kv_heads; h += 8) {
-        const bool is_v = h >= cache.kv_heads;
-        const uint32_t head = is_v ? h - cache.kv_heads : h;
-        uint8_t* out = is_v ? v : k;
-        if (!out) continue;
-        out += row * (is_v ? v_stride : k_stride) + head * D * (OUT16 ? 2 : 4);
-        const uint8_t* part = kv_group(cache, seq, slot, head, error);
-        if (!part) continue;
-        part += is_v ? hb : 0;
-        const float d = q8 ? __half2float(*reinterpret_cast<const __half*>(part + kv_scale_byte(x0, t, D))) : 1.f;
+    constexpr uint32_t ES = OUT16 ? 2 : 4, HALF = kv_half_bytes(D, Q8), ROWS = Q8 ? D / 32 : D / 16;   // 512-byte rows of K's (and V's) values
+    const uint32_t lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+    if (blockIdx.x == 0) kv_check_offsets(batch, error);
+    const uint32_t task = blockIdx.x * 8 + threadIdx.x / 32, place = task / cache.kv_heads, head = task % cache.kv_heads;
+    uint32_t seq, row0, mask;
+    uint64_t slot0;
+    if (place >= kv_group_places(batch.rows, batch.sequences) || !kv_group_of_place(batch, place, lane, seq, slot0, row0, mask)) return;
+    const uint8_t* group = kv_group(cache, seq, slot0, head, error);
+    if (!group) return;
+    uint4 wk[ROWS], wv[ROWS];
+    if (k)
 #pragma unroll
-        for (uint32_t i = 0; i < NV; ++i) {
-            const uint8_t* p = part + (is_v ? kv_v_byte(x0 + i, t, q8) : kv_k_byte(x0 + i, t, q8));
-            const float y = q8 ? static_cast<float>(static_cast<int>(*p) - 128) * d : __half2float(*reinterpret_cast<const __half*>(p));
-            if constexpr (OUT16) reinterpret_cast<__half*>(out)[x0 + i] = __float2half_rn(y);
-            else reinterpret_cast<float*>(out)[x0 + i] = y;
+        for (uint32_t i = 0; i < ROWS; ++i) wk[i] = reinterpret_cast<const uint4*>(group)[i * 32 + lane];
+    if (v)
+#pragma unroll
+        for (uint32_t i = 0; i < ROWS; ++i) wv[i] = reinterpret_cast<const uint4*>(group + HALF)[i * 32 + lane];
+    const bool on[2] = {(mask >> g & 1) != 0, (mask >> (g + 8) & 1) != 0};
+    if (k) {
+        uint8_t* base = k + head * D * ES;
+        const __half* scales = reinterpret_cast<const __half*>(group + kKvGroup * D);
+#pragma unroll
+        for (uint32_t i = 0; i < ROWS; ++i) {   // Q8: 64 dims (i / 2), slots 8 (i % 2) + g, dims 8 t of both halves; F16: 32 dims, 8 dims
+            const uint32_t slot = i % 2 * 8 + g;
+            if (!on[i % 2]) continue;
+            uint8_t* row = base + static_cast<uint64_t>(row0 + slot) * k_stride;
+            if constexpr (Q8) {
+                float x[8];
+                values_of(wk[i].x, wk[i].y, __half2float(scales[(i / 2 * 2) * kKvGroup + slot]), x);
+                store8<D, OUT16>(row, i / 2 * 64 + 8 * t, x);
+                values_of(wk[i].z, wk[i].w, __half2float(scales[(i / 2 * 2 + 1) * kKvGroup + slot]), x);
+                store8<D, OUT16>(row, i / 2 * 64 + 32 + 8 * t, x);
+            } else {
+                const uint32_t x = i / 2 * 32 + 8 * t;
+                if constexpr (OUT16) *reinterpret_cast<uint4*>(row + x * 2) = wk[i];
+                else {
+                    float y[8];
+                    const uint32_t w[4] = {wk[i].x, wk[i].y, wk[i].z, wk[i].w};
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) { const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j])); y[2 * j] = f.x; y[2 * j + 1] = f.y; }
+                    store8<D, OUT16>(row, x, y);
+                }
+            }
+        }
+    }
+    if (v) {
+        uint8_t* base = v + head * D * ES;
+        const __half* scales = reinterpret_cast<const __half*>(group + HALF + kKvGroup * D);
+#pragma unroll
+        for (uint32_t b = 0; b < D / 32; ++b) {
+            uint32_t h[4][2];   // [i][slots 2t, 2t + 1 | 8 more] of dim 8 i + g; transposed: [i][slot g | g + 8] of dims 8 i + 2 t, + 1
+            if constexpr (Q8) {
+                const uint32_t w[4] = {wv[b].x, wv[b].y, wv[b].z, wv[b].w};
+                const __half2 bias = __half2half2(__ushort_as_half(0x6480));   // 1152
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const uint32_t x = __byte_perm(w[i], 0x64646464u, 0x4140), y = __byte_perm(w[i], 0x64646464u, 0x4342);
+                    const __half2 p = __hsub2(*reinterpret_cast<const __half2*>(&x), bias), q = __hsub2(*reinterpret_cast<const __half2*>(&y), bias);
+                    h[i][0] = *reinterpret_cast<const uint32_t*>(&p); h[i][1] = *reinterpret_cast<const uint32_t*>(&q);
+                }
+            } else {
+                const uint4 x = wv[2 * b % ROWS], y = wv[(2 * b + 1) % ROWS];
+                h[0][0] = x.x; h[0][1] = x.y; h[1][0] = x.z; h[1][1] = x.w; h[2][0] = y.x; h[2][1] = y.y; h[3][0] = y.z; h[3][1] = y.w;
+            }
+#pragma unroll
+            for (uint32_t n = 0; n < 2; ++n) {
+                const uint32_t slot = g + 8 * n;
+                const float d = Q8 ? __half2float(scales[b * kKvGroup + slot]) : 1.f;
+                uint32_t o[4];
+                float2 f[4];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    o[i] = transposed(h[i][n]);
+                    f[i] = __half22float2(*reinterpret_cast<const __half2*>(&o[i]));
+                    if constexpr (Q8) { f[i].x *= d; f[i].y *= d; o[i] = half2_bits(f[i].x, f[i].y); }
+                }
+                uint8_t* row = base + static_cast<uint64_t>(row0 + slot) * v_stride;
+                if constexpr (OUT16) {   // neighbouring lanes swap, so that a lane has four dims in a row and four lanes a 32-byte sector
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; i += 2) {
+                        const uint32_t got = __shfl_xor_sync(0xffffffffu, t & 1 ? o[i] : o[i + 1], 1);
+                        if (on[n]) *reinterpret_cast<uint2*>(row + (32 * b + 8 * (i + (t & 1)) + t / 2 * 4) * 2) = t & 1 ? make_uint2(got, o[i + 1]) : make_uint2(o[i], got);
+                    }
+                } else if (on[n]) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) *reinterpret_cast<float2*>(row + (32 * b + 8 * i + 2 * t) * 4) = f[i];
+                }
+            }
         }
     }
 }
@@ -312,11 +523,19 @@ cache_keep_kernel(const tsp_kv_cache cache, const tsp_kv_batch batch, const uint
     }
 }
 
+static uint32_t value_blocks(const tsp_kv_cache& c, const tsp_kv_batch& b) {
+    return (kv_group_places(b.rows, b.sequences) * c.kv_heads + kHeadThreads / 32 - 1) / (kHeadThreads / 32);
+}
+
 template <uint32_t D, bool IN16, bool OUT16>
 static int launch_head_rows_d(const tsp_qk_norm_rope_args& a, const HeadRows& r, const tsp_kv_cache* cache, const tsp_kv_batch* batch, uint32_t rows, uint32_t* error,
                               cudaStream_t st) {
-    if (cache) TSP_CUDA(launch_pdl(head_rows_kernel<D, IN16, OUT16, true>, dim3(rows), dim3(kHeadThreads), 0, st, a, r, *cache, *batch, error));
-    else TSP_CUDA(launch_pdl(head_rows_kernel<D, IN16, OUT16, false>, dim3(rows), dim3(kHeadThreads), 0, st, a, r, tsp_kv_cache{}, tsp_kv_batch{}, error));
+    if (cache) TSP_CUDA(launch_pdl(head_rows_kernel<D, IN16, OUT16, true>, dim3(rows + value_blocks(*cache, *batch)), dim3(kHeadThreads), 0, st, a, r, *cache, *batch, error));
+    else {
+        // two heads' worth of lanes in flight a thread at most, as few idle ones as that allows: 40 heads of 128 dims in two passes of 320 threads
+        const uint32_t lanes = (r.q_heads + r.kv_heads) * (D / 8), passes = (lanes + 511) / 512, threads = ((lanes + passes - 1) / passes + 31) / 32 * 32;
+        TSP_CUDA(launch_pdl(head_rows_kernel<D, IN16, OUT16, false>, dim3(rows), dim3(threads), 0, st, a, r, tsp_kv_cache{}, tsp_kv_batch{}, error));
+    }
     return TSP_OK;
 }
 
@@ -337,13 +556,22 @@ int launch_head_rows(const tsp_qk_norm_rope_args& a, const void* q, uint64_t q_s
                                : launch_head_rows_t<256>(a, r, in_dtype, out_dtype, cache, batch, rows, error, st);
 }
 
+template <uint32_t D>
+static int launch_cache_read_d(const tsp_kv_cache& cache, const tsp_kv_batch& batch, uint8_t* k, uint64_t k_stride, uint8_t* v, uint64_t v_stride, bool out16, uint32_t* error,
+                               cudaStream_t st) {
+    const bool q8 = cache.type == TSP_TYPE_Q8_0;
+    auto kernel = q8 ? (out16 ? cache_read_kernel<D, true, true> : cache_read_kernel<D, false, true>) : (out16 ? cache_read_kernel<D, true, false> : cache_read_kernel<D, false, false>);
+    const uint32_t tasks = kv_group_places(batch.rows, batch.sequences) * cache.kv_heads;
+    TSP_CUDA(launch_pdl(kernel, dim3((tasks + 7) / 8), dim3(256), 0, st, cache, batch, k, k_stride, v, v_stride, error));
+    return TSP_OK;
+}
+
 int launch_cache_read(const tsp_kv_cache& cache, const tsp_kv_batch& batch, void* k, uint64_t k_stride, void* v, uint64_t v_stride, uint32_t dtype, uint32_t* error,
                       cudaStream_t st) {
-    auto kernel = cache.head_dim == 64    ? (dtype ? cache_read_kernel<64, true> : cache_read_kernel<64, false>)
-                  : cache.head_dim == 128 ? (dtype ? cache_read_kernel<128, true> : cache_read_kernel<128, false>)
-                                          : (dtype ? cache_read_kernel<256, true> : cache_read_kernel<256, false>);
-    TSP_CUDA(launch_pdl(kernel, dim3(batch.rows), dim3(256), 0, st, cache, batch, static_cast<uint8_t*>(k), k_stride, static_cast<uint8_t*>(v), v_stride, error));
-    return TSP_OK;
+    uint8_t *kb = static_cast<uint8_t*>(k), *vb = static_cast<uint8_t*>(v);
+    return cache.head_dim == 64    ? launch_cache_read_d<64>(cache, batch, kb, k_stride, vb, v_stride, dtype, error, st)
+           : cache.head_dim == 128 ? launch_cache_read_d<128>(cache, batch, kb, k_stride, vb, v_stride, dtype, error, st)
+                                   : launch_cache_read_d<256>(cache, batch, kb, k_stride, vb, v_stride, dtype, error, st);
 }
 
 int launch_cache_keep(const tsp_kv_cache& cache, const tsp_kv_batch& batch, const uint32_t* accepted, const uint32_t* counts, uint32_t* error, cudaStream_t st) {
