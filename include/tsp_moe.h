@@ -299,7 +299,7 @@ typedef struct tsp_kv_batch {
 #define TSP_ROPE_HALVES 0u
 #define TSP_ROPE_PAIRS 1u
 typedef struct tsp_qk_norm_rope_args {
-    const float* d_q_norm;       /* [head_dim] or NULL */
+    const float* d_q_norm;       /* [head_dim], 16-byte aligned, or NULL */
     const float* d_k_norm;
     const float* d_inv_freq;     /* [rotary_dim / 2]; may be NULL when rotary_dim is 0 */
     uint32_t head_dim, rotary_dim;   /* rotary_dim a multiple of 8, <= head_dim */

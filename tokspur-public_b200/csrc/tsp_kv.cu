@@ -25,6 +25,13 @@ template <bool F16> __device__ __forceinline__ void load4(const uint8_t* p, uint
         v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
     }
 }
+template <bool F16, uint32_t N> __device__ __forceinline__ void load_run(const uint8_t* p, uint32_t i, float (&v)[N]) {   // N = 2, 4, 8 values
+#pragma unroll
+    for (uint32_t k = 0; k < N; k += N < 4 ? 2 : 4) {
+        if constexpr (N < 4) { const float2 x = load2<F16>(p, i); v[0] = x.x; v[1] = x.y; }
+        else { float x[4]; load4<F16>(p, i + k, x); for (uint32_t c = 0; c < 4; ++c) v[k + c] = x[c]; }
+    }
+}
 template <bool F16> __device__ __forceinline__ void store4(uint8_t* p, uint32_t i, const float (&v)[4]) {
     if constexpr (F16) {
         const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
@@ -36,11 +43,14 @@ template <bool F16> __device__ __forceinline__ bool fits(float v) { return F16 ?
 // y / d rounded half to even, of the exact quotient: the rounded product may be one off, or sit on the wrong side of a tie; the remainder
 // y - r d is exact (r and d have 18 bits between them, and |y - r d| <= d over a grid of 2^-24 d at least)
 template <typename T> __device__ __forceinline__ int code_of(T y, T d, T inv) {
-    const T r0 = rint(y * inv), e2 = 2 * fma(-r0, d, y);
-    int r = static_cast<int>(fmax(fmin(r0, static_cast<T>(128)), static_cast<T>(-128)));
-    if (e2 > d || (e2 == d && (r & 1))) ++r;
-    else if (e2 < -d || (e2 == -d && (r & 1))) --r;
-    return max(-127, min(127, r));
+    const T r0 = fmax(fmin(rint(y * inv), static_cast<T>(128)), static_cast<T>(-128)), e2 = 2 * fma(-r0, d, y);
+    const int r = static_cast<int>(r0), odd = r & 1;
+    return max(-127, min(127, r + (e2 > d || (odd && e2 == d)) - (e2 < -d || (odd && e2 == -d))));
+}
+__device__ __forceinline__ float reciprocal(float d) {   // for code_of(), which puts right what this leaves; d is a binary16 number above 0
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+    return r;
 }
 
 // One head of K (a warp, lane l holds dims l NV .. l NV + NV - 1) into its slot. Returns false where it wrote zeros for it.
@@ -55,10 +65,11 @@ __device__ __forceinline__ bool put_keys(uint8_t* half, uint32_t t, bool q8, uin
         for (uint32_t i = 0; i < NV; ++i) { ok &= finite_f32(static_cast<float>(y[i])); top = fmax(top, fabs(y[i])); }
 #pragma unroll
         for (uint32_t o = 1; o < 32 / NV; o *= 2) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const __half d16 = __float2half_rn(static_cast<float>(top / 127.0));
+        const __half d16 = __float2half_rn(static_cast<float>(top * (1.0 / 127.0)));
         ok &= !__hisinf(d16);
         ok = __all_sync(0xffffffffu, ok);
-        const double d = ok ? static_cast<double>(__half2float(d16)) : 0, inv = d > 0 ? 1 / d : 0;
+        const float d32 = ok ? __half2float(d16) : 0.f;
+        const double d = d32, inv = d32 > 0.f ? reciprocal(d32) : 0.f;
         uint8_t code[NV];
 #pragma unroll
         for (uint32_t i = 0; i < NV; ++i) code[i] = static_cast<uint8_t>(d > 0 ? code_of<double>(y[i], d, inv) + 128 : 128);
@@ -104,7 +115,7 @@ __device__ __forceinline__ bool put_values(uint8_t* half, uint32_t rows, bool q8
 #pragma unroll
     for (uint32_t n = 0; n < 2; ++n) {
         if (on[n]) {
-#pragma unroll
+#pragma unroll 1
             for (uint32_t b = 0; b < D / 32; ++b)
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) {
@@ -119,7 +130,8 @@ __device__ __forceinline__ bool put_values(uint8_t* half, uint32_t rows, bool q8
         ok[n] = v != 0;
         fine &= ok[n];
     }
-#pragma unroll
+    // rolled: a step of a few rows waits for its instructions (unrolled, 24 rows took 13 us, half of it for those)
+#pragma unroll 1
     for (uint32_t b = 0; b < D / 32; ++b) {
         float v[2][8];
         uint32_t out[4][2];   // [i][slots 2t, 2t + 1 | 8 more]: binary16 values, or codes
@@ -135,8 +147,8 @@ __device__ __forceinline__ bool put_values(uint8_t* half, uint32_t rows, bool q8
             if (q8) {
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const __half d16 = __float2half_rn(static_cast<float>(static_cast<double>(top) / 127.0));
-                const float d = __half2float(d16), inv = d > 0.f ? 1.f / d : 0.f;
+                const __half d16 = __float2half_rn(top / 127.f);
+                const float d = __half2float(d16), inv = d > 0.f ? reciprocal(d) : 0.f;
 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i) v[n][i] = d > 0.f ? static_cast<float>(code_of<float>(v[n][i], d, inv)) : 0.f;
                 if (on[n] && t == 0) *reinterpret_cast<__half*>(half + kv_scale_byte(32 * b, g + 8 * n, D)) = d16;
@@ -208,155 +220,180 @@ struct HeadRows {
     uint32_t q_heads, kv_heads;   // kv_heads: of k_out (no cache)
 };
 
-// A block per row. Angles once per row; then eight lanes' worth of pairs per group of D / 8 lanes for the rows that go out as rows, a warp per
-// head for those that go into the cache.
-template <uint32_t D, bool IN16, bool OUT16, bool CACHE>
-__global__ void __launch_bounds__(CACHE ? kHeadThreads : 512)
-head_rows_kernel(const tsp_qk_norm_rope_args a, const HeadRows r, const tsp_kv_cache cache, const tsp_kv_batch batch, uint32_t* error) {
-    __shared__ float cs[D / 2], sn[D / 2];
-    __shared__ double cs64[CACHE ? D / 2 : 1], sn64[CACHE ? D / 2 : 1];
-    __shared__ double exchange[CACHE ? kHeadThreads / 32 : 1][CACHE ? D : 1];
-    pdl_launch_dependents();
-    pdl_wait();
-    const uint32_t row = blockIdx.x, tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-    uint32_t seq = 0, node = 0;
-    if constexpr (CACHE) {
-        if (row == 0) kv_check_offsets(batch, error);
-        if (row >= batch.rows) {   // the blocks behind the rows': values, a warp per group of slots and head
-            const uint32_t task = (row - batch.rows) * (kHeadThreads / 32) + warp, place = task / cache.kv_heads, head = task % cache.kv_heads;
-            uint64_t slot0;
-            uint32_t row0, mask;
-            if (place >= kv_group_places(batch.rows, batch.sequences) || !kv_group_of_place(batch, place, lane, seq, slot0, row0, mask)) return;
-            const bool q8 = cache.type == TSP_TYPE_Q8_0;
-            uint8_t* group = kv_group(cache, seq, slot0, head, error);
-            if (!group) return;
-            const bool fine = put_values<D, IN16>(group + kv_half_bytes(D, q8), mask, q8, lane,
-                                                  [&](uint32_t t) { return r.v + static_cast<uint64_t>(row0 + t) * r.v_stride + head * D * (IN16 ? 2u : 4u); });
-            if (!fine) raise_error(error, TSP_ERR_NONFINITE);
-            return;
-        }
-        if (!kv_row(batch, row, lane, seq, node)) return;
-    }
-    const uint32_t half = a.rotary_dim / 2;
+// Blocks of three kinds. Rows that go out as rows: a block has as many heads as its threads take at eight dims each, and walks every `stride`-th row with
+// them, the next row's values under way and its angles computed (in the other half of the buffer) while one is turned. Keys that go into
+// the cache: a block per row, a warp per head. Values that do: a warp per group of 16 slots and head.
+template <uint32_t D, bool IN16, bool OUT16>
+__device__ __forceinline__ void turn_rows(const tsp_qk_norm_rope_args& a, const HeadRows& r, uint32_t pass, uint32_t row, uint32_t stride, uint32_t end, uint32_t* error) {
+    __shared__ __align__(16) float cs[2][D / 2], sn[2][D / 2];
     constexpr uint32_t LANES = D / 8;   // lanes of a head
-    const uint32_t per = blockDim.x / LANES, out_heads = r.q_heads + (CACHE ? 0 : r.kv_heads), passes = (out_heads + per - 1) / per, l = tid % LANES;
+    const uint32_t tid = threadIdx.x, lane = tid % 32, half = a.rotary_dim / 2, heads = r.q_heads + r.kv_heads, l = tid % LANES;
+    const uint32_t h0 = pass * (blockDim.x / LANES) + tid / LANES, h = min(h0, heads - 1);   // a lane behind the last head takes that one again: whole warps shuffle
     // four pairs a lane: (u, v) at dims xu.., xv.., or interleaved in eight dims from xu on; the dims behind the rotated ones pair up as halves
     const uint32_t p0 = 4 * l, rest = p0 - half;
-    const bool turned = p0 < half, pairs = turned && a.style == TSP_ROPE_PAIRS;
+    const bool turned = p0 < half, pairs = turned && a.style == TSP_ROPE_PAIRS, is_k = h >= r.q_heads;
     const uint32_t xu = turned ? (pairs ? 2 * p0 : p0) : a.rotary_dim + rest, xv = turned ? (pairs ? xu + 4 : p0 + half) : xu + (D - a.rotary_dim) / 2;
-    float u[4], v[4];
-    auto load = [&](uint32_t pass) {   // whole warps stay together for the shuffles: a lane behind the last head takes that one again
-        const uint32_t h = min(pass * per + tid / LANES, out_heads - 1);
-        const uint8_t* in = h >= r.q_heads ? r.k + row * r.k_stride + (h - r.q_heads) * D * (IN16 ? 2 : 4) : r.q + row * r.q_stride + h * D * (IN16 ? 2 : 4);
-        load4<IN16>(in, xu, u);
-        load4<IN16>(in, xv, v);
-    };
-    if (passes) load(0);   // under way while the angles are computed
-    if (half) {
-        const double pos = r.positions[row];
-        for (uint32_t p = tid; p < half; p += blockDim.x) {
-            const double angle = pos * static_cast<double>(a.d_inv_freq[p]);
-            if constexpr (CACHE) {
-                double s, c;
-                sincos(angle, &s, &c);
-                c *= a.magnitude; s *= a.magnitude;
-                cs[p] = static_cast<float>(c); sn[p] = static_cast<float>(s);
-                cs64[p] = c; sn64[p] = s;
-            } else {   // turns, reduced in 64 bits
-                const double turns = angle * 0.15915494309189535;
-                float s, c;
-                sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &c);
-                cs[p] = c * a.magnitude; sn[p] = s * a.magnitude;
-            }
-        }
-        __syncthreads();
+    const uint32_t hh = is_k ? h - r.q_heads : h;
+    const uint8_t* in = (is_k ? r.k : r.q) + hh * D * (IN16 ? 2u : 4u);
+    uint8_t* out = (is_k ? r.k_out : r.q_out) + hh * D * (OUT16 ? 2u : 4u);
+    const uint64_t in_stride = is_k ? r.k_stride : r.q_stride, out_stride = is_k ? r.k_out_stride : r.q_out_stride;
+    const float* w = is_k ? a.d_k_norm : a.d_q_norm;
+    float wu[4] = {1.f, 1.f, 1.f, 1.f}, wv[4] = {1.f, 1.f, 1.f, 1.f}, nu[4], nv[4];
+    if (w) {
+        load4<false>(reinterpret_cast<const uint8_t*>(w), xu, wu);
+        load4<false>(reinterpret_cast<const uint8_t*>(w), xv, wv);
     }
+    auto fetch = [&](uint32_t at, uint32_t buffer) {
+        const uint8_t* src = in + at * in_stride;
+        load4<IN16>(src, xu, nu);
+        load4<IN16>(src, xv, nv);
+        for (uint32_t p = tid; p < half; p += blockDim.x) {
+            const double turns = static_cast<double>(r.positions[at]) * static_cast<double>(a.d_inv_freq[p]) * 0.15915494309189535;
+            float s, c;
+            sincospif(static_cast<float>(2 * (turns - rint(turns))), &s, &c);   // half turns, reduced in 64 bits
+            cs[buffer][p] = c * a.magnitude; sn[buffer][p] = s * a.magnitude;
+        }
+    };
+    if (row < end) fetch(row, 0);
     bool bad = false;
-    for (uint32_t pass = 0; pass < passes; ++pass) {
-        const uint32_t h0 = pass * per + tid / LANES, h = min(h0, out_heads - 1);
-        if (pass) load(pass);
-        const bool is_k = h >= r.q_heads;
-        uint8_t* out = is_k ? r.k_out + row * r.k_out_stride + (h - r.q_heads) * D * (OUT16 ? 2 : 4) : r.q_out + row * r.q_out_stride + h * D * (OUT16 ? 2 : 4);
-        const float* w = is_k ? a.d_k_norm : a.d_q_norm;
-        float wu[4] = {1.f, 1.f, 1.f, 1.f}, wv[4] = {1.f, 1.f, 1.f, 1.f};
+#pragma unroll 1
+    for (uint32_t buffer = 0; row < end; row += stride, buffer ^= 1) {
+        __syncthreads();
+        float u[4], v[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) { u[i] = nu[i]; v[i] = nv[i]; }
+        if (row + stride < end) fetch(row + stride, buffer ^ 1);
         if (w) {
             float ss = 0.f;
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) ss = fmaf(u[i], u[i], fmaf(v[i], v[i], ss));
 #pragma unroll
             for (uint32_t o = LANES / 2; o; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const float inv = 1.f / sqrtf(ss * (1.f / D) + a.eps);
+            const float inv = rsqrtf(ss * (1.f / D) + a.eps);
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) { wu[i] = w[xu + i]; wv[i] = w[xv + i]; u[i] = u[i] * inv * wu[i]; v[i] = v[i] * inv * wv[i]; }
+            for (uint32_t i = 0; i < 4; ++i) { u[i] = u[i] * inv * wu[i]; v[i] = v[i] * inv * wv[i]; }
         }
         if (turned) {
+            const float4 c4 = *reinterpret_cast<const float4*>(cs[buffer] + p0), n4 = *reinterpret_cast<const float4*>(sn[buffer] + p0);
+            const float c[4] = {c4.x, c4.y, c4.z, c4.w}, n[4] = {n4.x, n4.y, n4.z, n4.w};
             if (pairs) {
                 float t[4] = {u[0], u[2], v[0], v[2]}, s[4] = {u[1], u[3], v[1], v[3]};
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) { const float c = cs[p0 + i], n = sn[p0 + i], x = t[i]; t[i] = x * c - s[i] * n; s[i] = s[i] * c + x * n; }
+                for (uint32_t i = 0; i < 4; ++i) { const float x = t[i]; t[i] = x * c[i] - s[i] * n[i]; s[i] = s[i] * c[i] + x * n[i]; }
                 u[0] = t[0]; u[1] = s[0]; u[2] = t[1]; u[3] = s[1]; v[0] = t[2]; v[1] = s[2]; v[2] = t[3]; v[3] = s[3];
             } else {
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) { const float c = cs[p0 + i], n = sn[p0 + i], x = u[i]; u[i] = x * c - v[i] * n; v[i] = v[i] * c + x * n; }
+                for (uint32_t i = 0; i < 4; ++i) { const float x = u[i]; u[i] = x * c[i] - v[i] * n[i]; v[i] = v[i] * c[i] + x * n[i]; }
             }
         }
-        bool ok = true;
+        // magnitudes as integers: NaN lies above infinity
+        uint32_t top = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) ok &= fits<OUT16>(u[i]) && fits<OUT16>(v[i]);
+        for (uint32_t i = 0; i < 4; ++i) top = max(top, max(__float_as_uint(u[i]) & 0x7fffffffu, __float_as_uint(v[i]) & 0x7fffffffu));
         const uint32_t group = LANES == 32 ? 0xffffffffu : ((1u << (LANES % 32)) - 1) << (lane / LANES * LANES);
-        ok = (__ballot_sync(0xffffffffu, ok) & group) == group;
+        const bool ok = (__ballot_sync(0xffffffffu, top < (OUT16 ? 0x477ff000u : 0x7f800000u)) & group) == group;   // 65520 rounds to infinity in binary16
         if (!ok) {
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) u[i] = v[i] = 0.f;
         }
-        if (h0 < out_heads) {
+        if (h0 < heads) {
             bad |= !ok;
-            store4<OUT16>(out, xu, u);
-            store4<OUT16>(out, xv, v);
+            uint8_t* dst = out + row * out_stride;
+            store4<OUT16>(dst, xu, u);
+            store4<OUT16>(dst, xv, v);
         }
     }
-    if constexpr (CACHE) {
-        constexpr uint32_t NV = D / 32;
-        const bool q8 = cache.type == TSP_TYPE_Q8_0;
-        const uint64_t slot = static_cast<uint64_t>(batch.d_lengths[seq]) + node;
-        const uint32_t t = slot % kKvGroup;
-        for (uint32_t h = warp; h < cache.kv_heads; h += kHeadThreads / 32) {
-            uint8_t* group = kv_group(cache, seq, slot, h, error);
-            if (!group) continue;
-            const uint8_t* in = r.k + row * r.k_stride + h * D * (IN16 ? 2 : 4);
-            {
-                double y[NV];
+    if (bad) raise_error(error, TSP_ERR_NONFINITE);
+}
+
+template <uint32_t D, bool IN16, bool OUT16>
+__global__ void __launch_bounds__(512)
+turn_rows_kernel(const tsp_qk_norm_rope_args a, const HeadRows r, uint32_t passes, uint32_t rows, uint32_t* error) {
+    pdl_launch_dependents();
+    pdl_wait();
+    turn_rows<D, IN16, OUT16>(a, r, blockIdx.x % passes, blockIdx.x / passes, gridDim.x / passes, rows, error);
+}
+
+// Grid: value blocks, a key block per row, then `turning` blocks of `passes` each for the query rows
+template <uint32_t D, bool IN16, bool OUT16>
+__global__ void __launch_bounds__(kHeadThreads)
+append_rows_kernel(const tsp_qk_norm_rope_args a, const HeadRows r, const tsp_kv_cache cache, const tsp_kv_batch batch, uint32_t values, uint32_t passes, uint32_t* error) {
+    __shared__ double cs[D / 2], sn[D / 2], exchange[kHeadThreads / 32][D];
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+    const bool q8 = cache.type == TSP_TYPE_Q8_0;
+    if (blockIdx.x == 0) kv_check_offsets(batch, error);
+    if (blockIdx.x >= values + batch.rows) {
+        const uint32_t block = blockIdx.x - values - batch.rows, blocks = gridDim.x - values - batch.rows;
+        turn_rows<D, IN16, OUT16>(a, r, block % passes, block / passes, blocks / passes, min(batch.rows, batch.d_row_offsets[batch.sequences]), error);
+        return;
+    }
+    uint32_t seq, node;
+    if (blockIdx.x < values) {
+        const uint32_t task = blockIdx.x * (kHeadThreads / 32) + warp, place = task / cache.kv_heads, head = task % cache.kv_heads;
+        uint64_t slot0;
+        uint32_t row0, mask;
+        if (place >= kv_group_places(batch.rows, batch.sequences) || !kv_group_of_place(batch, place, lane, seq, slot0, row0, mask)) return;
+        uint8_t* group = kv_group(cache, seq, slot0, head, error);
+        if (!group) return;
+        const bool fine = put_values<D, IN16>(group + kv_half_bytes(D, q8), mask, q8, lane,
+                                              [&](uint32_t t) { return r.v + static_cast<uint64_t>(row0 + t) * r.v_stride + head * D * (IN16 ? 2u : 4u); });
+        if (!fine) raise_error(error, TSP_ERR_NONFINITE);
+        return;
+    }
+    constexpr uint32_t NV = D / 32;
+    const uint32_t row = blockIdx.x - values, half = a.rotary_dim / 2;
+    float key[NV];
+    if (warp < cache.kv_heads) load_run<IN16>(r.k + row * r.k_stride + warp * D * (IN16 ? 2u : 4u), lane * NV, key);
+    if (!kv_row(batch, row, lane, seq, node)) return;
+    if (half) {
+        const double pos = r.positions[row];
+        for (uint32_t p = tid; p < half; p += kHeadThreads) {
+            const double turns = pos * static_cast<double>(a.d_inv_freq[p]) * 0.15915494309189535;
+            double s, c;
+            sincospi(2 * (turns - rint(turns)), &s, &c);
+            cs[p] = c * a.magnitude; sn[p] = s * a.magnitude;
+        }
+        __syncthreads();
+    }
+    bool bad = false;
+    const uint64_t slot = static_cast<uint64_t>(batch.d_lengths[seq]) + node;
+#pragma unroll 1
+    for (uint32_t h = warp; h < cache.kv_heads; h += kHeadThreads / 32) {
+        uint8_t* group = kv_group(cache, seq, slot, h, error);
+        if (!group) continue;
+        if (h >= kHeadThreads / 32) load_run<IN16>(r.k + row * r.k_stride + h * D * (IN16 ? 2u : 4u), lane * NV, key);
+        double y[NV];
 #pragma unroll
-                for (uint32_t i = 0; i < NV; ++i) y[i] = load1<IN16>(in, lane * NV + i);
-                if (a.d_k_norm) {
-                    double ss = 0;
+        for (uint32_t i = 0; i < NV; ++i) y[i] = key[i];
+        if (a.d_k_norm) {
+            double ss = 0;
 #pragma unroll
-                    for (uint32_t i = 0; i < NV; ++i) ss = fma(y[i], y[i], ss);
+            for (uint32_t i = 0; i < NV; ++i) ss = fma(y[i], y[i], ss);
 #pragma unroll
-                    for (uint32_t o = 16; o; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                    const double inv = 1.0 / sqrt(ss / D + static_cast<double>(a.eps));
+            for (uint32_t o = 16; o; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const double inv = rsqrt(ss * (1.0 / D) + static_cast<double>(a.eps));
 #pragma unroll
-                    for (uint32_t i = 0; i < NV; ++i) y[i] = y[i] * inv * static_cast<double>(a.d_k_norm[lane * NV + i]);
+            for (uint32_t i = 0; i < NV; ++i) y[i] = y[i] * inv * static_cast<double>(a.d_k_norm[lane * NV + i]);
+        }
+        if (half) {
+            double* mine = exchange[warp];
+            __syncwarp();
+#pragma unroll
+            for (uint32_t i = 0; i < NV; ++i) mine[lane * NV + i] = y[i];
+            __syncwarp();
+#pragma unroll
+            for (uint32_t i = 0; i < NV; ++i) {
+                const uint32_t x = lane * NV + i;
+                if (x < a.rotary_dim) {
+                    const bool pairs = a.style == TSP_ROPE_PAIRS, second = pairs ? x & 1 : x >= half;
+                    const uint32_t p = pairs ? x / 2 : (second ? x - half : x), other = pairs ? x ^ 1 : (second ? x - half : x + half);
+                    y[i] = y[i] * cs[p] + mine[other] * (second ? sn[p] : -sn[p]);
                 }
-                if (half) {
-                    double* mine = exchange[warp];
-                    __syncwarp();
-#pragma unroll
-                    for (uint32_t i = 0; i < NV; ++i) mine[lane * NV + i] = y[i];
-                    __syncwarp();
-#pragma unroll
-                    for (uint32_t i = 0; i < NV; ++i) {
-                        const uint32_t x = lane * NV + i;
-                        if (x < a.rotary_dim) {
-                            const bool pairs = a.style == TSP_ROPE_PAIRS, second = pairs ? x & 1 : x >= half;
-                            const uint32_t p = pairs ? x / 2 : (second ? x - half : x), other = pairs ? x ^ 1 : (second ? x - half : x + half);
-                            y[i] = second ? y[i] * cs64[p] + mine[other] * sn64[p] : y[i] * cs64[p] - mine[other] * sn64[p];
-                        }
-                    }
-                }
-                bad |= !put_keys<D>(group, t, q8, lane, y);
             }
         }
+        bad |= !put_keys<D>(group, slot % kKvGroup, q8, lane, y);
     }
     if (bad) raise_error(error, TSP_ERR_NONFINITE);
 }
@@ -472,50 +509,60 @@ cache_read_kernel(const tsp_kv_cache cache, const tsp_kv_batch batch, uint8_t* k
     }
 }
 
-// A block per (sequence, head): every source row is in shared memory before the first destination is written (a destination may be a
-// later row's source only through an index below it, which ascending indices rule out, but rows move in parallel here).
+// A block per (sequence, head): every source slot is in shared memory before the first destination is written. Pieces of a slot: 16 bytes of K, the four
+// bytes (two halves) of V that a group of its 512-byte rows has of the slot, scales.
+template <uint32_t D, bool Q8>
 __global__ void __launch_bounds__(256)
 cache_keep_kernel(const tsp_kv_cache cache, const tsp_kv_batch batch, const uint32_t* accepted, const uint32_t* counts, uint32_t* error) {
-    extern __shared__ uint8_t staged[];
+    constexpr uint32_t KP = D * (Q8 ? 1 : 2) / 16, VP = Q8 ? D / 4 : D / 2, SP = Q8 ? D / 16 : 0, PER = KP + VP + SP, HALF = kv_half_bytes(D, Q8);
+    extern __shared__ uint4 staged[];   // [slots][KP] K, then words [slots][VP] V, then halves [slots][SP]
+    __shared__ uint8_t* place[2][TSP_KV_MAX_DRAFT];   // groups of sources and destinations
     __shared__ uint32_t from[TSP_KV_MAX_DRAFT];
     pdl_launch_dependents();
     pdl_wait();
     const uint32_t s = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
     if (s == 0 && h == 0) kv_check_offsets(batch, error);
     const uint32_t first = batch.d_row_offsets[s], end = batch.d_row_offsets[s + 1], n = counts[s];
-    if (n == 0) return;
-    const bool q8 = cache.type == TSP_TYPE_Q8_0;
     const uint64_t length = batch.d_lengths[s];
+    if (n == 0) return;
     bool bad = end < first || end > batch.rows || n > TSP_KV_MAX_DRAFT || n > end - first;
     if (!bad && tid < n) {
         const uint32_t x = accepted[first + tid];
         bad = x >= end - first || (tid && accepted[first + tid - 1] >= x);
         from[tid] = x;
+        if (!bad) {
+            place[0][tid] = kv_group(cache, s, length + x, h, error);
+            place[1][tid] = kv_group(cache, s, length + tid, h, error);
+            bad = !place[0][tid] || !place[1][tid];
+        }
     }
     if (__syncthreads_or(bad)) { if (tid == 0) raise_error(error, TSP_ERR_INDEX); return; }
-    const uint32_t dim = cache.head_dim, row_bytes = q8 ? 2 * (dim + dim / 16) : 4 * dim, hb = kv_half_bytes(dim, q8);
-    // every page that is read or written exists
-    if (tid < n) bad = !kv_group(cache, s, length + from[tid], h, error) || !kv_group(cache, s, length + tid, h, error);
-    if (__syncthreads_or(bad)) return;
-    const uint32_t unit = q8 ? 1 : 2, values = dim * 2, per = values + (q8 ? dim / 16 : 0);   // values of K and V, then scales
-    for (int pass = 0; pass < 2; ++pass) {
-        for (uint32_t i = tid; i < n * per; i += 256) {
-            const uint32_t j = i / per, c = i % per;
-            const uint64_t slot = length + (pass ? j : from[j]);
-            uint8_t* part = kv_group(cache, s, slot, h, error);
-            const uint32_t t = slot % kKvGroup;
-            uint8_t* mine = staged + j * row_bytes;
-            if (c < values) {
-                const bool is_v = c >= dim;
-                const uint32_t x = is_v ? c - dim : c;
-                uint8_t* p = part + (is_v ? hb + kv_v_byte(x, t, q8) : kv_k_byte(x, t, q8));
-                if (q8) { if (pass) *p = mine[c]; else mine[c] = *p; }
-                else if (pass) *reinterpret_cast<uint16_t*>(p) = reinterpret_cast<uint16_t*>(mine)[c];
-                else reinterpret_cast<uint16_t*>(mine)[c] = *reinterpret_cast<uint16_t*>(p);
+    uint32_t* words = reinterpret_cast<uint32_t*>(staged + n * KP);
+    uint16_t* halves = reinterpret_cast<uint16_t*>(words + n * VP);
+#pragma unroll 1
+    for (uint32_t pass = 0; pass < 2; ++pass) {
+#pragma unroll 1
+        for (uint32_t i = tid; i < n * PER; i += 256) {
+            const uint32_t j = i / PER, c = i % PER, t = static_cast<uint32_t>((length + (pass ? j : from[j])) % kKvGroup), lane = t % 8 / 2, e = t % 2 + t / 8 * 2;
+            uint8_t* group = place[pass][j];
+            if (c < KP) {
+                uint4 *p = reinterpret_cast<uint4*>(group + (c / 4 * kKvGroup + t) * 64 + c % 4 * 16), *m = staged + j * KP + c;
+                if (pass) *p = *m; else *m = *p;
+            } else if (c < KP + VP) {
+                const uint32_t u = c - KP;
+                uint8_t* p = group + HALF + (u * 4 + lane) * 16;
+                uint32_t* m = words + j * VP + u;
+                if constexpr (Q8) {
+                    if (pass) { const uint32_t w = *m; p[e] = w; p[4 + e] = w >> 8; p[8 + e] = w >> 16; p[12 + e] = w >> 24; }
+                    else *m = p[e] | p[4 + e] << 8 | p[8 + e] << 16 | static_cast<uint32_t>(p[12 + e]) << 24;
+                } else {
+                    uint16_t* q = reinterpret_cast<uint16_t*>(p);
+                    if (pass) { const uint32_t w = *m; q[e] = w; q[4 + e] = w >> 16; }
+                    else *m = q[e] | static_cast<uint32_t>(q[4 + e]) << 16;
+                }
             } else {
-                const uint32_t b = c - values, is_v = b >= dim / 32;
-                uint16_t* p = reinterpret_cast<uint16_t*>(part + (is_v ? hb : 0) + kv_scale_byte((is_v ? b - dim / 32 : b) * 32, t, dim));
-                uint16_t* m = reinterpret_cast<uint16_t*>(mine + values * unit) + b;
+                const uint32_t u = c - KP - VP, is_v = u >= D / 32;
+                uint16_t *p = reinterpret_cast<uint16_t*>(group + (is_v ? HALF : 0) + kKvGroup * D) + (u - is_v * (D / 32)) * kKvGroup + t, *m = halves + j * SP + u;
                 if (pass) *p = *m; else *m = *p;
             }
         }
@@ -530,12 +577,16 @@ static uint32_t value_blocks(const tsp_kv_cache& c, const tsp_kv_batch& b) {
 template <uint32_t D, bool IN16, bool OUT16>
 static int launch_head_rows_d(const tsp_qk_norm_rope_args& a, const HeadRows& r, const tsp_kv_cache* cache, const tsp_kv_batch* batch, uint32_t rows, uint32_t* error,
                               cudaStream_t st) {
-    if (cache) TSP_CUDA(launch_pdl(head_rows_kernel<D, IN16, OUT16, true>, dim3(rows + value_blocks(*cache, *batch)), dim3(kHeadThreads), 0, st, a, r, *cache, *batch, error));
-    else {
-        // two heads' worth of lanes in flight a thread at most, as few idle ones as that allows: 40 heads of 128 dims in two passes of 320 threads
-        const uint32_t lanes = (r.q_heads + r.kv_heads) * (D / 8), passes = (lanes + 511) / 512, threads = ((lanes + passes - 1) / passes + 31) / 32 * 32;
-        TSP_CUDA(launch_pdl(head_rows_kernel<D, IN16, OUT16, false>, dim3(rows), dim3(threads), 0, st, a, r, tsp_kv_cache{}, tsp_kv_batch{}, error));
+    const uint32_t lanes = (r.q_heads + r.kv_heads) * (D / 8), sms = static_cast<uint32_t>(sm_count() > 0 ? sm_count() : 1);
+    // a few blocks per SM walk the rows: 4096 rows of 40 heads of 128 binary16 values 16 us, a block per row 24
+    if (!cache) {   // as few idle threads as passes of at most 512 allow: 40 heads of 128 dims in two passes of 320 threads
+        const uint32_t passes = (lanes + 511) / 512, threads = ((lanes + passes - 1) / passes + 31) / 32 * 32, walkers = (sms * (2048 / threads) + passes - 1) / passes;
+        TSP_CUDA(launch_pdl(turn_rows_kernel<D, IN16, OUT16>, dim3(passes * (rows < walkers ? rows : walkers)), dim3(threads), 0, st, a, r, passes, rows, error));
+        return TSP_OK;
     }
+    const uint32_t values = value_blocks(*cache, *batch), passes = (lanes + kHeadThreads - 1) / kHeadThreads, walkers = passes ? (sms * 4 + passes - 1) / passes : 0;
+    TSP_CUDA(launch_pdl(append_rows_kernel<D, IN16, OUT16>, dim3(values + rows + passes * (rows < walkers ? rows : walkers)), dim3(kHeadThreads), 0, st, a, r, *cache,
+                        *batch, values, passes ? passes : 1u, error));
     return TSP_OK;
 }
 
@@ -574,13 +625,22 @@ int launch_cache_read(const tsp_kv_cache& cache, const tsp_kv_batch& batch, void
                                    : launch_cache_read_d<256>(cache, batch, kb, k_stride, vb, v_stride, dtype, error, st);
 }
 
+template <uint32_t D, bool Q8>
+static int launch_cache_keep_d(const tsp_kv_cache& cache, const tsp_kv_batch& batch, const uint32_t* accepted, const uint32_t* counts, uint32_t* error, cudaStream_t st) {
+    constexpr size_t smem = TSP_KV_MAX_DRAFT * (Q8 ? 2 * (D + D / 16) : 4 * D);
+    static thread_local SmemAttrCache attr;
+    TSP_CUDA(ensure_dynamic_smem(cache_keep_kernel<D, Q8>, attr, smem));
+    TSP_CUDA(launch_pdl(cache_keep_kernel<D, Q8>, dim3(batch.sequences, cache.kv_heads), dim3(256), smem, st, cache, batch, accepted, counts, error));
+    return TSP_OK;
+}
+
 int launch_cache_keep(const tsp_kv_cache& cache, const tsp_kv_batch& batch, const uint32_t* accepted, const uint32_t* counts, uint32_t* error, cudaStream_t st) {
     const bool q8 = cache.type == TSP_TYPE_Q8_0;
-    const size_t smem = TSP_KV_MAX_DRAFT * (q8 ? 2 * (cache.head_dim + cache.head_dim / 16) : 4 * cache.head_dim);
-    static thread_local SmemAttrCache attr;
-    TSP_CUDA(ensure_dynamic_smem(cache_keep_kernel, attr, smem));
-    TSP_CUDA(launch_pdl(cache_keep_kernel, dim3(batch.sequences, cache.kv_heads), dim3(256), smem, st, cache, batch, accepted, counts, error));
-    return TSP_OK;
+    switch (cache.head_dim) {
+        case 64: return q8 ? launch_cache_keep_d<64, true>(cache, batch, accepted, counts, error, st) : launch_cache_keep_d<64, false>(cache, batch, accepted, counts, error, st);
+        case 128: return q8 ? launch_cache_keep_d<128, true>(cache, batch, accepted, counts, error, st) : launch_cache_keep_d<128, false>(cache, batch, accepted, counts, error, st);
+        default: return q8 ? launch_cache_keep_d<256, true>(cache, batch, accepted, counts, error, st) : launch_cache_keep_d<256, false>(cache, batch, accepted, counts, error, st);
+    }
 }
 
 }  // namespace tsp

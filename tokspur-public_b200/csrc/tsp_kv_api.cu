@@ -47,7 +47,7 @@ static int check_turn(const tsp_qk_norm_rope_args* a) {
     TSP_REQUIRE(a->style == TSP_ROPE_HALVES || a->style == TSP_ROPE_PAIRS, "norm and rotation: unknown pairing");
     TSP_REQUIRE(a->eps >= 0.f && std::isfinite(a->eps) && std::isfinite(a->magnitude), "norm and rotation: eps or magnitude out of range");
     TSP_REQUIRE(a->rotary_dim == 0 || a->d_inv_freq, "norm and rotation: no frequencies");
-    TSP_REQUIRE(aligned4(a->d_inv_freq) && aligned4(a->d_q_norm) && aligned4(a->d_k_norm), "norm and rotation: unaligned weights or frequencies");
+    TSP_REQUIRE(aligned4(a->d_inv_freq) && aligned16(a->d_q_norm) && aligned16(a->d_k_norm), "norm and rotation: unaligned weights or frequencies");
     return TSP_OK;
 }
 
