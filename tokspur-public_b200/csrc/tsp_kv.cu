@@ -7,10 +7,6 @@ namespace tsp {
 
 constexpr uint32_t kHeadThreads = 256;
 
-template <bool F16> __device__ __forceinline__ float load1(const uint8_t* p, uint32_t i) {
-    if constexpr (F16) return __half2float(reinterpret_cast<const __half*>(p)[i]);
-    else return reinterpret_cast<const float*>(p)[i];
-}
 template <bool F16> __device__ __forceinline__ float2 load2(const uint8_t* p, uint32_t i) {
     if constexpr (F16) return __half22float2(*reinterpret_cast<const __half2*>(p + i * 2));
     else return *reinterpret_cast<const float2*>(p + i * 4);
@@ -40,14 +36,29 @@ template <bool F16> __device__ __forceinline__ void store4(uint8_t* p, uint32_t 
 }
 template <bool F16> __device__ __forceinline__ bool fits(float v) { return F16 ? fabsf(v) < 65520.f : finite_f32(v); }   // 65520 rounds to infinity in binary16
 
-// y / d rounded half to even, of the exact quotient: the rounded product may be one off, or sit on the wrong side of a tie; the remainder
-// y - r d is exact (r and d have 18 bits between them, and |y - r d| <= d over a grid of 2^-24 d at least)
-template <typename T> __device__ __forceinline__ int code_of(T y, T d, T inv) {
-    const T r0 = fmax(fmin(rint(y * inv), static_cast<T>(128)), static_cast<T>(-128)), e2 = 2 * fma(-r0, d, y);
-    const int r = static_cast<int>(r0), odd = r & 1;
-    return max(-127, min(127, r + (e2 > d || (odd && e2 == d)) - (e2 < -d || (odd && e2 == -d))));
+// N values y over d rounded half to even, of the exact quotients, within +-127. The product with an approximate reciprocal rounds to a neighbour of the
+// quotient at worst; the remainder y - r d is exact (r and d have 18 bits between them, and |y - r d| <= d over a grid of 2^-24 d at least), and
+// tells where that matters: near the middle between two codes (and where d is subnormal, so that codes pass 127), all are put right.
+template <typename T, uint32_t N> __device__ __forceinline__ void codes_of(const T (&y)[N], float d, float inv, float (&code)[N]) {
+    float far = 0.f;
+    T e[N];
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) {
+        code[i] = __fadd_rn(__fadd_rn(static_cast<float>(y[i]) * inv, 12582912.f), -12582912.f);   // to the nearest whole number
+        e[i] = fma(static_cast<T>(-code[i]), static_cast<T>(d), y[i]);
+        far = fmaxf(far, fabsf(static_cast<float>(e[i])));
+    }
+    if (far > 0.49999f * d || d < 0x1p-14f) {
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) {
+            const float r0 = fmaxf(fminf(code[i], 128.f), -128.f);
+            const T e2 = 2 * fma(static_cast<T>(-r0), static_cast<T>(d), y[i]), w = d;
+            const int r = static_cast<int>(r0), odd = r & 1;
+            code[i] = static_cast<float>(max(-127, min(127, r + (e2 > w || (odd && e2 == w)) - (e2 < -w || (odd && e2 == -w)))));
+        }
+    }
 }
-__device__ __forceinline__ float reciprocal(float d) {   // for code_of(), which puts right what this leaves; d is a binary16 number above 0
+__device__ __forceinline__ float reciprocal(float d) {   // for codes_of(); d is a binary16 number above 0
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
     return r;
@@ -69,10 +80,11 @@ __device__ __forceinline__ bool put_keys(uint8_t* half, uint32_t t, bool q8, uin
         ok &= !__hisinf(d16);
         ok = __all_sync(0xffffffffu, ok);
         const float d32 = ok ? __half2float(d16) : 0.f;
-        const double d = d32, inv = d32 > 0.f ? reciprocal(d32) : 0.f;
+        float whole[NV];
         uint8_t code[NV];
+        if (d32 > 0.f) codes_of<double, NV>(y, d32, reciprocal(d32), whole);
 #pragma unroll
-        for (uint32_t i = 0; i < NV; ++i) code[i] = static_cast<uint8_t>(d > 0 ? code_of<double>(y[i], d, inv) + 128 : 128);
+        for (uint32_t i = 0; i < NV; ++i) code[i] = static_cast<uint8_t>(d32 > 0.f ? static_cast<int>(whole[i]) + 128 : 128);
         uint8_t* p = half + kv_k_byte(x0, t, true);
         if constexpr (NV == 2) *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(code[0] | code[1] << 8);
         else {
@@ -115,7 +127,7 @@ __device__ __forceinline__ bool put_values(uint8_t* half, uint32_t rows, bool q8
 #pragma unroll
     for (uint32_t n = 0; n < 2; ++n) {
         if (on[n]) {
-#pragma unroll 1
+#pragma unroll
             for (uint32_t b = 0; b < D / 32; ++b)
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) {
@@ -148,9 +160,11 @@ __device__ __forceinline__ bool put_values(uint8_t* half, uint32_t rows, bool q8
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const __half d16 = __float2half_rn(top / 127.f);
-                const float d = __half2float(d16), inv = d > 0.f ? reciprocal(d) : 0.f;
+                const float d = __half2float(d16);
+                float whole[8];
+                if (d > 0.f) codes_of<float, 8>(v[n], d, reciprocal(d), whole);
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) v[n][i] = d > 0.f ? static_cast<float>(code_of<float>(v[n][i], d, inv)) : 0.f;
+                for (uint32_t i = 0; i < 8; ++i) v[n][i] = d > 0.f ? whole[i] : 0.f;
                 if (on[n] && t == 0) *reinterpret_cast<__half*>(half + kv_scale_byte(32 * b, g + 8 * n, D)) = d16;
             }
 #pragma unroll
@@ -220,61 +234,76 @@ struct HeadRows {
     uint32_t q_heads, kv_heads;   // kv_heads: of k_out (no cache)
 };
 
-// Blocks of three kinds. Rows that go out as rows: a block has as many heads as its threads take at eight dims each, and walks every `stride`-th row with
-// them, the next row's values under way and its angles computed (in the other half of the buffer) while one is turned. Keys that go into
-// the cache: a block per row, a warp per head. Values that do: a warp per group of 16 slots and head.
-template <uint32_t D, bool IN16, bool OUT16>
-__device__ __forceinline__ void turn_rows(const tsp_qk_norm_rope_args& a, const HeadRows& r, uint32_t pass, uint32_t row, uint32_t stride, uint32_t end, uint32_t* error) {
-    __shared__ __align__(16) float cs[2][D / 2], sn[2][D / 2];
-    constexpr uint32_t LANES = D / 8;   // lanes of a head
+// Blocks of three kinds. Rows that go out as rows: a block takes RB rows and as many heads as its threads hold at eight dims each; the rows' values are under
+// way while the threads compute the rows' angles, one each. Keys that go into the cache: a block per row, a warp per head. Values that do: a
+// warp per group of 16 slots and head.
+template <bool F16> struct Raw4;   // four values as they lie in memory
+template <> struct Raw4<true> {
+    uint2 w;
+    __device__ __forceinline__ void load(const uint8_t* p) { w = *reinterpret_cast<const uint2*>(p); }
+    __device__ __forceinline__ void to(float (&v)[4]) const {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+        v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+    }
+};
+template <> struct Raw4<false> {
+    float4 w;
+    __device__ __forceinline__ void load(const uint8_t* p) { w = *reinterpret_cast<const float4*>(p); }
+    __device__ __forceinline__ void to(float (&v)[4]) const { v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w; }
+};
+template <uint32_t D, bool IN16, bool OUT16, uint32_t RB>
+__device__ __forceinline__ void turn_rows(const tsp_qk_norm_rope_args& a, const HeadRows& r, uint32_t pass, uint32_t row0, uint32_t end, uint32_t* error) {
+    __shared__ __align__(16) float cs[RB][D / 2], sn[RB][D / 2];
+    constexpr uint32_t LANES = D / 8, IE = IN16 ? 2 : 4, OE = OUT16 ? 2 : 4;   // lanes of a head
     const uint32_t tid = threadIdx.x, lane = tid % 32, half = a.rotary_dim / 2, heads = r.q_heads + r.kv_heads, l = tid % LANES;
     const uint32_t h0 = pass * (blockDim.x / LANES) + tid / LANES, h = min(h0, heads - 1);   // a lane behind the last head takes that one again: whole warps shuffle
     // four pairs a lane: (u, v) at dims xu.., xv.., or interleaved in eight dims from xu on; the dims behind the rotated ones pair up as halves
-    const uint32_t p0 = 4 * l, rest = p0 - half;
+    const uint32_t p0 = 4 * l;
     const bool turned = p0 < half, pairs = turned && a.style == TSP_ROPE_PAIRS, is_k = h >= r.q_heads;
-    const uint32_t xu = turned ? (pairs ? 2 * p0 : p0) : a.rotary_dim + rest, xv = turned ? (pairs ? xu + 4 : p0 + half) : xu + (D - a.rotary_dim) / 2;
+    const uint32_t xu = turned ? (pairs ? 2 * p0 : p0) : half + p0, xv = turned ? (pairs ? xu + 4 : p0 + half) : xu + (D - a.rotary_dim) / 2;
     const uint32_t hh = is_k ? h - r.q_heads : h;
-    const uint8_t* in = (is_k ? r.k : r.q) + hh * D * (IN16 ? 2u : 4u);
-    uint8_t* out = (is_k ? r.k_out : r.q_out) + hh * D * (OUT16 ? 2u : 4u);
     const uint64_t in_stride = is_k ? r.k_stride : r.q_stride, out_stride = is_k ? r.k_out_stride : r.q_out_stride;
+    const uint8_t* in = (is_k ? r.k : r.q) + row0 * in_stride + (hh * D + xu) * IE;
+    uint8_t* out = (is_k ? r.k_out : r.q_out) + row0 * out_stride + (hh * D + xu) * OE;
+    const uint32_t iv = (xv - xu) * IE, ov = (xv - xu) * OE;
+    Raw4<IN16> ru[RB], rv[RB];
+#pragma unroll
+    for (uint32_t j = 0; j < RB; ++j)
+        if (row0 + j < end) { ru[j].load(in + j * in_stride); rv[j].load(in + j * in_stride + iv); }
     const float* w = is_k ? a.d_k_norm : a.d_q_norm;
-    float wu[4] = {1.f, 1.f, 1.f, 1.f}, wv[4] = {1.f, 1.f, 1.f, 1.f}, nu[4], nv[4];
-    if (w) {
-        load4<false>(reinterpret_cast<const uint8_t*>(w), xu, wu);
-        load4<false>(reinterpret_cast<const uint8_t*>(w), xv, wv);
-    }
-    auto fetch = [&](uint32_t at, uint32_t buffer) {
-        const uint8_t* src = in + at * in_stride;
-        load4<IN16>(src, xu, nu);
-        load4<IN16>(src, xv, nv);
-        for (uint32_t p = tid; p < half; p += blockDim.x) {
-            const double turns = static_cast<double>(r.positions[at]) * static_cast<double>(a.d_inv_freq[p]) * 0.15915494309189535;
+    Raw4<false> wu, wv;
+    if (w) { wu.load(reinterpret_cast<const uint8_t*>(w + xu)); wv.load(reinterpret_cast<const uint8_t*>(w + xv)); }
+    if (half) {
+        for (uint32_t i = tid; i < RB * half; i += blockDim.x) {
+            const uint32_t j = RB == 1 ? 0 : i / half, p = RB == 1 ? i : i - j * half;
+            if (row0 + j >= end) break;
+            const double turns = static_cast<double>(r.positions[row0 + j]) * static_cast<double>(a.d_inv_freq[p]) * 0.15915494309189535;
             float s, c;
             sincospif(static_cast<float>(2 * (turns - rint(turns))), &s, &c);   // half turns, reduced in 64 bits
-            cs[buffer][p] = c * a.magnitude; sn[buffer][p] = s * a.magnitude;
+            cs[j][p] = c * a.magnitude; sn[j][p] = s * a.magnitude;
         }
-    };
-    if (row < end) fetch(row, 0);
-    bool bad = false;
-#pragma unroll 1
-    for (uint32_t buffer = 0; row < end; row += stride, buffer ^= 1) {
         __syncthreads();
-        float u[4], v[4];
+    }
+    bool bad = false;
+    const uint32_t group = LANES == 32 ? 0xffffffffu : ((1u << (LANES % 32)) - 1) << (lane / LANES * LANES);
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) { u[i] = nu[i]; v[i] = nv[i]; }
-        if (row + stride < end) fetch(row + stride, buffer ^ 1);
+    for (uint32_t j = 0; j < RB; ++j) {
+        if (row0 + j >= end) break;
+        float u[4], v[4];
+        ru[j].to(u); rv[j].to(v);
         if (w) {
-            float ss = 0.f;
+            float ss = 0.f, fu[4], fv[4];
+            wu.to(fu); wv.to(fv);
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) ss = fmaf(u[i], u[i], fmaf(v[i], v[i], ss));
 #pragma unroll
             for (uint32_t o = LANES / 2; o; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
             const float inv = rsqrtf(ss * (1.f / D) + a.eps);
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) { u[i] = u[i] * inv * wu[i]; v[i] = v[i] * inv * wv[i]; }
+            for (uint32_t i = 0; i < 4; ++i) { u[i] = u[i] * inv * fu[i]; v[i] = v[i] * inv * fv[i]; }
         }
         if (turned) {
-            const float4 c4 = *reinterpret_cast<const float4*>(cs[buffer] + p0), n4 = *reinterpret_cast<const float4*>(sn[buffer] + p0);
+            const float4 c4 = *reinterpret_cast<const float4*>(cs[j] + p0), n4 = *reinterpret_cast<const float4*>(sn[j] + p0);
             const float c[4] = {c4.x, c4.y, c4.z, c4.w}, n[4] = {n4.x, n4.y, n4.z, n4.w};
             if (pairs) {
                 float t[4] = {u[0], u[2], v[0], v[2]}, s[4] = {u[1], u[3], v[1], v[3]};
@@ -290,32 +319,30 @@ __device__ __forceinline__ void turn_rows(const tsp_qk_norm_rope_args& a, const 
         uint32_t top = 0;
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) top = max(top, max(__float_as_uint(u[i]) & 0x7fffffffu, __float_as_uint(v[i]) & 0x7fffffffu));
-        const uint32_t group = LANES == 32 ? 0xffffffffu : ((1u << (LANES % 32)) - 1) << (lane / LANES * LANES);
         const bool ok = (__ballot_sync(0xffffffffu, top < (OUT16 ? 0x477ff000u : 0x7f800000u)) & group) == group;   // 65520 rounds to infinity in binary16
         if (!ok) {
+            bad |= h0 < heads;
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) u[i] = v[i] = 0.f;
         }
         if (h0 < heads) {
-            bad |= !ok;
-            uint8_t* dst = out + row * out_stride;
-            store4<OUT16>(dst, xu, u);
-            store4<OUT16>(dst, xv, v);
+            store4<OUT16>(out + j * out_stride, 0, u);
+            store4<OUT16>(out + j * out_stride + ov, 0, v);
         }
     }
     if (bad) raise_error(error, TSP_ERR_NONFINITE);
 }
 
-template <uint32_t D, bool IN16, bool OUT16>
+template <uint32_t D, bool IN16, bool OUT16, uint32_t RB>
 __global__ void __launch_bounds__(512)
 turn_rows_kernel(const tsp_qk_norm_rope_args a, const HeadRows r, uint32_t passes, uint32_t rows, uint32_t* error) {
     pdl_launch_dependents();
     pdl_wait();
-    turn_rows<D, IN16, OUT16>(a, r, blockIdx.x % passes, blockIdx.x / passes, gridDim.x / passes, rows, error);
+    turn_rows<D, IN16, OUT16, RB>(a, r, blockIdx.x % passes, blockIdx.x / passes * RB, rows, error);
 }
 
-// Grid: value blocks, a key block per row, then `turning` blocks of `passes` each for the query rows
-template <uint32_t D, bool IN16, bool OUT16>
+// Grid: value blocks, a key block per row, then `passes` blocks for every RB query rows
+template <uint32_t D, bool IN16, bool OUT16, uint32_t RB>
 __global__ void __launch_bounds__(kHeadThreads)
 append_rows_kernel(const tsp_qk_norm_rope_args a, const HeadRows r, const tsp_kv_cache cache, const tsp_kv_batch batch, uint32_t values, uint32_t passes, uint32_t* error) {
     __shared__ double cs[D / 2], sn[D / 2], exchange[kHeadThreads / 32][D];
@@ -325,8 +352,8 @@ append_rows_kernel(const tsp_qk_norm_rope_args a, const HeadRows r, const tsp_kv
     const bool q8 = cache.type == TSP_TYPE_Q8_0;
     if (blockIdx.x == 0) kv_check_offsets(batch, error);
     if (blockIdx.x >= values + batch.rows) {
-        const uint32_t block = blockIdx.x - values - batch.rows, blocks = gridDim.x - values - batch.rows;
-        turn_rows<D, IN16, OUT16>(a, r, block % passes, block / passes, blocks / passes, min(batch.rows, batch.d_row_offsets[batch.sequences]), error);
+        const uint32_t block = blockIdx.x - values - batch.rows;
+        turn_rows<D, IN16, OUT16, RB>(a, r, block % passes, block / passes * RB, min(batch.rows, batch.d_row_offsets[batch.sequences]), error);
         return;
     }
     uint32_t seq, node;
@@ -577,16 +604,20 @@ static uint32_t value_blocks(const tsp_kv_cache& c, const tsp_kv_batch& b) {
 template <uint32_t D, bool IN16, bool OUT16>
 static int launch_head_rows_d(const tsp_qk_norm_rope_args& a, const HeadRows& r, const tsp_kv_cache* cache, const tsp_kv_batch* batch, uint32_t rows, uint32_t* error,
                               cudaStream_t st) {
-    const uint32_t lanes = (r.q_heads + r.kv_heads) * (D / 8), sms = static_cast<uint32_t>(sm_count() > 0 ? sm_count() : 1);
-    // a few blocks per SM walk the rows: 4096 rows of 40 heads of 128 binary16 values 16 us, a block per row 24
+    // Four rows a block, so that a thread computes an angle or two and has 64 bytes under way (4096 rows of 40 heads of 128 binary16 values: a row a block 24 us);
+    // one while that is no more than two blocks per SM
+    const uint32_t lanes = (r.q_heads + r.kv_heads) * (D / 8), threads = cache ? kHeadThreads : 0, sms = static_cast<uint32_t>(sm_count() > 0 ? sm_count() : 1);
     if (!cache) {   // as few idle threads as passes of at most 512 allow: 40 heads of 128 dims in two passes of 320 threads
-        const uint32_t passes = (lanes + 511) / 512, threads = ((lanes + passes - 1) / passes + 31) / 32 * 32, walkers = (sms * (2048 / threads) + passes - 1) / passes;
-        TSP_CUDA(launch_pdl(turn_rows_kernel<D, IN16, OUT16>, dim3(passes * (rows < walkers ? rows : walkers)), dim3(threads), 0, st, a, r, passes, rows, error));
+        const uint32_t passes = (lanes + 511) / 512, width = ((lanes + passes - 1) / passes + 31) / 32 * 32;
+        if (rows * passes <= 2 * sms) TSP_CUDA(launch_pdl(turn_rows_kernel<D, IN16, OUT16, 1>, dim3(passes * rows), dim3(width), 0, st, a, r, passes, rows, error));
+        else TSP_CUDA(launch_pdl(turn_rows_kernel<D, IN16, OUT16, 4>, dim3(passes * ((rows + 3) / 4)), dim3(width), 0, st, a, r, passes, rows, error));
         return TSP_OK;
     }
-    const uint32_t values = value_blocks(*cache, *batch), passes = (lanes + kHeadThreads - 1) / kHeadThreads, walkers = passes ? (sms * 4 + passes - 1) / passes : 0;
-    TSP_CUDA(launch_pdl(append_rows_kernel<D, IN16, OUT16>, dim3(values + rows + passes * (rows < walkers ? rows : walkers)), dim3(kHeadThreads), 0, st, a, r, *cache,
-                        *batch, values, passes ? passes : 1u, error));
+    const uint32_t values = value_blocks(*cache, *batch), passes = (lanes + threads - 1) / threads, at_least_one = passes ? passes : 1;
+    if (rows * passes <= 2 * sms)
+        TSP_CUDA(launch_pdl(append_rows_kernel<D, IN16, OUT16, 1>, dim3(values + rows + passes * rows), dim3(threads), 0, st, a, r, *cache, *batch, values, at_least_one, error));
+    else
+        TSP_CUDA(launch_pdl(append_rows_kernel<D, IN16, OUT16, 4>, dim3(values + rows + passes * ((rows + 3) / 4)), dim3(threads), 0, st, a, r, *cache, *batch, values, at_least_one, error));
     return TSP_OK;
 }
 
