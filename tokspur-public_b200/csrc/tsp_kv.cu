@@ -341,27 +341,28 @@ turn_rows_kernel(const tsp_qk_norm_rope_args a, const HeadRows r, uint32_t passe
     turn_rows<D, IN16, OUT16, RB>(a, r, blockIdx.x % passes, blockIdx.x / passes * RB, rows, error);
 }
 
-// Grid: value blocks, a key block per row, then `passes` blocks for every RB query rows
+// Grid: value blocks, key blocks, then `passes` blocks for every RB query rows. A key block: four slots (a quarter of a group), a warp per head.
+constexpr uint32_t kKeyRows = 4;
 template <uint32_t D, bool IN16, bool OUT16, uint32_t RB>
 __global__ void __launch_bounds__(kHeadThreads)
-append_rows_kernel(const tsp_qk_norm_rope_args a, const HeadRows r, const tsp_kv_cache cache, const tsp_kv_batch batch, uint32_t values, uint32_t passes, uint32_t* error) {
-    __shared__ double cs[D / 2], sn[D / 2], exchange[kHeadThreads / 32][D];
+append_rows_kernel(const tsp_qk_norm_rope_args a, const HeadRows r, const tsp_kv_cache cache, const tsp_kv_batch batch, uint32_t values, uint32_t keys, uint32_t passes,
+                   uint32_t* error) {
+    __shared__ double cs[kKeyRows][D / 2], sn[kKeyRows][D / 2], exchange[kHeadThreads / 32][D];
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+    const uint32_t tid = threadIdx.x, lane = tid % 32, warp = tid / 32, places = kv_group_places(batch.rows, batch.sequences);
     const bool q8 = cache.type == TSP_TYPE_Q8_0;
     if (blockIdx.x == 0) kv_check_offsets(batch, error);
-    if (blockIdx.x >= values + batch.rows) {
-        const uint32_t block = blockIdx.x - values - batch.rows;
+    if (blockIdx.x >= values + keys) {
+        const uint32_t block = blockIdx.x - values - keys;
         turn_rows<D, IN16, OUT16, RB>(a, r, block % passes, block / passes * RB, min(batch.rows, batch.d_row_offsets[batch.sequences]), error);
         return;
     }
-    uint32_t seq, node;
+    uint32_t seq, row0, mask;
+    uint64_t slot0;
     if (blockIdx.x < values) {
         const uint32_t task = blockIdx.x * (kHeadThreads / 32) + warp, place = task / cache.kv_heads, head = task % cache.kv_heads;
-        uint64_t slot0;
-        uint32_t row0, mask;
-        if (place >= kv_group_places(batch.rows, batch.sequences) || !kv_group_of_place(batch, place, lane, seq, slot0, row0, mask)) return;
+        if (place >= places || !kv_group_of_place(batch, place, lane, seq, slot0, row0, mask)) return;
         uint8_t* group = kv_group(cache, seq, slot0, head, error);
         if (!group) return;
         const bool fine = put_values<D, IN16>(group + kv_half_bytes(D, q8), mask, q8, lane,
@@ -369,58 +370,66 @@ append_rows_kernel(const tsp_qk_norm_rope_args a, const HeadRows r, const tsp_kv
         if (!fine) raise_error(error, TSP_ERR_NONFINITE);
         return;
     }
-    constexpr uint32_t NV = D / 32;
-    const uint32_t row = blockIdx.x - values, half = a.rotary_dim / 2;
-    float key[NV];
-    if (warp < cache.kv_heads) load_run<IN16>(r.k + row * r.k_stride + warp * D * (IN16 ? 2u : 4u), lane * NV, key);
-    if (!kv_row(batch, row, lane, seq, node)) return;
+    constexpr uint32_t NV = D / 32, QUARTERS = kKvGroup / kKeyRows;
+    const uint32_t quarter = (blockIdx.x - values) % QUARTERS, half = a.rotary_dim / 2;
+    if (!kv_group_of_place(batch, (blockIdx.x - values) / QUARTERS, lane, seq, slot0, row0, mask)) return;
+    mask &= ((1u << kKeyRows) - 1) << (quarter * kKeyRows);
+    if (!mask) return;
+    const uint32_t t0 = __ffs(mask) - 1, t1 = 32 - __clz(mask);   // the quarter's slots of this step
+    auto key_row = [&](uint32_t t, uint32_t h) { return r.k + static_cast<uint64_t>(row0 + t) * r.k_stride + h * D * (IN16 ? 2u : 4u); };
+    float next[NV];
+    if (warp < cache.kv_heads) load_run<IN16>(key_row(t0, warp), lane * NV, next);
     if (half) {
-        const double pos = r.positions[row];
-        for (uint32_t p = tid; p < half; p += kHeadThreads) {
-            const double turns = pos * static_cast<double>(a.d_inv_freq[p]) * 0.15915494309189535;
+        for (uint32_t i = tid; i < (t1 - t0) * half; i += kHeadThreads) {
+            const uint32_t j = i / half, p = i - j * half;
+            const double turns = static_cast<double>(r.positions[row0 + t0 + j]) * static_cast<double>(a.d_inv_freq[p]) * 0.15915494309189535;
             double s, c;
             sincospi(2 * (turns - rint(turns)), &s, &c);
-            cs[p] = c * a.magnitude; sn[p] = s * a.magnitude;
+            cs[j][p] = c * a.magnitude; sn[j][p] = s * a.magnitude;
         }
         __syncthreads();
     }
     bool bad = false;
-    const uint64_t slot = static_cast<uint64_t>(batch.d_lengths[seq]) + node;
 #pragma unroll 1
     for (uint32_t h = warp; h < cache.kv_heads; h += kHeadThreads / 32) {
-        uint8_t* group = kv_group(cache, seq, slot, h, error);
+        uint8_t* group = kv_group(cache, seq, slot0, h, error);
         if (!group) continue;
-        if (h >= kHeadThreads / 32) load_run<IN16>(r.k + row * r.k_stride + h * D * (IN16 ? 2u : 4u), lane * NV, key);
-        double y[NV];
+        if (h >= kHeadThreads / 32) load_run<IN16>(key_row(t0, h), lane * NV, next);
+#pragma unroll 1
+        for (uint32_t t = t0; t < t1; ++t) {
+            double y[NV];
 #pragma unroll
-        for (uint32_t i = 0; i < NV; ++i) y[i] = key[i];
-        if (a.d_k_norm) {
-            double ss = 0;
+            for (uint32_t i = 0; i < NV; ++i) y[i] = next[i];
+            if (t + 1 < t1) load_run<IN16>(key_row(t + 1, h), lane * NV, next);
+            if (a.d_k_norm) {
+                double ss = 0;
 #pragma unroll
-            for (uint32_t i = 0; i < NV; ++i) ss = fma(y[i], y[i], ss);
+                for (uint32_t i = 0; i < NV; ++i) ss = fma(y[i], y[i], ss);
 #pragma unroll
-            for (uint32_t o = 16; o; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const double inv = rsqrt(ss * (1.0 / D) + static_cast<double>(a.eps));
+                for (uint32_t o = 16; o; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                const double inv = rsqrt(ss * (1.0 / D) + static_cast<double>(a.eps));
 #pragma unroll
-            for (uint32_t i = 0; i < NV; ++i) y[i] = y[i] * inv * static_cast<double>(a.d_k_norm[lane * NV + i]);
-        }
-        if (half) {
-            double* mine = exchange[warp];
-            __syncwarp();
+                for (uint32_t i = 0; i < NV; ++i) y[i] = y[i] * inv * static_cast<double>(a.d_k_norm[lane * NV + i]);
+            }
+            if (half) {
+                double* mine = exchange[warp];
+                __syncwarp();
 #pragma unroll
-            for (uint32_t i = 0; i < NV; ++i) mine[lane * NV + i] = y[i];
-            __syncwarp();
+                for (uint32_t i = 0; i < NV; ++i) mine[lane * NV + i] = y[i];
+                __syncwarp();
 #pragma unroll
-            for (uint32_t i = 0; i < NV; ++i) {
-                const uint32_t x = lane * NV + i;
-                if (x < a.rotary_dim) {
-                    const bool pairs = a.style == TSP_ROPE_PAIRS, second = pairs ? x & 1 : x >= half;
-                    const uint32_t p = pairs ? x / 2 : (second ? x - half : x), other = pairs ? x ^ 1 : (second ? x - half : x + half);
-                    y[i] = y[i] * cs[p] + mine[other] * (second ? sn[p] : -sn[p]);
+                for (uint32_t i = 0; i < NV; ++i) {
+                    const uint32_t x = lane * NV + i;
+                    if (x < a.rotary_dim) {
+                        const bool pairs = a.style == TSP_ROPE_PAIRS, second = pairs ? x & 1 : x >= half;
+                        const uint32_t p = pairs ? x / 2 : (second ? x - half : x), other = pairs ? x ^ 1 : (second ? x - half : x + half);
+                        const double s = sn[t - t0][p];
+                        y[i] = y[i] * cs[t - t0][p] + mine[other] * (second ? s : -s);
+                    }
                 }
             }
+            bad |= !put_keys<D>(group, t, q8, lane, y);
         }
-        bad |= !put_keys<D>(group, slot % kKvGroup, q8, lane, y);
     }
     if (bad) raise_error(error, TSP_ERR_NONFINITE);
 }
@@ -614,10 +623,11 @@ static int launch_head_rows_d(const tsp_qk_norm_rope_args& a, const HeadRows& r,
         return TSP_OK;
     }
     const uint32_t values = value_blocks(*cache, *batch), passes = (lanes + threads - 1) / threads, at_least_one = passes ? passes : 1;
+    const uint32_t keys = kv_group_places(batch->rows, batch->sequences) * (kKvGroup / kKeyRows);
     if (rows * passes <= 2 * sms)
-        TSP_CUDA(launch_pdl(append_rows_kernel<D, IN16, OUT16, 1>, dim3(values + rows + passes * rows), dim3(threads), 0, st, a, r, *cache, *batch, values, at_least_one, error));
+        TSP_CUDA(launch_pdl(append_rows_kernel<D, IN16, OUT16, 1>, dim3(values + keys + passes * rows), dim3(threads), 0, st, a, r, *cache, *batch, values, keys, at_least_one, error));
     else
-        TSP_CUDA(launch_pdl(append_rows_kernel<D, IN16, OUT16, 4>, dim3(values + rows + passes * ((rows + 3) / 4)), dim3(threads), 0, st, a, r, *cache, *batch, values, at_least_one, error));
+        TSP_CUDA(launch_pdl(append_rows_kernel<D, IN16, OUT16, 4>, dim3(values + keys + passes * ((rows + 3) / 4)), dim3(threads), 0, st, a, r, *cache, *batch, values, keys, at_least_one, error));
     return TSP_OK;
 }
 
