@@ -9,36 +9,42 @@ import ctypes as C
 import torch
 
 from . import capi
-from .layer import stream_ptr
 
 TYPES = {"q8_0": capi.TYPE_Q8_0, "f16": capi.TYPE_F16}
 STYLES = {"halves": capi.ROPE_HALVES, "pairs": capi.ROPE_PAIRS}
+SIZES = {torch.float32: 4, torch.float16: 2}   # of the row types; the library's dtype is 0 for four bytes, 1 for two
 
 
-def _ptr(t: torch.Tensor | None):
-    return None if t is None else t.data_ptr()
+def _rows(name: str, t: torch.Tensor, dtype: torch.dtype, heads: int, dim: int, least: int) -> tuple[int, int]:
+    """Pointer and row stride in bytes of [rows, heads, dim], after the checks that the library cannot make."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim or shape[0] < least or stride[2] != 1 or (stride[1] != dim and heads > 1) \
+            or t.dtype is not dtype or dtype not in SIZES or not t.is_cuda:
+        raise ValueError(f"{name}: {t.dtype} {tuple(shape)} with strides {stride} on {t.device} does not hold {least} rows of {heads} densely packed heads of {dim} {dtype}")
+    return t.data_ptr(), stride[0] * SIZES[dtype]
 
 
-def _stride(t: torch.Tensor | None) -> int:
-    return 0 if t is None else t.stride(0) * t.element_size()
+def _words(name: str, t: torch.Tensor, dtype: torch.dtype, least: int) -> int:
+    if t.dtype is not dtype or t.numel() < least or not t.is_contiguous() or not t.is_cuda:
+        raise ValueError(f"{name}: {least} dense values of {dtype} on a CUDA device")
+    return t.data_ptr()
 
 
-def _dtype(t: torch.Tensor) -> int:
-    if t.dtype not in (torch.float32, torch.float16):
-        raise TypeError(f"rows are float32 or float16, got {t.dtype}")
-    return int(t.dtype == torch.float16)
+_entries: dict = {}
 
 
-def _rows(name: str, t: torch.Tensor | None, like: torch.Tensor | None = None, heads: int | None = None, dim: int | None = None, least: int = 0):
-    """Checks what the library cannot see of a tensor of rows."""
-    if t is None:
-        return
-    if t.dim() != 3 or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
-        raise ValueError(f"{name}: rows are [rows, heads, head_dim] with densely packed heads")
-    if (heads is not None and t.shape[1] != heads) or (dim is not None and t.shape[2] != dim) or t.shape[0] < least:
-        raise ValueError(f"{name}: shape {tuple(t.shape)} does not hold {least} rows of {heads} heads of {dim}")
-    if like is not None and t.dtype != like.dtype:
-        raise TypeError(f"{name}: rows of {t.dtype} beside rows of {like.dtype}")
+def _call(name: str, like: torch.Tensor, error: torch.Tensor | None, *args) -> None:
+    """The library's entry on the device of `like`, on torch's current stream there."""
+    entry = _entries.get(name)
+    if entry is None:
+        entry = _entries[name] = getattr(capi.lib(), name)
+    device = like.get_device()
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _call(name, like, error, *args)
+    rc = entry(*args, None if error is None else error.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    if rc:
+        capi.check(rc)
 
 
 class KvCache:
@@ -85,7 +91,7 @@ class QkNormRope:
             if t is not None and (t.dtype != torch.float32 or t.numel() < n or not t.is_contiguous()):
                 raise ValueError("norm weights and frequencies are dense float32")
         self.tensors, self.head_dim = (inv_freq, q_norm, k_norm), head_dim
-        self.struct = capi.QkNormRope(_ptr(q_norm), _ptr(k_norm), _ptr(inv_freq), head_dim, rotary_dim, STYLES[style], eps, magnitude)
+        self.struct = capi.QkNormRope(*(None if t is None else t.data_ptr() for t in (q_norm, k_norm, inv_freq)), head_dim, rotary_dim, STYLES[style], eps, magnitude)
         self.ref = C.byref(self.struct)
 
 
@@ -96,55 +102,55 @@ def _check_batch(cache: KvCache, batch: KvBatch):
 
 def qk_norm_rope(turn: QkNormRope, q, k, positions, q_out, k_out, error):
     """q / k [rows, heads, head_dim] (either may be None) -> q_out / k_out of any of the two dtypes; positions int32 [rows]."""
-    x = q if q is not None else k
-    _rows("q", q, dim=turn.head_dim)
-    _rows("k", k, like=q, dim=turn.head_dim, least=x.shape[0])
-    o = q_out if q is not None else k_out
-    for name, t, src in (("q_out", q_out, q), ("k_out", k_out, k)):
-        if src is not None:
-            _rows(name, t, like=o, heads=src.shape[1], dim=turn.head_dim, least=x.shape[0])
-    if positions.dtype != torch.int32 or positions.numel() < x.shape[0] or not positions.is_contiguous():
-        raise ValueError("positions are int32, one for each row")
-    capi.call("tsp_qk_norm_rope", turn.ref, _ptr(q), _stride(q), _ptr(k), _stride(k), _dtype(x), positions.data_ptr(), x.shape[0],
-              0 if q is None else q.shape[1], 0 if k is None else k.shape[1], _ptr(q_out), _stride(q_out), _ptr(k_out), _stride(k_out), _dtype(o),
-              _ptr(error), stream_ptr())
+    x, o, dim = (q, q_out, turn.head_dim) if q is not None else (k, k_out, turn.head_dim)
+    rows, dt, ot = x.shape[0], x.dtype, o.dtype
+    hq = hk = qs = ks = qos = kos = 0
+    qp = kp = qop = kop = None
+    if q is not None:
+        hq = q.shape[1]
+        qp, qs = _rows("q", q, dt, hq, dim, rows)
+        qop, qos = _rows("q_out", q_out, ot, hq, dim, rows)
+    if k is not None:
+        hk = k.shape[1]
+        kp, ks = _rows("k", k, dt, hk, dim, rows)
+        kop, kos = _rows("k_out", k_out, ot, hk, dim, rows)
+    _call("tsp_qk_norm_rope", x, error, turn.ref, qp, qs, kp, ks, int(dt is torch.float16), _words("positions", positions, torch.int32, rows), rows, hq, hk, qop, qos,
+          kop, kos, int(ot is torch.float16))
 
 
 def kv_cache_append(cache: KvCache, batch: KvBatch, k, v, error):
     _check_batch(cache, batch)
-    _rows("k", k, heads=cache.kv_heads, dim=cache.head_dim, least=batch.rows)
-    _rows("v", v, like=k, heads=cache.kv_heads, dim=cache.head_dim, least=batch.rows)
-    capi.call("tsp_kv_cache_append", cache.ref, batch.ref, k.data_ptr(), _stride(k), v.data_ptr(), _stride(v), _dtype(k), _ptr(error), stream_ptr())
+    dt = k.dtype
+    kp, ks = _rows("k", k, dt, cache.kv_heads, cache.head_dim, batch.rows)
+    vp, vs = _rows("v", v, dt, cache.kv_heads, cache.head_dim, batch.rows)
+    _call("tsp_kv_cache_append", k, error, cache.ref, batch.ref, kp, ks, vp, vs, int(dt is torch.float16))
 
 
 def qk_norm_rope_append(turn: QkNormRope, cache: KvCache, batch: KvBatch, q, k, v, positions, q_out, error):
     """Norm and rotation of q into q_out; of k into the cache, beside v."""
     _check_batch(cache, batch)
-    _rows("q", q, dim=cache.head_dim, least=batch.rows)
-    _rows("k", k, like=q, heads=cache.kv_heads, dim=cache.head_dim, least=batch.rows)
-    _rows("v", v, like=q, heads=cache.kv_heads, dim=cache.head_dim, least=batch.rows)
-    _rows("q_out", q_out, heads=q.shape[1], dim=cache.head_dim, least=batch.rows)
-    if positions.dtype != torch.int32 or positions.numel() < batch.rows or not positions.is_contiguous():
-        raise ValueError("positions are int32, one for each row")
-    capi.call("tsp_qk_norm_rope_append", turn.ref, cache.ref, batch.ref, q.data_ptr(), _stride(q), k.data_ptr(), _stride(k), v.data_ptr(), _stride(v),
-              _dtype(q), positions.data_ptr(), q.shape[1], q_out.data_ptr(), _stride(q_out), _dtype(q_out), _ptr(error), stream_ptr())
+    dt, ot, dim, heads, rows = q.dtype, q_out.dtype, cache.head_dim, q.shape[1], batch.rows
+    qp, qs = _rows("q", q, dt, heads, dim, rows)
+    kp, ks = _rows("k", k, dt, cache.kv_heads, dim, rows)
+    vp, vs = _rows("v", v, dt, cache.kv_heads, dim, rows)
+    op, os = _rows("q_out", q_out, ot, heads, dim, rows)
+    _call("tsp_qk_norm_rope_append", q, error, turn.ref, cache.ref, batch.ref, qp, qs, kp, ks, vp, vs, int(dt is torch.float16),
+          _words("positions", positions, torch.int32, rows), heads, op, os, int(ot is torch.float16))
 
 
 def kv_cache_read(cache: KvCache, batch: KvBatch, k_out, v_out, error):
+    """Either of k_out and v_out may be None."""
     _check_batch(cache, batch)
-    o = k_out if k_out is not None else v_out
-    _rows("k_out", k_out, heads=cache.kv_heads, dim=cache.head_dim, least=batch.rows)
-    _rows("v_out", v_out, like=o, heads=cache.kv_heads, dim=cache.head_dim, least=batch.rows)
-    capi.call("tsp_kv_cache_read", cache.ref, batch.ref, _ptr(k_out), _stride(k_out), _ptr(v_out), _stride(v_out), _dtype(o), _ptr(error), stream_ptr())
+    x = k_out if k_out is not None else v_out
+    kp, ks = (None, 0) if k_out is None else _rows("k_out", k_out, x.dtype, cache.kv_heads, cache.head_dim, batch.rows)
+    vp, vs = (None, 0) if v_out is None else _rows("v_out", v_out, x.dtype, cache.kv_heads, cache.head_dim, batch.rows)
+    _call("tsp_kv_cache_read", x, error, cache.ref, batch.ref, kp, ks, vp, vs, int(x.dtype is torch.float16))
 
 
 def kv_cache_keep(cache: KvCache, batch: KvBatch, accepted, counts, error):
     """accepted int32 [rows] (a sequence's accepted nodes from its row offset on, ascending), counts int32 [sequences]."""
     _check_batch(cache, batch)
-    for name, t, n in (("accepted", accepted, batch.rows), ("counts", counts, batch.sequences)):
-        if t.dtype != torch.int32 or t.numel() < n or not t.is_contiguous():
-            raise ValueError(f"{name}: int32, {n} of them")
-    capi.call("tsp_kv_cache_keep", cache.ref, batch.ref, accepted.data_ptr(), counts.data_ptr(), _ptr(error), stream_ptr())
+    _call("tsp_kv_cache_keep", accepted, error, cache.ref, batch.ref, _words("accepted", accepted, torch.int32, batch.rows), _words("counts", counts, torch.int32, batch.sequences))
 
 
 def tree_attention_scratch(device="cuda") -> torch.Tensor:
@@ -156,9 +162,8 @@ def tree_attention_scratch(device="cuda") -> torch.Tensor:
 def tree_attention(cache: KvCache, batch: KvBatch, q, out, tree_mask, max_rows: int, scale: float, scratch, error):
     """q [rows, q_heads, head_dim] -> out, the same shape and dtype; tree_mask int64 [rows] (bit i: the row sees token i of its step) or None (chain)."""
     _check_batch(cache, batch)
-    _rows("q", q, dim=cache.head_dim, least=batch.rows)
-    _rows("out", out, like=q, heads=q.shape[1], dim=cache.head_dim, least=batch.rows)
-    if tree_mask is not None and (tree_mask.dtype != torch.int64 or tree_mask.numel() < batch.rows or not tree_mask.is_contiguous()):
-        raise ValueError("the tree's words are int64, one for each row")
-    capi.call("tsp_tree_attention", cache.ref, batch.ref, q.data_ptr(), _stride(q), _ptr(tree_mask), q.shape[1], max_rows, scale, out.data_ptr(), _stride(out),
-              _dtype(q), scratch.data_ptr(), scratch.numel(), _ptr(error), stream_ptr())
+    dt, heads, dim, rows = q.dtype, q.shape[1], cache.head_dim, batch.rows
+    qp, qs = _rows("q", q, dt, heads, dim, rows)
+    op, os = _rows("out", out, dt, heads, dim, rows)
+    _call("tsp_tree_attention", q, error, cache.ref, batch.ref, qp, qs, None if tree_mask is None else _words("tree words", tree_mask, torch.int64, rows), heads, max_rows,
+          scale, op, os, int(dt is torch.float16), scratch.data_ptr(), scratch.numel())
