@@ -79,13 +79,25 @@ __device__ __forceinline__ void tm_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ bool tm_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, 1u << 21)); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {   // two FP32 operations in one
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
 template <uint32_t D, bool Q8>
 __global__ void __launch_bounds__(kTmThreads, 1)
 tree_mma_kernel(const AttnParams p) {
     using S = TmShape<D, Q8>;
-    constexpr uint32_t NONE = 0xffffffffu, NB = D / 32;
+    constexpr uint32_t NONE = 0xffffffffu, NB = D / 32, K_LINES = kKvGroup * D * (Q8 ? 1 : 2) / 512;   // rows of 512 bytes that a group's keys (and values) are
     extern __shared__ uint8_t raw[];
     TmSmem<D, Q8>& sm = *reinterpret_cast<TmSmem<D, Q8>*>(raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u));
     const uint32_t tid = threadIdx.x, lane = tid % 32, warp = __shfl_sync(NONE, tid / 32, 0);
@@ -237,19 +249,20 @@ tree_mma_kernel(const AttnParams p) {
                     if (w == 0 && lane == 0) { sm.odd[j % 8][0] = static_cast<uint32_t>(all); sm.odd[j % 8][1] = static_cast<uint32_t>(all >> 32); }
                 }
                 if constexpr (Q8) {   // largest scales: below 2^(e - 14), e the binary16 exponent; the tiles are times 2^(21 - e), codes times scales below 2^14
-                    uint32_t top[2] = {0, 0};
-                    for (uint32_t i = lane; i < kTmGroups * NB * kKvGroup / 8; i += 32) {
-                        const uint32_t gi = i / (NB * 2), x = i % (NB * 2), gone8 = static_cast<uint32_t>(drop >> (gi * kKvGroup + x % 2 * 8)) & 0xffu;
+                    uint32_t top[2];
 #pragma unroll
-                        for (uint32_t side = 0; side < 2; ++side) {
-                            const uint4 d = *reinterpret_cast<const uint4*>(stage + gi * S::kGroupBytes + side * S::kHalf + kKvGroup * D + x * 16);
-                            const uint32_t words[4] = {d.x, d.y, d.z, d.w};
+                    for (uint32_t side = 0; side < 2; ++side) {
+                        constexpr uint32_t EACH = NB * 2;   // 16-byte pieces of a group's scales: eight slots of a block of 32 dims
+                        const uint32_t gi = lane / EACH % kTmGroups, x = lane % EACH;   // head_dim 64: the upper lanes look at the same again
+                        const uint4 d = *reinterpret_cast<const uint4*>(stage + gi * S::kGroupBytes + side * S::kHalf + kKvGroup * D + x * 16);
+                        uint32_t words[4] = {d.x & 0x7fff7fffu, d.y & 0x7fff7fffu, d.z & 0x7fff7fffu, d.w & 0x7fff7fffu};
+                        if (edge) {
+                            const uint32_t out = static_cast<uint32_t>(drop >> (gi * kKvGroup + x % 2 * 8));
 #pragma unroll
-                            for (uint32_t c = 0; c < 8; ++c) {
-                                const uint32_t bits = words[c / 2] >> (16 * (c & 1)) & 0x7fffu;
-                                if (!(gone8 >> c & 1)) top[side] = max(top[side], bits);
-                            }
+                            for (uint32_t c = 0; c < 4; ++c) words[c] &= (out >> (2 * c) & 1 ? 0u : 0x0000ffffu) | (out >> (2 * c) & 2 ? 0u : 0xffff0000u);
                         }
+                        const uint32_t most = __vmaxu2(__vmaxu2(words[0], words[1]), __vmaxu2(words[2], words[3]));
+                        top[side] = max(most & 0xffffu, most >> 16);
                     }
                     const int ek = static_cast<int>(min(max(__reduce_max_sync(NONE, top[0]) >> 10, 1u), 30u)), ev = static_cast<int>(min(max(__reduce_max_sync(NONE, top[1]) >> 10, 1u), 30u));
                     k_up = pow2(21 - ek); v_up = pow2(21 - ev);
@@ -257,37 +270,37 @@ tree_mma_kernel(const AttnParams p) {
                 }
                 // K: [64 dims][64 slots] rows of 128 bytes; a lane's 16 bytes are dims 8 t.. of both 32s (Q8_0) or 8 t.. of one (binary16) of slot 8 n + g
 #pragma unroll
-                for (uint32_t i = 0; i < S::kHalf / 512 * kTmGroups / 8; ++i) {
-                    constexpr uint32_t LINES = kKvGroup * D * (Q8 ? 1 : 2) / 512;   // of a group
+                for (uint32_t i = 0; i < K_LINES * kTmGroups / 8; ++i) {
+                    constexpr uint32_t LINES = K_LINES;
                     const uint32_t line = i * 8 + w;
-                    if (line >= LINES * kTmGroups) break;
                     const uint32_t gi = line / LINES, x = line % LINES, in = x % 2 * 8 + g, slot = gi * kKvGroup + in;
                     const uint8_t* group = stage + gi * S::kGroupBytes;
                     const uint4 c = *reinterpret_cast<const uint4*>(group + x * 512 + lane * 16);
                     if constexpr (Q8) {
-                        const uint32_t panel = x / 2;
-                        const uint32_t words[4] = {c.x, c.y, c.z, c.w};
-                        uint32_t high[8], low[8];
+                        // odd slots put their second half first: eight lanes on eight different 16 bytes
+                        const uint32_t panel = x / 2, turned = g & 1;
+                        const uint32_t words[4] = {turned ? c.z : c.x, turned ? c.w : c.y, turned ? c.x : c.z, turned ? c.y : c.w};
+                        const uint8_t* scales = group + kKvGroup * D + (2 * panel * kKvGroup + in) * 2;
+                        uint8_t* to = sm.k[buf][0] + panel * (kTmUnit * 128) + slot * 128;
 #pragma unroll
-                        for (uint32_t h = 0; h < 2; ++h) {
-                            const __half2 d = __float2half2_rn(__half2float(*reinterpret_cast<const __half*>(group + kKvGroup * D + ((2 * panel + h) * kKvGroup + in) * 2)) * k_up);
+                        for (uint32_t side = 0; side < 2; ++side) {
+                            const uint32_t h = side ^ turned;
+                            const __half2 d = __float2half2_rn(__half2float(*reinterpret_cast<const __half*>(scales + h * (kKvGroup * 2))) * k_up);
+                            uint32_t high[4], low[4];
 #pragma unroll
                             for (uint32_t x2 = 0; x2 < 2; ++x2) {
                                 uint32_t y[2];
-                                codes_to_halves(words[2 * h + x2], y[0], y[1]);
+                                codes_to_halves(words[2 * side + x2], y[0], y[1]);
 #pragma unroll
                                 for (uint32_t z = 0; z < 2; ++z) {
                                     const __half2 v = __hmul2(bits_h2(y[z]), d);
-                                    high[4 * h + 2 * x2 + z] = h2_bits(v);
-                                    low[4 * h + 2 * x2 + z] = h2_bits(__hfma2(bits_h2(y[z]), d, __hneg2(v)));
+                                    high[2 * x2 + z] = h2_bits(v);
+                                    low[2 * x2 + z] = h2_bits(__hfma2(bits_h2(y[z]), d, __hneg2(v)));
                                 }
                             }
-                        }
-#pragma unroll
-                        for (uint32_t side = 0; side < 2; ++side) {   // odd slots write their second half first: eight lanes on eight different 16 bytes
-                            const uint32_t h = side ^ (g & 1), at = panel * (kTmUnit * 128) + slot * 128 + (((4 * h + t) ^ (slot & 7)) << 4);
-                            *reinterpret_cast<uint4*>(sm.k[buf][0] + at) = h ? make_uint4(high[4], high[5], high[6], high[7]) : make_uint4(high[0], high[1], high[2], high[3]);
-                            *reinterpret_cast<uint4*>(sm.k[buf][S::kParts - 1] + at) = h ? make_uint4(low[4], low[5], low[6], low[7]) : make_uint4(low[0], low[1], low[2], low[3]);
+                            const uint32_t at = ((4 * h + t) ^ (slot & 7)) << 4;
+                            *reinterpret_cast<uint4*>(to + at) = make_uint4(high[0], high[1], high[2], high[3]);
+                            *reinterpret_cast<uint4*>(to + (S::kParts - 1) * S::kKPart + at) = make_uint4(low[0], low[1], low[2], low[3]);
                         }
                     } else {
                         const uint32_t b = x / 2;   // 32 dims
@@ -302,10 +315,9 @@ tree_mma_kernel(const AttnParams p) {
             if (!ok) break;
             if (!gone) {
                 // V: [dims][64 slots], rows of 128 bytes; a lane's 16 bytes are dims 8 i + g, slots 2 t, 2 t + 1, 8 more
-                constexpr uint32_t LINES = kKvGroup * D * (Q8 ? 1 : 2) / 512;
 #pragma unroll
-                for (uint32_t i = 0; i < LINES * kTmGroups / 8; ++i) {
-                    const uint32_t line = i * 8 + w, gi = line / LINES, x = line % LINES;
+                for (uint32_t i = 0; i < K_LINES * kTmGroups / 8; ++i) {
+                    const uint32_t line = i * 8 + w, gi = line / K_LINES, x = line % K_LINES;
                     const uint8_t* values = stage + gi * S::kGroupBytes + S::kHalf;
                     const uint4 c = *reinterpret_cast<const uint4*>(values + x * 512 + lane * 16);
                     const uint32_t words[4] = {c.x, c.y, c.z, c.w};
@@ -377,17 +389,20 @@ tree_mma_kernel(const AttnParams p) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.q_ready[item & 1]);
         };
-        AttnItem it = item_of<kTmRows, kTmUnit>(p, sm.cum, u0);
-        load_q(it, 0);
+        // An item is looked up where something of it is wanted, not kept: a score row of 64 leaves no registers for it
+        auto item_at = [&](uint32_t unit) { return item_of<kTmRows, kTmUnit>(p, sm.cum, u0 + unit); };
+        load_q(item_at(0), 0);
         uint32_t j = 0;
         for (uint32_t item = 0; j < n && ok; ++item) {
-            const uint32_t first = j, stop = static_cast<uint32_t>(min(it.end, u1) - u0);
-            AttnItem next = it;
-            if (stop < n) {
-                next = item_of<kTmRows, kTmUnit>(p, sm.cum, u0 + stop);
-                load_q(next, item + 1);   // that buffer's last readers, the scores of the item before this one, are done
+            const uint32_t first = j;
+            uint32_t stop, inner;   // units of the run's part of the item, of those inside the context
+            {
+                const AttnItem it = item_at(j);
+                stop = static_cast<uint32_t>(min(it.end, u1) - u0);
+                const uint64_t plain = it.start + it.length / kTmUnit;
+                inner = plain <= u0 ? 0u : static_cast<uint32_t>(min(plain - u0, static_cast<uint64_t>(stop)));
+                if (stop < n) load_q(item_at(stop), item + 1);   // that buffer's last readers, the scores of the item before this one, are done
             }
-            uint64_t word = 0;
             float m = -INFINITY, l = 0.f, ref = 0.f, limit = -INFINITY;
             int lift = 64;   // of the V tiles: the accumulator is at the smallest so far
             bool dead = false;
@@ -406,9 +421,11 @@ tree_mma_kernel(const AttnParams p) {
                 dead |= sm.gone[j % 8] != 0;
                 const int k_lift = Q8 ? static_cast<int>(sm.k_lift[j % 8]) : 0, v_lift = Q8 ? static_cast<int>(sm.v_lift[j % 8]) : 0;
                 const float fj = Q8 ? f * pow2(-k_lift) : f;
-                const uint64_t slot0 = (u0 + j - it.start) * kTmUnit;
-                if (slot0 + kTmUnit > it.length) {
-                    if (!word && r < it.rows) {
+                if (j >= inner) {
+                    const AttnItem it = item_at(j);
+                    const uint64_t slot0 = (u0 + j - it.start) * kTmUnit;
+                    uint64_t word = 0;
+                    if (r < it.rows) {
                         uint32_t node, head;
                         place(it, node, head);
                         word = p.mask ? p.mask[it.row0 + node] : ~0ull >> (63 - min(node, 63u));
@@ -455,15 +472,19 @@ tree_mma_kernel(const AttnParams p) {
                     }
                     lift = min(lift, v_lift);
                 }
-                // V tiles at a higher power of two than the accumulator: the weights take what is between
-                const float down = Q8 ? pow2(max(lift - v_lift, -100)) : 1.f;
+                // V tiles at a higher power of two than the accumulator: the weights take what is between, and the sum gives it back
+                const float shift = Q8 ? max(static_cast<float>(lift - v_lift), -100.f) : 0.f;
                 uint32_t w[32];
+                float2 sum = make_float2(0.f, 0.f);
+                const float2 fj2 = make_float2(fj, fj), ref2 = make_float2(ref + shift, ref + shift);
 #pragma unroll
                 for (uint32_t c = 0; c < 32; ++c) {
-                    const float a = exp2_approx(fmaf(s[c / 16][2 * c % 32], fj, ref)), b = exp2_approx(fmaf(s[c / 16][2 * c % 32 + 1], fj, ref));
-                    l += a + b;
-                    w[c] = h2_bits(__floats2half2_rn(Q8 ? a * down : a, Q8 ? b * down : b));
+                    float2 x2 = fma2(make_float2(s[c / 16][2 * c % 32], s[c / 16][2 * c % 32 + 1]), fj2, ref2);
+                    x2.x = exp2_approx(x2.x); x2.y = exp2_approx(x2.y);
+                    sum = add2(sum, x2);
+                    w[c] = h2_bits(__floats2half2_rn(x2.x, x2.y));
                 }
+                l = fmaf(sum.x + sum.y, Q8 ? exp2_approx(-shift) : 1.f, l);
                 ok = j < 2 || tm_wait(&sm.pv_done[buf], turn ^ 1);   // PV of unit j - 2 has read this buffer
                 if (!ok) break;
                 tm_fence_after();
@@ -478,6 +499,7 @@ tree_mma_kernel(const AttnParams p) {
             ok = tm_wait(&sm.pv_done[last & 1], (last >> 1) & 1);
             if (!ok) break;
             tm_fence_after();
+            const AttnItem it = item_at(first);
             const bool whole = it.start >= u0 && it.end <= u1;
             const float scale = Q8 ? pow2(max(min(-lift, 120), -120)) : 1.f;
             if (whole) {
@@ -525,7 +547,6 @@ tree_mma_kernel(const AttnParams p) {
                 }
             }
             tm_fence_before();   // the accumulator is read before the next item's first weights are said to be ready
-            it = next;
         }
     }
     if (!ok && lane == 0) raise_error(p.error, TSP_ERR_TIMEOUT);
