@@ -4,7 +4,7 @@
 // the M of tcgen05 MMAs: S = Q K^T (N = 64 slots, K = dims) and O += P V (N = dims, K = 64 slots), both with the left operand in tensor memory and the cache's
 // tile in shared memory. Units are 64 slots; they are dealt to the blocks as there, and pieces of items that span blocks are joined the same way.
 //
-// Roles of a block's 16 warps (one block per SM): 0 copies groups of 16 slots into a ring; 1 issues the MMAs; 4..7 are the softmax, a thread per query row:
+// Roles of a block's 24 warps (one block per SM): 0 copies groups of 16 slots into a ring; 3 looks at what came; 1 issues the MMAs; 4..7 are the softmax, a thread per query row:
 // a score row from tensor memory to registers, weights back to tensor memory as binary16, reference, sum and the rare rescaling of the accumulator, and at an
 // item's end the accumulator's row; 8..15 turn codes into the MMAs' tiles. Scores, weights, query rows and tiles are double-buffered, so the QK of
 // one unit runs under the softmax of the one before and the PV of the one before that.
@@ -16,8 +16,12 @@
 
 namespace tsp {
 
-constexpr uint32_t kTmRows = 128, kTmUnit = 64, kTmThreads = 512, kTmGroups = kTmUnit / kKvGroup;
-constexpr uint32_t kTmSoftmax = 4, kTmTiles = 8;   // first softmax warp, first tile warp
+constexpr uint32_t kTmRows = 128, kTmUnit = 64, kTmGroups = kTmUnit / kKvGroup;
+constexpr uint32_t kTmSoftmax = 4, kTmTiles = 8, kTmTileWarps = 16, kTmThreads = 32 * (kTmTiles + kTmTileWarps);   // first softmax warp, first tile warp
+// Registers after the hand-over between the warpgroups (setmaxnreg): together no more than the count at launch (80) times the six warpgroups, or the softmax
+// would wait for ever; the launcher checks it. At the end all go back to that count.
+constexpr int kTmLaunchRegs = 80, kTmIssueRegs = 64, kTmSoftmaxRegs = 160, kTmTileRegs = 64;
+static_assert(kTmIssueRegs + kTmSoftmaxRegs + 4 * kTmTileRegs <= 6 * kTmLaunchRegs, "hand-over of registers");
 // piece of an item: references and sums of 128 rows, a flag, then the rows' dims four by four, rows side by side: [dim / 4][row][4]
 constexpr uint32_t kTmPartHead = 288;
 __host__ __device__ constexpr uint64_t tm_part_floats() { return kTmPartHead + kTmRows * 128; }
@@ -39,11 +43,12 @@ struct TmSmem {
     alignas(128) uint8_t ring[S::kStages][S::kStage];
     uint64_t cum[TSP_KV_MAX_SEQUENCES + 1];
     uint64_t warp_sums[kTmThreads / 32];
-    uint64_t code_full[S::kStages], code_empty[S::kStages];
+    uint64_t code_full[S::kStages], code_known[S::kStages], code_empty[S::kStages];
     uint64_t k_ready[2], v_ready[2], s_full[2], s_free[2], p_ready[2], pv_done[2], q_ready[2];
     AttnItem edge[2];
-    // per unit (mod 8: the copies are four units ahead of the softmax at most): no page; the tiles' powers of two; drafted slots whose values are not finite
-    uint32_t gone[8], k_lift[8], v_lift[8], odd[8][2];
+    // per unit (mod 8: the copies are four units ahead of the softmax at most): no page; the tiles' powers of two; drafted slots whose
+    // values are not finite; slots that count as zero
+    uint32_t gone[8], k_lift[8], v_lift[8], odd[8][2], drop[8][2];
     uint32_t tmem, last[2], span[2][2], bad_rows[kTmRows / 32];
 };
 
@@ -78,7 +83,17 @@ __device__ __forceinline__ void tm_mma64(uint32_t d, uint32_t a, uint32_t b_smem
 __device__ __forceinline__ void tm_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ bool tm_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, 1u << 21)); }
+// Bounded wait by a whole warp. Every try may sleep for up to a millisecond: sixteen warps that asked again at once took a sixth of the issue slots from the
+// others. Two seconds in all, then the caller gives up.
+__device__ __forceinline__ bool tm_wait(uint64_t* bar, uint32_t parity) {
+    const uint32_t at = smem_u32(bar);
+    uint32_t done = 0;
+#pragma unroll 1
+    for (uint32_t i = 0; i < 2000 && !done; ++i)
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(done) : "r"(at), "r"(parity), "r"(1000000u) : "memory");
+    return __all_sync(0xffffffffu, done != 0);
+}
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {   // two FP32 operations in one
     float2 d;
     asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
@@ -103,9 +118,9 @@ tree_mma_kernel(const AttnParams p) {
     const uint32_t tid = threadIdx.x, lane = tid % 32, warp = __shfl_sync(NONE, tid / 32, 0);
     pdl_launch_dependents();
     if (tid == 0) {
-        for (uint32_t i = 0; i < S::kStages; ++i) { mbar_init(&sm.code_full[i], 1); mbar_init(&sm.code_empty[i], 8); }
+        for (uint32_t i = 0; i < S::kStages; ++i) { mbar_init(&sm.code_full[i], 1); mbar_init(&sm.code_known[i], 1); mbar_init(&sm.code_empty[i], kTmTileWarps); }
         for (uint32_t i = 0; i < 2; ++i) {
-            mbar_init(&sm.k_ready[i], 8); mbar_init(&sm.v_ready[i], 8); mbar_init(&sm.s_full[i], 2); mbar_init(&sm.s_free[i], 4);
+            mbar_init(&sm.k_ready[i], kTmTileWarps); mbar_init(&sm.v_ready[i], kTmTileWarps); mbar_init(&sm.s_full[i], 2); mbar_init(&sm.s_free[i], 4);
             mbar_init(&sm.p_ready[i], 4); mbar_init(&sm.pv_done[i], 1); mbar_init(&sm.q_ready[i], 4);
         }
         mbar_fence_init();
@@ -126,128 +141,128 @@ tree_mma_kernel(const AttnParams p) {
     const uint32_t tmem = __shfl_sync(NONE, sm.tmem, 0), n = static_cast<uint32_t>(u1 - u0);
     auto part_at = [&](uint64_t block, bool at_start) { return p.parts + (2 * block + (at_start ? 0 : 1)) * tm_part_floats(); };
     bool ok = true;
-
-    if (warp == 0) {
-        // ---- copies: the lanes look up the groups of eight units, then the units go out one after another
-        for (uint32_t base = 0; base < n && ok; base += 8) {
-            const uint32_t j = base + lane / 4, part = lane % 4;
-            const uint8_t* src = nullptr;
-            bool wanted = false, bad = false;
-            if (j < n) {
-                const AttnItem it = item_of<kTmRows, kTmUnit>(p, sm.cum, u0 + j);
-                const uint64_t slot = (u0 + j - it.start) * kTmUnit + part * kKvGroup;
-                if (it.dead) bad = true;
-                else if (slot < it.total) {
-                    wanted = true;
-                    src = kv_group(p.cache, it.seq, slot, it.head, p.error);
-                    bad = !src;
+    // A role's warpgroup asks for its registers in its own branch, and goes back to the count at launch at its end: not before the softmax has been given
+    // what it asks for (a short role that took its own back first would leave it waiting), so all meet once that is done
+    if (warp < kTmSoftmax) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTmIssueRegs));
+        __syncthreads();
+        if (warp == 0) {
+            // ---- copies: the lanes look up the groups of eight units, then the units go out one after another
+            for (uint32_t base = 0; base < n && ok; base += 8) {
+                const uint32_t j = base + lane / 4, part = lane % 4;
+                const uint8_t* src = nullptr;
+                bool wanted = false, bad = false;
+                if (j < n) {
+                    const AttnItem it = item_of<kTmRows, kTmUnit>(p, sm.cum, u0 + j);
+                    const uint64_t slot = (u0 + j - it.start) * kTmUnit + part * kKvGroup;
+                    if (it.dead) bad = true;
+                    else if (slot < it.total) {
+                        wanted = true;
+                        src = kv_group(p.cache, it.seq, slot, it.head, p.error);
+                        bad = !src;
+                    }
                 }
-            }
-            const uint32_t bads = __ballot_sync(NONE, bad), wants = __ballot_sync(NONE, wanted);
-            const uint64_t first = __shfl_sync(NONE, reinterpret_cast<uint64_t>(src), lane & ~3u);
-            const uint32_t rows = __ballot_sync(NONE, reinterpret_cast<uint64_t>(src) == first + part * S::kGroupBytes);
-            for (uint32_t k = 0; k < 8 && base + k < n; ++k) {
-                const uint32_t u = base + k, st = u % S::kStages, round = u / S::kStages;
-                ok = !round || tm_wait(&sm.code_empty[st], (round - 1) & 1);
-                if (!ok) break;
-                const uint32_t gone = bads >> (4 * k) & 15u, want = gone ? 0u : wants >> (4 * k) & 15u;
-                if (elect_one()) {
-                    sm.gone[u % 8] = gone;
-                    mbar_arrive_expect_tx(&sm.code_full[st], __popc(want) * S::kGroupBytes);
-                }
-                __syncwarp();
-                const bool whole = want == 15u && (rows >> (4 * k) & 15u) == 15u;
-                if (lane / 4 == k && (whole ? part == 0 : (want >> part & 1) != 0))
-                    bulk_g2s(sm.ring[st] + part * S::kGroupBytes, src, whole ? S::kStage : S::kGroupBytes, &sm.code_full[st]);
-                __syncwarp();
-            }
-        }
-    } else if (warp == 1) {
-        // ---- MMAs: QK of a unit, then PV of the unit before
-        uint64_t end = u0;
-        uint32_t item = 0;
-        bool fresh_next = true;
-        for (uint32_t j = 0; j <= n; ++j) {
-            const bool fresh = fresh_next;   // of unit j - 1: its PV starts an accumulator
-            if (j < n) {
-                if (u0 + j >= end) {
-                    end = item_of<kTmRows, kTmUnit>(p, sm.cum, u0 + j).end;
-                    ok = tm_wait(&sm.q_ready[item & 1], (item >> 1) & 1);
+                const uint32_t bads = __ballot_sync(NONE, bad), wants = __ballot_sync(NONE, wanted);
+                const uint64_t first = __shfl_sync(NONE, reinterpret_cast<uint64_t>(src), lane & ~3u);
+                const uint32_t rows = __ballot_sync(NONE, reinterpret_cast<uint64_t>(src) == first + part * S::kGroupBytes);
+                for (uint32_t k = 0; k < 8 && base + k < n; ++k) {
+                    const uint32_t u = base + k, st = u % S::kStages, round = u / S::kStages;
+                    ok = !round || tm_wait(&sm.code_empty[st], (round - 1) & 1);
                     if (!ok) break;
-                    ++item;
-                    fresh_next = true;
-                } else fresh_next = false;
-                const uint32_t buf = j & 1, turn = (j >> 1) & 1;
-                ok = tm_wait(&sm.k_ready[buf], turn) && (j < 2 || tm_wait(&sm.s_free[buf], turn ^ 1));
-                if (!ok) break;
-                tm_fence_after();
-                if (elect_one()) {
-                    const uint32_t q = tmem + S::kQ + ((item - 1) & 1) * (D / 2), s = tmem + S::kS + buf * kTmUnit;
-#pragma unroll
-                    for (uint32_t part = 0; part < S::kParts; ++part)
-#pragma unroll
-                        for (uint32_t c = 0; c < D / 64; ++c) tm_mma64<kTmUnit>(s, q + c * 32, smem_u32(sm.k[buf][part]) + c * (kTmUnit * 128), part | c);
-                    mbar_arrive(&sm.s_full[buf]);   // what the tile warps say of the unit
-                    tm_commit(&sm.s_full[buf]);
+                    const uint32_t gone = bads >> (4 * k) & 15u, want = gone ? 0u : wants >> (4 * k) & 15u;
+                    if (elect_one()) {
+                        sm.gone[u % 8] = gone;
+                        mbar_arrive_expect_tx(&sm.code_full[st], __popc(want) * S::kGroupBytes);
+                    }
+                    __syncwarp();
+                    const bool whole = want == 15u && (rows >> (4 * k) & 15u) == 15u;
+                    if (lane / 4 == k && (whole ? part == 0 : (want >> part & 1) != 0))
+                        bulk_g2s(sm.ring[st] + part * S::kGroupBytes, src, whole ? S::kStage : S::kGroupBytes, &sm.code_full[st]);
+                    __syncwarp();
                 }
-                __syncwarp();
             }
-            if (j) {
-                const uint32_t buf = (j - 1) & 1, turn = ((j - 1) >> 1) & 1;
-                ok = tm_wait(&sm.v_ready[buf], turn) && tm_wait(&sm.p_ready[buf], turn);
-                if (!ok) break;
-                tm_fence_after();
-                if (elect_one()) {
+        } else if (warp == 1) {
+            // ---- MMAs: QK of a unit, then PV of the unit before
+            uint64_t end = u0;
+            uint32_t item = 0;
+            bool fresh_next = true;
+            for (uint32_t j = 0; j <= n; ++j) {
+                const bool fresh = fresh_next;   // of unit j - 1: its PV starts an accumulator
+                if (j < n) {
+                    if (u0 + j >= end) {
+                        end = item_of<kTmRows, kTmUnit>(p, sm.cum, u0 + j).end;
+                        ok = tm_wait(&sm.q_ready[item & 1], (item >> 1) & 1);
+                        if (!ok) break;
+                        ++item;
+                        fresh_next = true;
+                    } else fresh_next = false;
+                    const uint32_t buf = j & 1, turn = (j >> 1) & 1;
+                    ok = tm_wait(&sm.k_ready[buf], turn) && (j < 2 || tm_wait(&sm.s_free[buf], turn ^ 1));
+                    if (!ok) break;
+                    tm_fence_after();
+                    if (elect_one()) {
+                        const uint32_t q = tmem + S::kQ + ((item - 1) & 1) * (D / 2), s = tmem + S::kS + buf * kTmUnit;
 #pragma unroll
-                    for (uint32_t part = 0; part < S::kParts; ++part)
-                        tm_mma64<D>(tmem + S::kO, tmem + S::kP + buf * (kTmUnit / 2), smem_u32(sm.v[buf][part]), part | (fresh ? 0u : 1u));
-                    tm_commit(&sm.pv_done[buf]);
+                        for (uint32_t part = 0; part < S::kParts; ++part)
+#pragma unroll
+                            for (uint32_t c = 0; c < D / 64; ++c) tm_mma64<kTmUnit>(s, q + c * 32, smem_u32(sm.k[buf][part]) + c * (kTmUnit * 128), part | c);
+                        mbar_arrive(&sm.s_full[buf]);   // what the tile warps say of the unit
+                        tm_commit(&sm.s_full[buf]);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
+                if (j) {
+                    const uint32_t buf = (j - 1) & 1, turn = ((j - 1) >> 1) & 1;
+                    ok = tm_wait(&sm.v_ready[buf], turn) && tm_wait(&sm.p_ready[buf], turn);
+                    if (!ok) break;
+                    tm_fence_after();
+                    if (elect_one()) {
+#pragma unroll
+                        for (uint32_t part = 0; part < S::kParts; ++part)
+                            tm_mma64<D>(tmem + S::kO, tmem + S::kP + buf * (kTmUnit / 2), smem_u32(sm.v[buf][part]), part | (fresh ? 0u : 1u));
+                        tm_commit(&sm.pv_done[buf]);
+                    }
+                    __syncwarp();
+                }
             }
-        }
-    } else if (warp == 2) {
-        if (lane < 2) sm.edge[lane] = item_of<kTmRows, kTmUnit>(p, sm.cum, lane ? u1 - 1 : u0);
-    } else if (warp >= kTmTiles) {
-        // ---- tiles: a warp takes every eighth row of 512 bytes of K, then of V
-        const uint32_t w = warp - kTmTiles, g = lane / 4, t = lane % 4;
-        uint64_t end = u0, start = 0, length = 0, total = 0;
-        for (uint32_t j = 0; j < n; ++j) {
-            if (u0 + j >= end) {
-                const AttnItem it = item_of<kTmRows, kTmUnit>(p, sm.cum, u0 + j);
-                end = it.end; start = it.start; length = it.length; total = it.total;
-            }
-            const uint32_t st = j % S::kStages, buf = j & 1, turn = (j >> 1) & 1;
-            ok = tm_wait(&sm.code_full[st], (j / S::kStages) & 1) && (j < 2 || tm_wait(&sm.s_full[buf], turn ^ 1));   // QK of unit j - 2 has read this K tile
-            if (!ok) break;
-            const uint8_t* stage = sm.ring[st];
-            const bool gone = sm.gone[j % 8] != 0;
-            const uint64_t slot0 = (u0 + j - start) * kTmUnit;
-            const bool edge = slot0 + kTmUnit > length;
-            uint64_t there = ~0ull, drop = 0;   // slots of this unit that exist; that count as zero
-            float k_up = 1.f, v_up = 1.f;
-            if (!gone) {
-                if (edge) {
-                    there = total - slot0 >= 64 ? ~0ull : (1ull << (total - slot0)) - 1;
+        } else if (warp == 2) {
+            if (lane < 2) sm.edge[lane] = item_of<kTmRows, kTmUnit>(p, sm.cum, lane ? u1 - 1 : u0);
+        } else if (warp == 3) {
+            // ---- what there is to know of a unit before its tiles are made: slots that count as zero, largest scales
+            uint64_t end = u0, start = 0, length = 0, total = 0;
+            for (uint32_t j = 0; j < n; ++j) {
+                if (u0 + j >= end) {
+                    const AttnItem it = item_of<kTmRows, kTmUnit>(p, sm.cum, u0 + j);
+                    end = it.end; start = it.start; length = it.length; total = it.total;
+                }
+                const uint32_t st = j % S::kStages;
+                ok = tm_wait(&sm.code_full[st], (j / S::kStages) & 1);
+                if (!ok) break;
+                const uint8_t* stage = sm.ring[st];
+                const uint64_t slot0 = (u0 + j - start) * kTmUnit;
+                uint64_t drop = 0, odd_slots = 0;
+                const bool gone = sm.gone[j % 8] != 0, edge = slot0 + kTmUnit > length;
+                if (edge && !gone) {
+                    const uint64_t there = total - slot0 >= 64 ? ~0ull : (1ull << (total - slot0)) - 1;
                     const uint64_t drafted = slot0 >= length ? ~0ull : ~0ull << (length - slot0);
                     uint32_t odd[2] = {0, 0};
                     if constexpr (Q8) {
                         for (uint32_t i = lane; i < kTmGroups * NB * kKvGroup; i += 32) {
                             const uint32_t gi = i / (NB * kKvGroup), x = i % (NB * kKvGroup), slot = gi * kKvGroup + x % kKvGroup;
-                            const bool is = (*reinterpret_cast<const uint16_t*>(stage + gi * S::kGroupBytes + S::kHalf + kKvGroup * D + x * 2) & 0x7c00u) == 0x7c00u;
-                            odd[slot / 32] |= static_cast<uint32_t>(is) << slot % 32;
+                            const uint32_t is = (*reinterpret_cast<const uint16_t*>(stage + gi * S::kGroupBytes + S::kHalf + kKvGroup * D + x * 2) & 0x7c00u) == 0x7c00u;
+                            if (slot < 32) odd[0] |= is << slot; else odd[1] |= is << (slot - 32);
                         }
                     } else {
                         for (uint32_t i = lane; i < kTmUnit * D; i += 32) {   // halves of V: [group][32 dims][m][g][t][i][e]
                             const uint32_t gi = i / (kKvGroup * D), x = i % (kKvGroup * D), e = x % 4, tt = x / 8 % 4, slot = gi * kKvGroup + 2 * tt + (e & 1) + 8 * (e >> 1);
-                            const bool is = (*reinterpret_cast<const uint16_t*>(stage + gi * S::kGroupBytes + S::kHalf + x * 2) & 0x7c00u) == 0x7c00u;
-                            odd[slot / 32] |= static_cast<uint32_t>(is) << slot % 32;
+                            const uint32_t is = (*reinterpret_cast<const uint16_t*>(stage + gi * S::kGroupBytes + S::kHalf + x * 2) & 0x7c00u) == 0x7c00u;
+                            if (slot < 32) odd[0] |= is << slot; else odd[1] |= is << (slot - 32);
                         }
                     }
-                    const uint64_t all = (static_cast<uint64_t>(__reduce_or_sync(NONE, odd[1])) << 32 | __reduce_or_sync(NONE, odd[0])) & drafted & there;
-                    drop = all | ~there;
-                    if (w == 0 && lane == 0) { sm.odd[j % 8][0] = static_cast<uint32_t>(all); sm.odd[j % 8][1] = static_cast<uint32_t>(all >> 32); }
+                    odd_slots = (static_cast<uint64_t>(__reduce_or_sync(NONE, odd[1])) << 32 | __reduce_or_sync(NONE, odd[0])) & drafted & there;
+                    drop = odd_slots | ~there;
                 }
+                int ek = 21, ev = 21;
                 if constexpr (Q8) {   // largest scales: below 2^(e - 14), e the binary16 exponent; the tiles are times 2^(21 - e), codes times scales below 2^14
                     uint32_t top[2];
 #pragma unroll
@@ -264,15 +279,40 @@ tree_mma_kernel(const AttnParams p) {
                         const uint32_t most = __vmaxu2(__vmaxu2(words[0], words[1]), __vmaxu2(words[2], words[3]));
                         top[side] = max(most & 0xffffu, most >> 16);
                     }
-                    const int ek = static_cast<int>(min(max(__reduce_max_sync(NONE, top[0]) >> 10, 1u), 30u)), ev = static_cast<int>(min(max(__reduce_max_sync(NONE, top[1]) >> 10, 1u), 30u));
-                    k_up = pow2(21 - ek); v_up = pow2(21 - ev);
-                    if (w == 0 && lane == 0) { sm.k_lift[j % 8] = 21 - ek; sm.v_lift[j % 8] = 21 - ev; }
+                    ek = static_cast<int>(min(max(__reduce_max_sync(NONE, top[0]) >> 10, 1u), 30u));
+                    ev = static_cast<int>(min(max(__reduce_max_sync(NONE, top[1]) >> 10, 1u), 30u));
                 }
+                if (lane == 0) {
+                    sm.k_lift[j % 8] = 21 - ek; sm.v_lift[j % 8] = 21 - ev;
+                    sm.odd[j % 8][0] = static_cast<uint32_t>(odd_slots); sm.odd[j % 8][1] = static_cast<uint32_t>(odd_slots >> 32);
+                    sm.drop[j % 8][0] = static_cast<uint32_t>(drop); sm.drop[j % 8][1] = static_cast<uint32_t>(drop >> 32);
+                    mbar_arrive(&sm.code_known[st]);
+                }
+                __syncwarp();
+            }
+        }
+        __syncwarp();
+        __syncthreads();   // a warp that asked for registers now would keep asking until the others are done
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTmLaunchRegs));
+    } else if (warp >= kTmTiles) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTmTileRegs));
+        __syncthreads();
+        // ---- tiles: a warp takes every 16th row of 512 bytes of K, then of V
+        const uint32_t w = warp - kTmTiles, g = lane / 4, t = lane % 4;
+        for (uint32_t j = 0; j < n; ++j) {
+            const uint32_t st = j % S::kStages, buf = j & 1, turn = (j >> 1) & 1;
+            ok = tm_wait(&sm.code_known[st], (j / S::kStages) & 1) && tm_wait(&sm.code_full[st], (j / S::kStages) & 1) && (j < 2 || tm_wait(&sm.s_full[buf], turn ^ 1));   // QK of unit j - 2 has read this K tile
+            if (!ok) break;
+            const uint8_t* stage = sm.ring[st];
+            const bool gone = sm.gone[j % 8] != 0;
+            const float k_up = pow2(static_cast<int>(sm.k_lift[j % 8])), v_up = pow2(static_cast<int>(sm.v_lift[j % 8]));
+            if (!gone) {
                 // K: [64 dims][64 slots] rows of 128 bytes; a lane's 16 bytes are dims 8 t.. of both 32s (Q8_0) or 8 t.. of one (binary16) of slot 8 n + g
 #pragma unroll
-                for (uint32_t i = 0; i < K_LINES * kTmGroups / 8; ++i) {
+                for (uint32_t i = 0; i < (K_LINES * kTmGroups + kTmTileWarps - 1) / kTmTileWarps; ++i) {
                     constexpr uint32_t LINES = K_LINES;
-                    const uint32_t line = i * 8 + w;
+                    const uint32_t line = i * kTmTileWarps + w;
+                    if (line >= LINES * kTmGroups) break;   // head_dim 64: half of the warps
                     const uint32_t gi = line / LINES, x = line % LINES, in = x % 2 * 8 + g, slot = gi * kKvGroup + in;
                     const uint8_t* group = stage + gi * S::kGroupBytes;
                     const uint4 c = *reinterpret_cast<const uint4*>(group + x * 512 + lane * 16);
@@ -316,14 +356,15 @@ tree_mma_kernel(const AttnParams p) {
             if (!gone) {
                 // V: [dims][64 slots], rows of 128 bytes; a lane's 16 bytes are dims 8 i + g, slots 2 t, 2 t + 1, 8 more
 #pragma unroll
-                for (uint32_t i = 0; i < K_LINES * kTmGroups / 8; ++i) {
-                    const uint32_t line = i * 8 + w, gi = line / K_LINES, x = line % K_LINES;
+                for (uint32_t i = 0; i < (K_LINES * kTmGroups + kTmTileWarps - 1) / kTmTileWarps; ++i) {
+                    const uint32_t line = i * kTmTileWarps + w, gi = line / K_LINES, x = line % K_LINES;
+                    if (line >= K_LINES * kTmGroups) break;
                     const uint8_t* values = stage + gi * S::kGroupBytes + S::kHalf;
                     const uint4 c = *reinterpret_cast<const uint4*>(values + x * 512 + lane * 16);
                     const uint32_t words[4] = {c.x, c.y, c.z, c.w};
                     uint32_t keep[2] = {NONE, NONE};
-                    if (edge) {
-                        const uint32_t out = static_cast<uint32_t>(drop >> (gi * kKvGroup)) & 0xffffu;
+                    const uint32_t out = sm.drop[j % 8][gi / 2] >> (gi % 2 * kKvGroup) & 0xffffu;
+                    if (out) {
 #pragma unroll
                         for (uint32_t h = 0; h < 2; ++h) keep[h] = (out >> (8 * h + 2 * t) & 1 ? 0u : 0x0000ffffu) | (out >> (8 * h + 2 * t) & 2 ? 0u : 0xffff0000u);
                     }
@@ -360,7 +401,12 @@ tree_mma_kernel(const AttnParams p) {
             __syncwarp();
             if (lane == 0) { mbar_arrive(&sm.v_ready[buf]); mbar_arrive(&sm.code_empty[st]); }
         }
-    } else if (warp >= kTmSoftmax) {
+        __syncwarp();
+        __syncthreads();   // a warp that asked for registers now would keep asking until the others are done
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTmLaunchRegs));
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTmSoftmaxRegs));
+        __syncthreads();
         // ---- softmax: a thread per query row
         const uint32_t quarter = warp - kTmSoftmax, r = quarter * 32 + lane, base = tmem + (quarter << 21);   // the warp's lanes of tensor memory
         const float f = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-25f);   // not 0: it multiplies minus infinity
@@ -440,10 +486,10 @@ tree_mma_kernel(const AttnParams p) {
                         else if (sm.odd[j % 8][c / 32] >> (c % 32) & 1) s[c / 32][c % 32] = NAN;
                     }
                 }
-                float x = -INFINITY;
+                float x4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (uint32_t c = 0; c < 64; ++c) x = fmaxf(x, s[c / 32][c % 32]);
-                x *= fj;
+                for (uint32_t c = 0; c < 64; ++c) x4[c % 4] = fmaxf(x4[c % 4], s[c / 32][c % 32]);
+                const float x = fmaxf(fmaxf(x4[0], x4[1]), fmaxf(x4[2], x4[3])) * fj;
                 const bool fresh = j == first;
                 if (__any_sync(NONE, x > limit) || v_lift < lift) {
                     float old = 1.f;
@@ -475,16 +521,17 @@ tree_mma_kernel(const AttnParams p) {
                 // V tiles at a higher power of two than the accumulator: the weights take what is between, and the sum gives it back
                 const float shift = Q8 ? max(static_cast<float>(lift - v_lift), -100.f) : 0.f;
                 uint32_t w[32];
-                float2 sum = make_float2(0.f, 0.f);
+                float2 sum[4] = {};
                 const float2 fj2 = make_float2(fj, fj), ref2 = make_float2(ref + shift, ref + shift);
 #pragma unroll
                 for (uint32_t c = 0; c < 32; ++c) {
                     float2 x2 = fma2(make_float2(s[c / 16][2 * c % 32], s[c / 16][2 * c % 32 + 1]), fj2, ref2);
                     x2.x = exp2_approx(x2.x); x2.y = exp2_approx(x2.y);
-                    sum = add2(sum, x2);
+                    sum[c % 4] = add2(sum[c % 4], x2);
                     w[c] = h2_bits(__floats2half2_rn(x2.x, x2.y));
                 }
-                l = fmaf(sum.x + sum.y, Q8 ? exp2_approx(-shift) : 1.f, l);
+                sum[0] = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+                l = fmaf(sum[0].x + sum[0].y, Q8 ? exp2_approx(-shift) : 1.f, l);
                 ok = j < 2 || tm_wait(&sm.pv_done[buf], turn ^ 1);   // PV of unit j - 2 has read this buffer
                 if (!ok) break;
                 tm_fence_after();
@@ -548,6 +595,9 @@ tree_mma_kernel(const AttnParams p) {
             }
             tm_fence_before();   // the accumulator is read before the next item's first weights are said to be ready
         }
+        __syncwarp();
+        __syncthreads();   // a warp that asked for registers now would keep asking until the others are done
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTmLaunchRegs));
     }
     if (!ok && lane == 0) raise_error(p.error, TSP_ERR_TIMEOUT);
     tm_fence_before();
@@ -574,8 +624,8 @@ tree_mma_kernel(const AttnParams p) {
     }
     if (tid < kTmRows / 32) sm.bad_rows[tid] = 0;
     __syncthreads();
-    const uint32_t r = tid % kTmRows, lot = tid / kTmRows;   // a row by four threads, each every fourth float4
-    constexpr uint32_t LOTS = kTmThreads / kTmRows, V = D / 4 / LOTS;
+    const uint32_t r = tid % kTmRows, lot = tid / kTmRows;   // a row by four threads, each every fourth float4; the other warps only meet them
+    constexpr uint32_t LOTS = 4, V = D / 4 / LOTS;
 #pragma unroll 1
     for (uint32_t side = 0; side < 2; ++side) {
         if (!sm.last[side]) continue;
@@ -587,12 +637,12 @@ tree_mma_kernel(const AttnParams p) {
         float top = -INFINITY, sum = 0.f;
         bool dead = false;
 #pragma unroll 4
-        for (uint32_t i = 0; i < pieces; ++i) top = fmaxf(top, load_piece(part_of(i) + r));
+        for (uint32_t i = 0; i < (lot < LOTS ? pieces : 0); ++i) top = fmaxf(top, load_piece(part_of(i) + r));
         float4 y[V];
 #pragma unroll
         for (uint32_t k = 0; k < V; ++k) y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-        for (uint32_t i = 0; i < pieces; ++i) {
+#pragma unroll 1
+        for (uint32_t i = 0; i < (lot < LOTS ? pieces : 0); ++i) {
             const float* part = part_of(i);
             const float m = load_piece(part + r), l = load_piece(part + kTmRows + r), fi = weight_of(m, top);
             dead |= load_piece(part + 2 * kTmRows) != 0.f;
@@ -613,9 +663,9 @@ tree_mma_kernel(const AttnParams p) {
             y[k].x *= inv; y[k].y *= inv; y[k].z *= inv; y[k].w *= inv;
             good &= in_range<true>(y[k].x) && in_range<true>(y[k].y) && in_range<true>(y[k].z) && in_range<true>(y[k].w);
         }
-        if (!good && r < it.rows) atomicOr(&sm.bad_rows[r / 32], 1u << r % 32);
+        if (!good && r < it.rows && lot < LOTS) atomicOr(&sm.bad_rows[r / 32], 1u << r % 32);
         __syncthreads();
-        if (r < it.rows) {
+        if (r < it.rows && lot < LOTS) {
             const bool bad = sm.bad_rows[r / 32] >> r % 32 & 1;
             if (bad && !dead && lot == 0) raise_error(p.error, TSP_ERR_NONFINITE);
             const uint32_t flat = it.tile * kTmRows + r, node = flat / p.group, head = it.head * p.group + flat % p.group;
@@ -636,6 +686,13 @@ template <uint32_t D, bool Q8>
 static int launch_tree_mma_t(const AttnParams& p, cudaStream_t st) {
     constexpr size_t smem = sizeof(TmSmem<D, Q8>) + 1024;
     static_assert(smem <= 232448, "shared memory of a block");
+    static thread_local int regs_ok = -1;
+    if (regs_ok < 0) {
+        cudaFuncAttributes fa;
+        TSP_CUDA(cudaFuncGetAttributes(&fa, tree_mma_kernel<D, Q8>));
+        regs_ok = fa.numRegs == kTmLaunchRegs;
+    }
+    if (!regs_ok) return fail(TSP_E_CUDA, "attention: the kernel's register count does not allow its hand-over");
     static thread_local SmemAttrCache attr;
     TSP_CUDA(ensure_dynamic_smem(tree_mma_kernel<D, Q8>, attr, smem));
     const int sms = sm_count();
