@@ -558,3 +558,44 @@ def test_pages_behind_four_gigabytes():
         ck, cv = R.cached(k[off[s]:off[s + 1]], "q8_0"), R.cached(v[off[s]:off[s + 1]], "q8_0")
         want, spread, vmax = R.attended(q[s], ck, cv, np.ones(counts[s], bool), dim ** -0.5)
         assert np.abs(out[s].cpu().numpy() - want).max() <= vmax * (4 * 136 * U32 * spread + (counts[s] + 64) * U32)
+
+
+@pytest.mark.parametrize("type_,dim,heads,group,counts,lengths", [("q8_0", 128, 8, 4, [17, 32], [9000, 3001]), ("q8_0", 128, 4, 4, [64], [30011]), ("f16", 128, 4, 8, [5, 33, 2], [12007, 4095, 64]),
+                                                                  ("q8_0", 64, 8, 8, [9], [20000]), ("f16", 64, 8, 3, [6, 21], [16000, 9999]), ("q8_0", 256, 4, 2, [4, 1], [14000, 8000]),
+                                                                  ("q8_0", 128, 8, 1, [1] * 24, [100 * i for i in range(24)]), ("f16", 128, 2, 6, [2], [40000])])
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_long_runs(type_, dim, heads, group, counts, lengths, dtype):
+    """Contexts that give every block more units than its stages hold, of several items or of one; the cache is written and read back by its own
+    operators, and torch in 64 bits attends over what it holds."""
+    g = torch.Generator(device="cuda").manual_seed(dim + len(counts))
+    page, total = 64, [a + b for a, b in zip(counts, lengths)]
+    need = [-(-n // page) for n in total]
+    table = np.full((len(total), max(need)), 0xffffffff, np.uint32)
+    order, at = np.random.default_rng(1).permutation(sum(need) + 1), 0
+    for s, n in enumerate(need):
+        table[s, :n] = order[at:at + n]
+        at += n
+    pool = torch.full((sum(need) + 1, A.page_bytes(type_, page, heads, dim)), 255, dtype=torch.uint8, device="cuda")
+    cache, err = A.KvCache(pool, dev(table), page, heads, dim, type_), error_word()
+    everything, off = make_batch(total, [0] * len(total))
+    k, v = (torch.randn(sum(total), heads, dim, generator=g, device="cuda") for _ in range(2))
+    A.kv_cache_append(cache, everything, k, v, err)
+    A.kv_cache_read(cache, everything, k, v, err)
+    rows = sum(counts)
+    q = torch.randn(rows, heads * group, dim, generator=g, device="cuda").to(torch.float32 if dtype == "f32" else torch.float16)
+    batch, first = make_batch(counts, lengths)
+    out, scratch = torch.empty_like(q), A.tree_attention_scratch()
+    for _ in range(3):
+        out.fill_(11)
+        A.tree_attention(cache, batch, q, out, None, max(counts), dim ** -0.5, scratch, err)
+    assert int(err) == 0
+    num = den = 0.0
+    for s in range(len(counts)):
+        n, L = counts[s], lengths[s]
+        kk, vv = (x[off[s]:off[s + 1]].double().permute(1, 0, 2).repeat_interleave(group, 0) for x in (k, v))
+        x = q[first[s]:first[s + 1]].double().permute(1, 0, 2) @ kk.transpose(1, 2) * dim ** -0.5
+        visible = torch.arange(L + n, device="cuda")[None] <= L + torch.arange(n, device="cuda")[:, None]
+        want = (torch.softmax(x.masked_fill(~visible, -np.inf), -1) @ vv).permute(1, 0, 2)
+        d = out[first[s]:first[s + 1]].double() - want
+        num, den = num + float((d * d).sum()), den + float((want * want).sum())
+    assert np.sqrt(num / den) <= (2e-3 if dtype == "f16" else 5e-6)

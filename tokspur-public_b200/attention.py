@@ -15,22 +15,31 @@ STYLES = {"halves": capi.ROPE_HALVES, "pairs": capi.ROPE_PAIRS}
 SIZES = {torch.float32: 4, torch.float16: 2}   # of the row types; the library's dtype is 0 for four bytes, 1 for two
 
 
+def _refuse(name, t, dtype, heads, dim, least):
+    raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device} does not hold {least} rows of {heads} densely packed heads of {dim} {dtype}")
+
+
 def _rows(name: str, t: torch.Tensor, dtype: torch.dtype, heads: int, dim: int, least: int) -> tuple[int, int]:
-    """Pointer and row stride in bytes of [rows, heads, dim], after the checks that the library cannot make."""
-    shape, stride = t.shape, t.stride()
-    if len(shape) != 3 or shape[1] != heads or shape[2] != dim or shape[0] < least or stride[2] != 1 or (stride[1] != dim and heads > 1) \
-            or t.dtype is not dtype or dtype not in SIZES or not t.is_cuda:
-        raise ValueError(f"{name}: {t.dtype} {tuple(shape)} with strides {stride} on {t.device} does not hold {least} rows of {heads} densely packed heads of {dim} {dtype}")
+    """Pointer and row stride in bytes of [rows, heads, dim], after the checks that the library cannot make. A call of a few microseconds is
+    in good part these lines: they ask each tensor as little as they can."""
+    stride = t.stride()
+    if len(stride) != 3 or stride[2] != 1 or (stride[1] != dim and heads > 1) or t.dtype is not dtype:
+        _refuse(name, t, dtype, heads, dim, least)
+    rows, h, d = t.shape
+    if h != heads or d != dim or rows < least:
+        _refuse(name, t, dtype, heads, dim, least)
     return t.data_ptr(), stride[0] * SIZES[dtype]
 
 
 def _words(name: str, t: torch.Tensor, dtype: torch.dtype, least: int) -> int:
-    if t.dtype is not dtype or t.numel() < least or not t.is_contiguous() or not t.is_cuda:
-        raise ValueError(f"{name}: {least} dense values of {dtype} on a CUDA device")
+    if t.dtype is not dtype or t.numel() < least or not t.is_contiguous():
+        raise ValueError(f"{name}: {least} dense values of {dtype}")
     return t.data_ptr()
 
 
 _entries: dict = {}
+# the current stream's handle without a Stream object around it (a microsecond less a call), where torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _call(name: str, like: torch.Tensor, error: torch.Tensor | None, *args) -> None:
@@ -40,9 +49,11 @@ def _call(name: str, like: torch.Tensor, error: torch.Tensor | None, *args) -> N
         entry = _entries[name] = getattr(capi.lib(), name)
     device = like.get_device()
     if device != torch.cuda.current_device():
+        if device < 0:
+            raise ValueError(f"{name}: rows on {like.device}")
         with torch.cuda.device(device):
             return _call(name, like, error, *args)
-    rc = entry(*args, None if error is None else error.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    rc = entry(*args, None if error is None else error.data_ptr(), _raw_stream(device))
     if rc:
         capi.check(rc)
 

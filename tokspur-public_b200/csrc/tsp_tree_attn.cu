@@ -63,8 +63,10 @@ tree_attention_kernel(const AttnParams p) {
     if (lane < 2) sm.key[warp][lane] = ~0ull;
     unit_prefix<R, kKvGroup, S::kThreads>(p, sm.cum, sm.warp_sums);
     const uint64_t units = sm.cum[p.batch.sequences];
-    const uint64_t quota = max(static_cast<uint64_t>(kLeastUnits), (units + gridDim.x - 1) / gridDim.x);
-    const uint64_t u0 = min(units, blockIdx.x * quota), u1 = min(units, u0 + quota);
+    if (!units) return;
+    const AttnRuns runs(p, units, item_of<R>(p, sm.cum, 0));
+    uint64_t u0, u1;
+    runs.run(blockIdx.x, units, u0, u1);
     if (u0 >= u1) return;
 
     // ---- a warp's run. A lane has two rows (ra, rb) and, of a unit's 16 slots, four scores of each with R = 16, two with R = 8. s[4 * n + c], with
@@ -542,10 +544,10 @@ tree_attention_kernel(const AttnParams p) {
                     const AttnItem& it = tid ? last : first;
                     uint32_t joins = 0;
                     if (tid ? open1 : open0) {
-                        const uint32_t c0 = static_cast<uint32_t>(it.start / quota), c1 = static_cast<uint32_t>((it.end - 1) / quota);
-                        joins = atomicAdd(p.counters + c0, 1u) == c1 - c0;
+                        const uint32_t c0 = runs.first(it.start), count = runs.count(it.start, it.end);
+                        joins = atomicAdd(p.counters + c0, 1u) == count - 1;
                         if (joins) p.counters[c0] = 0;
-                        sm.span[tid][0] = c0; sm.span[tid][1] = c1 - c0 + 1;
+                        sm.span[tid][0] = c0; sm.span[tid][1] = count;
                     }
                     sm.last[tid] = joins;
                     __threadfence();
@@ -557,7 +559,7 @@ tree_attention_kernel(const AttnParams p) {
             item = mine ? &last : &first;
             const uint32_t c0 = sm.span[mine][0];
             n = sm.span[mine][1];
-            p0 = block_part(c0, item->start == c0 * quota);
+            p0 = block_part(c0, runs.at_run_start(item->start));
             p1 = block_part(c0 + 1, true);
             stride = 2 * static_cast<uint32_t>(part_floats());
             pl = n > 1 ? p1 + static_cast<uint64_t>(n - 2) * stride : p0;

@@ -157,4 +157,38 @@ __device__ __forceinline__ void unit_prefix(const AttnParams& p, uint64_t* cum, 
     __syncthreads();
 }
 
+// Which units a block runs over, and which blocks an item has. The units of a ragged batch are dealt in equal runs, whatever item they are of. A single
+// sequence's items (heads, row tiles) are all alike: where there are no more of them than blocks, every item gets the same number of blocks of its
+// own, so that no block has pieces of two to join (one row over 4096 slots: 19 us against 15).
+struct AttnRuns {
+    uint64_t quota, item;   // units of a block's run; of an item where items have blocks of their own, else 0
+    uint32_t blocks;        // of an item then
+
+    __device__ __forceinline__ AttnRuns(const AttnParams& p, uint64_t units, const AttnItem& any) : item(0), blocks(0) {
+        const uint64_t each = any.end - any.start, items = units / each;
+        if (p.batch.sequences == 1 && items <= gridDim.x) {
+            item = each;
+            blocks = gridDim.x / static_cast<uint32_t>(items);
+            quota = max(static_cast<uint64_t>(kLeastUnits), (each + blocks - 1) / blocks);
+        } else quota = max(static_cast<uint64_t>(kLeastUnits), (units + gridDim.x - 1) / gridDim.x);
+    }
+    __device__ __forceinline__ void run(uint32_t block, uint64_t units, uint64_t& u0, uint64_t& u1) const {
+        if (item) {
+            const uint64_t start = block / blocks * item;
+            u0 = min(start + block % blocks * quota, start + item);
+            u1 = min(u0 + quota, start + item);
+            if (start >= units) u0 = u1 = units;
+        } else {
+            u0 = min(units, block * quota);
+            u1 = min(units, u0 + quota);
+        }
+    }
+    // first block of the item that starts at unit `start`, and how many it has
+    __device__ __forceinline__ uint32_t first(uint64_t start) const { return static_cast<uint32_t>(item ? start / item * blocks : start / quota); }
+    __device__ __forceinline__ uint32_t count(uint64_t start, uint64_t end) const {
+        return static_cast<uint32_t>(item ? (item + quota - 1) / quota : (end - 1) / quota - start / quota + 1);
+    }
+    __device__ __forceinline__ bool at_run_start(uint64_t start) const { return item != 0 || start % quota == 0; }   // of that first block
+};
+
 }  // namespace tsp

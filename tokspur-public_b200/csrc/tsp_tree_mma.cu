@@ -17,11 +17,11 @@
 namespace tsp {
 
 constexpr uint32_t kTmRows = 128, kTmUnit = 64, kTmGroups = kTmUnit / kKvGroup;
-constexpr uint32_t kTmSoftmax = 4, kTmTiles = 8, kTmTileWarps = 16, kTmThreads = 32 * (kTmTiles + kTmTileWarps);   // first softmax warp, first tile warp
+constexpr uint32_t kTmSoftmax = 4, kTmTiles = 8, kTmTileWarps = 8, kTmThreads = 32 * (kTmTiles + kTmTileWarps);   // first softmax warp, first tile warp
 // Registers after the hand-over between the warpgroups (setmaxnreg): together no more than the count at launch (80) times the six warpgroups, or the softmax
 // would wait for ever; the launcher checks it. At the end all go back to that count.
-constexpr int kTmLaunchRegs = 80, kTmIssueRegs = 64, kTmSoftmaxRegs = 160, kTmTileRegs = 64;
-static_assert(kTmIssueRegs + kTmSoftmaxRegs + 4 * kTmTileRegs <= 6 * kTmLaunchRegs, "hand-over of registers");
+constexpr int kTmLaunchRegs = 128, kTmIssueRegs = 104, kTmSoftmaxRegs = 192, kTmTileRegs = 104;
+static_assert(kTmIssueRegs + kTmSoftmaxRegs + kTmTileWarps / 4 * kTmTileRegs <= (2 + kTmTileWarps / 4) * kTmLaunchRegs, "hand-over of registers");
 // piece of an item: references and sums of 128 rows, a flag, then the rows' dims four by four, rows side by side: [dim / 4][row][4]
 constexpr uint32_t kTmPartHead = 288;
 __host__ __device__ constexpr uint64_t tm_part_floats() { return kTmPartHead + kTmRows * 128; }
@@ -29,7 +29,7 @@ __host__ __device__ constexpr uint64_t tm_part_floats() { return kTmPartHead + k
 template <uint32_t D, bool Q8>
 struct TmShape {
     static constexpr uint32_t kGroupBytes = kv_group_bytes(D, Q8), kHalf = kv_half_bytes(D, Q8), kStage = kTmGroups * kGroupBytes;
-    static constexpr uint32_t kStages = 3, kParts = Q8 ? 2 : 1;                        // parts: high, low
+    static constexpr uint32_t kStages = 3, kParts = Q8 ? 2 : 1;                      // parts: high, low
     static constexpr uint32_t kKPart = kTmUnit * D * 2, kVPart = kTmUnit * D * 2;      // bytes of a part of a K tile ([64 dims][64 slots][64]) and a V tile ([dims][64 slots])
     // tensor memory: query rows (two buffers), scores (two), weights (two), accumulator
     static constexpr uint32_t kQ = 0, kS = kQ + 2 * (D / 2), kP = kS + 2 * kTmUnit, kO = kP + 2 * (kTmUnit / 2), kCols = 512;
@@ -128,8 +128,10 @@ tree_mma_kernel(const AttnParams p) {
     pdl_wait();
     unit_prefix<kTmRows, kTmUnit, kTmThreads>(p, sm.cum, sm.warp_sums);
     const uint64_t units = sm.cum[p.batch.sequences];
-    const uint64_t quota = max(static_cast<uint64_t>(kLeastUnits), (units + gridDim.x - 1) / gridDim.x);
-    const uint64_t u0 = min(units, blockIdx.x * quota), u1 = min(units, u0 + quota);
+    if (!units) return;
+    const AttnRuns runs(p, units, item_of<kTmRows, kTmUnit>(p, sm.cum, 0));
+    uint64_t u0, u1;
+    runs.run(blockIdx.x, units, u0, u1);
     if (u0 >= u1) return;
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(S::kCols) : "memory");
@@ -614,10 +616,10 @@ tree_mma_kernel(const AttnParams p) {
         const AttnItem& it = tid ? last : first;
         uint32_t joins = 0;
         if (tid ? open1 : open0) {
-            const uint32_t c0 = static_cast<uint32_t>(it.start / quota), c1 = static_cast<uint32_t>((it.end - 1) / quota);
-            joins = atomicAdd(p.counters + c0, 1u) == c1 - c0;
+            const uint32_t c0 = runs.first(it.start), count = runs.count(it.start, it.end);
+            joins = atomicAdd(p.counters + c0, 1u) == count - 1;
             if (joins) p.counters[c0] = 0;
-            sm.span[tid][0] = c0; sm.span[tid][1] = c1 - c0 + 1;
+            sm.span[tid][0] = c0; sm.span[tid][1] = count;
         }
         sm.last[tid] = joins;
         __threadfence();
@@ -631,7 +633,7 @@ tree_mma_kernel(const AttnParams p) {
         if (!sm.last[side]) continue;
         const AttnItem& it = side ? last : first;
         const uint32_t c0 = sm.span[side][0], pieces = sm.span[side][1];
-        const float* part0 = part_at(c0, it.start == c0 * quota);
+        const float* part0 = part_at(c0, runs.at_run_start(it.start));
         const float* part1 = part_at(c0 + 1, true);
         auto part_of = [&](uint32_t i) { return i == 0 ? part0 : part1 + 2ull * (i - 1) * tm_part_floats(); };
         float top = -INFINITY, sum = 0.f;
