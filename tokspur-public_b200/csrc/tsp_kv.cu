@@ -1,6 +1,4 @@
 // Query / key head norm and rotation, and the paged key / value cache that the rows go into: written (quantised), read back, compacted.
-#include <type_traits>
-
 #include "tsp_kv.cuh"
 
 namespace tsp {
@@ -107,11 +105,6 @@ __device__ __forceinline__ bool put_keys(uint8_t* half, uint32_t t, bool q8, uin
 // 16 slots of a head's values, a warp: lane (g, t) takes dims 8 i + 2 t, + 1 of slots g and g + 8, in the order of an MMA fragment, and a transposing
 // move of 8 x 8 matrices puts four slots beside each other as the cache holds them: whole 512-byte rows go out. `rows`: slots of the group that are
 // written (bit i: slot i), `at(slot)`: a slot's values. (A warp per row and head, byte by byte: three prompts of 3000 rows 100 us, now 38.)
-__device__ __forceinline__ uint32_t transposed(uint32_t v) {
-    uint32_t r;
-    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-    return r;
-}
 __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);

@@ -1,4 +1,4 @@
-// Paged key / value cache: where a slot's values lie, and which sequence and slot a row of a step has. The layout (include/tsp_moe.h) is
+// Paged key / value cache: where a slot's values lie. The layout (include/tsp_moe.h) is
 // the order in which the attention kernels' MMA operands want the bytes: a lane's 16 bytes of K are 16 dims of one slot (8 + 8 of two blocks
 // of 32, so that the products of one MMA share a scale), its 16 bytes of V are 4 dims x 4 slots; both are whole 512-byte rows per warp.
 #pragma once
@@ -13,13 +13,9 @@ constexpr uint32_t kKvGroup = 16;   // slots whose bytes lie together
 __host__ __device__ constexpr uint32_t kv_half_bytes(uint32_t dim, bool q8) { return q8 ? 17u * dim : 32u * dim; }
 __host__ __device__ constexpr uint32_t kv_group_bytes(uint32_t dim, bool q8) { return 2u * kv_half_bytes(dim, q8); }
 
-// Byte of dim x of slot t (0..15) within the K or V part of its group
+// Byte of dim x of slot t (0..15) within the K part of its group, of its scale within the K or V part
 __device__ __forceinline__ uint32_t kv_k_byte(uint32_t x, uint32_t t, bool q8) {
     return q8 ? (x / 64 * kKvGroup + t) * 64 + x % 32 / 8 * 16 + x % 64 / 32 * 8 + x % 8 : (x / 32 * kKvGroup + t) * 64 + x % 32 * 2;
-}
-__device__ __forceinline__ uint32_t kv_v_byte(uint32_t x, uint32_t t, bool q8) {
-    const uint32_t lane = t % 8 / 2, e = t % 2 + t / 8 * 2;
-    return q8 ? ((x / 32 * 8 + x % 8) * 4 + lane) * 16 + x % 32 / 8 * 4 + e : ((((x / 16) * 8 + x % 8) * 4 + lane) * 2 + x % 16 / 8) * 8 + e * 2;
 }
 __device__ __forceinline__ uint32_t kv_scale_byte(uint32_t x, uint32_t t, uint32_t dim) { return kKvGroup * dim + (x / 32 * kKvGroup + t) * 2; }
 
@@ -37,16 +33,11 @@ __device__ __forceinline__ uint8_t* kv_group(const tsp_kv_cache& c, uint32_t seq
     return nullptr;
 }
 
-// Sequence of a row, by a whole warp in two steps of 32 offsets each (sequences <= 1024); false for a row of the padding
-__device__ __forceinline__ bool kv_row(const tsp_kv_batch& b, uint32_t row, uint32_t lane, uint32_t& seq, uint32_t& node) {
-    const uint32_t step = (b.sequences + 31) / 32;
-    const uint32_t a = __popc(__ballot_sync(0xffffffffu, (lane + 1) * step <= b.sequences && b.d_row_offsets[min((lane + 1) * step, b.sequences)] <= row)) * step;
-    const uint32_t s = a + __popc(__ballot_sync(0xffffffffu, lane < step && a + lane + 1 <= b.sequences && b.d_row_offsets[min(a + lane + 1, b.sequences)] <= row));
-    seq = s;
-    if (s >= b.sequences) return false;
-    const uint32_t first = b.d_row_offsets[s];
-    node = row - first;
-    return first <= row && row < b.d_row_offsets[s + 1];
+// 8 x 8 matrix of binary16 over a warp, transposed: lane (g, t) gives entries (g, 2t), (g, 2t + 1) and gets (2t, g), (2t + 1, g)
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
 }
 
 // Offsets that do not start at 0, descend or pass the rows: raised by the threads of one block

@@ -2,10 +2,12 @@
 //
 // o = sum_j p_j v_j / sum_j p_j, p_j = 2^(f q.k_j - ref), f = scale log2(e), in one pass over the cache with a running reference and sum of every row.
 //
-// The query rows of one kv head (drafted tokens x heads of the group) share the head's keys and values: they are worked on in tiles of R = 8 or 16
-// rows by warp MMAs (m16n8k16). With eight rows the slots of the cache (scores) and the dims (values) are the M of the MMAs and the rows their
-// N; with sixteen the rows are the M. Work is cut into units of 16 slots of one (sequence, head, row tile) item; the units of the whole batch, item
-// after item, are dealt to the blocks in equal runs and a block's run to its warps, so that one long context fills the GPU as a ragged batch does.
+// The query rows of one kv head (drafted tokens x heads of the group) share the head's keys and values: they are worked on in tiles of eight
+// rows by warp MMAs (m16n8k16): the slots of the cache (scores) and the dims (values) are the M of the MMAs and the rows their N. (Tiles of sixteen
+// rows, as the M of the MMAs, halve the reads of the cache, which come from the L2 anyway, and leave registers for eight warps instead of sixteen:
+// 32 sequences of 4 rows x 4 heads over 4000 slots 72 us against 62, FP32 rows 89 against 77.) Work is cut into units of 16 slots of one
+// (sequence, head, row tile) item; the units of the whole batch, item after item, are dealt to the blocks in equal runs and a block's run to its
+// warps, so that one long context fills the GPU as a ragged batch does.
 // A warp is on its own until the end of its run: it copies its units into its own ring of stages (bulk copies, a group of 16 slots is one contiguous
 // piece), keeps reference, sum and accumulators in registers, and writes the rows of an item that lies within its run. Pieces of items
 // that do not (two a warp at most) meet at the end of the block, and what still is a piece there goes to the scratch, where the last block of the
@@ -21,22 +23,23 @@
 
 namespace tsp {
 
-constexpr uint32_t kPartHead = 64;   // floats in front of a piece's rows: 16 references, 16 sums, a flag
-__host__ __device__ constexpr uint64_t part_floats() { return kPartHead + 2048; }   // R x D <= 2048
+constexpr uint32_t kTile = 8;       // rows
+constexpr uint32_t kPartHead = 32;   // floats in front of a piece's rows: references, sums, a flag
+__host__ __device__ constexpr uint64_t part_floats() { return kPartHead + kTile * 256; }
 constexpr uint32_t kMaxWarps = 16;   // AttnParams::parts: [2 kAttnMaxBlocks] pieces of blocks, then [kAttnMaxBlocks][kMaxWarps] of warps
 
-template <uint32_t D, bool Q8, uint32_t R>
+template <uint32_t D, bool Q8>
 struct AttnShape {
     static constexpr uint32_t kGroupBytes = kv_group_bytes(D, Q8), kHalf = kv_half_bytes(D, Q8);
     // Warps: as many as the registers allow (128 a thread with sixteen) and as three stages each fit shared memory
-    static constexpr uint32_t kWarps = R == 8 && 16 * 3 * kGroupBytes <= 212992 ? 16 : 8 * 3 * kGroupBytes <= 212992 ? 8 : 4, kThreads = 32 * kWarps;
+    static constexpr uint32_t kWarps = 16 * 3 * kGroupBytes <= 212992 ? 16 : 8 * 3 * kGroupBytes <= 212992 ? 8 : 4, kThreads = 32 * kWarps;
     static constexpr uint32_t kStages = 212992 / (kWarps * kGroupBytes) < 6 ? 212992 / (kWarps * kGroupBytes) : 6;
     static constexpr uint32_t kRing = kStages * kGroupBytes;   // a warp's
-    static_assert(kStages >= 3 && kRing >= (R * D + kPartHead) * 4 && R * D <= 2048, "a warp's last piece lies in its ring");
+    static_assert(kStages >= 3 && kRing >= (kTile * D + kPartHead) * 4, "a warp's last piece lies in its ring");
 };
-template <uint32_t D, bool Q8, bool F16, uint32_t R>
+template <uint32_t D, bool Q8>
 struct AttnSmem {
-    using S = AttnShape<D, Q8, R>;
+    using S = AttnShape<D, Q8>;
     alignas(128) uint8_t ring[S::kWarps][S::kRing];
     uint64_t full[S::kWarps][S::kStages];
     uint64_t cum[TSP_KV_MAX_SEQUENCES + 1];
@@ -48,33 +51,32 @@ struct AttnSmem {
     uint32_t last[2], span[2][2];            // whether the block joins its first / last item; the item's blocks
 };
 
-template <uint32_t D, bool Q8, bool F16, uint32_t R>
-__global__ void __launch_bounds__(AttnShape<D, Q8, R>::kThreads, 1)
+template <uint32_t D, bool Q8, bool F16>
+__global__ void __launch_bounds__(AttnShape<D, Q8>::kThreads, 1)
 tree_attention_kernel(const AttnParams p) {
-    using S = AttnShape<D, Q8, R>;
+    using S = AttnShape<D, Q8>;
     constexpr uint32_t NB = D / 32, W = S::kWarps, P = S::kStages, NONE = 0xffffffffu;
     extern __shared__ uint8_t raw[];
-    AttnSmem<D, Q8, F16, R>& sm = *reinterpret_cast<AttnSmem<D, Q8, F16, R>*>(raw);
+    AttnSmem<D, Q8>& sm = *reinterpret_cast<AttnSmem<D, Q8>*>(raw);
     const uint32_t tid = threadIdx.x, lane = tid % 32, warp = tid / 32, g = lane / 4, t = lane % 4;
     pdl_launch_dependents();
     if (lane < P) mbar_init(&sm.full[warp][lane], 1);
     mbar_fence_init();
     pdl_wait();
     if (lane < 2) sm.key[warp][lane] = ~0ull;
-    unit_prefix<R, kKvGroup, S::kThreads>(p, sm.cum, sm.warp_sums);
+    unit_prefix<kTile, kKvGroup, S::kThreads>(p, sm.cum, sm.warp_sums);
     const uint64_t units = sm.cum[p.batch.sequences];
     if (!units) return;
-    const AttnRuns runs(p, units, item_of<R>(p, sm.cum, 0));
+    const AttnRuns runs(p, units, item_of<kTile>(p, sm.cum, 0));
     uint64_t u0, u1;
     runs.run(blockIdx.x, units, u0, u1);
     if (u0 >= u1) return;
 
-    // ---- a warp's run. A lane has two rows (ra, rb) and, of a unit's 16 slots, four scores of each with R = 16, two with R = 8. s[4 * n + c], with
-    // R = 16: row c / 2, slot 8 n + 2 t + c % 2 (MMA n); with R = 8: row c % 2, slot g + 8 (c / 2).
-    constexpr uint32_t NS = R == 8 ? 4 : 8, NI = R == 8 ? 2 : 4, QR = R / 4;
-    const uint32_t ra = R == 8 ? 2 * t : g, rb = R == 8 ? 2 * t + 1 : g + 8;
-    auto second = [](uint32_t i) { return R == 8 ? i % 2 != 0 : i % 4 >= 2; };
-    auto slot_in = [&](uint32_t i) { return R == 8 ? g + 8 * (i / 2) : 8 * (i / 4) + 2 * t + i % 2; };
+    // ---- a warp's run. A lane has two rows (ra, rb) and, of a unit's 16 slots, two scores of each: s[c] of row c % 2, slot g + 8 (c / 2)
+    constexpr uint32_t NS = 4;
+    const uint32_t ra = 2 * t, rb = 2 * t + 1;
+    auto second = [](uint32_t i) { return i % 2 != 0; };
+    auto slot_in = [&](uint32_t i) { return g + 8 * (i / 2); };
     float* const warp_part = p.parts + (2ull * kAttnMaxBlocks + blockIdx.x * kMaxWarps + warp) * part_floats();
     {
         // warps without a unit are the last ones: the pieces of an item lie in neighbouring rings
@@ -88,7 +90,7 @@ tree_attention_kernel(const AttnParams p) {
                 src = 0;
                 const uint64_t u = a + issued + lane;
                 if (u < b) {
-                    const AttnItem x = item_of<R>(p, sm.cum, u);
+                    const AttnItem x = item_of<kTile>(p, sm.cum, u);
                     if (!x.dead) src = reinterpret_cast<uint64_t>(kv_group(p.cache, x.seq, (u - x.start) * kKvGroup, x.head, p.error));
                 }
             }
@@ -106,101 +108,89 @@ tree_attention_kernel(const AttnParams p) {
 
         bool lost = false;   // a wait has run out
         for (uint32_t done = 0; done < mine;) {
-            const AttnItem it = item_of<R>(p, sm.cum, a + done);
+            const AttnItem it = item_of<kTile>(p, sm.cum, a + done);
             const uint32_t stop = static_cast<uint32_t>(min(it.end, b) - a);
             if (lane == 0) { if (a + done == u0) sm.edge[0] = it; if (a + stop == u1) sm.edge[1] = it; }
             // ---- the item's rows as fragments: step 2 b + h holds, in lane (row % 8, t), dims 32 b + 8 t + 4 h + 0..3, the order of a lane's keys
-            uint32_t qf[F16 ? 1 : 2][D / 16][QR];
+            uint32_t qf[F16 ? 1 : 2][D / 16][2];
             float fa, fb;
             [[maybe_unused]] float start[NB][2];   // Q8_0, binary16 rows: -1152 times the sum of the row's 32 dims
             auto row_of = [&](uint32_t r, uint32_t& node, uint32_t& head) {
-                const uint32_t flat = it.tile * R + r;
+                const uint32_t flat = it.tile * kTile + r;
                 node = flat / p.group;
                 head = it.head * p.group + flat % p.group;
             };
             {
                 const float f = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-25f);   // not 0: it multiplies minus infinity
                 fa = fb = f;
-                // Q rows of the fragments: g (and g + 8)
+                uint32_t node, head;
+                row_of(g, node, head);   // the fragments' row
+                const uint8_t* row = p.q + static_cast<uint64_t>(it.row0 + node) * p.q_stride + head * D * (F16 ? 2u : 4u);
+                const bool there = g < it.rows;
+                if constexpr (F16) {
+                    const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
-                for (uint32_t half = 0; half < R / 8; ++half) {
-                    const uint32_t r = g + 8 * half;
-                    uint32_t node, head;
-                    row_of(r, node, head);
-                    const uint8_t* row = p.q + static_cast<uint64_t>(it.row0 + node) * p.q_stride + head * D * (F16 ? 2u : 4u);
-                    const bool there = r < it.rows;
-                    if constexpr (F16) {
-                        const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
+                    for (uint32_t k = 0; k < NB; ++k) {
+                        const uint4 v = there ? *reinterpret_cast<const uint4*>(row + (k * 32 + 8 * t) * 2) : make_uint4(0, 0, 0, 0);
+                        qf[0][2 * k][0] = v.x ^ flip; qf[0][2 * k][1] = v.y ^ flip;
+                        qf[0][2 * k + 1][0] = v.z ^ flip; qf[0][2 * k + 1][1] = v.w ^ flip;
+                    }
+                } else {   // the row times a power of two that puts its largest value at 2^14: both parts keep their 11 bits
+                    float top = 0.f;
 #pragma unroll
-                        for (uint32_t k = 0; k < NB; ++k) {
-                            const uint4 v = there ? *reinterpret_cast<const uint4*>(row + (k * 32 + 8 * t) * 2) : make_uint4(0, 0, 0, 0);
-                            qf[0][2 * k][half] = v.x ^ flip; qf[0][2 * k][half + R / 8] = v.y ^ flip;
-                            qf[0][2 * k + 1][half] = v.z ^ flip; qf[0][2 * k + 1][half + R / 8] = v.w ^ flip;
+                    for (uint32_t k = 0; k < NB; ++k) {
+                        const float4* v = reinterpret_cast<const float4*>(row + (k * 32 + 8 * t) * 4);
+#pragma unroll
+                        for (uint32_t h = 0; h < 2; ++h) {
+                            const float4 x = there ? v[h] : make_float4(0.f, 0.f, 0.f, 0.f);
+                            top = fmaxf(top, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
                         }
-                    } else {   // the row times a power of two that puts its largest value at 2^14: both parts keep their 11 bits
-                        float top = 0.f;
+                    }
+                    top = fmaxf(top, __shfl_xor_sync(NONE, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(NONE, top, 2));
+                    const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+                    const int shift = top > 0.f && e < 128 ? max(-115, min(40, 14 - e)) : 0;
+                    const float up = __uint_as_float(static_cast<uint32_t>(shift + 127) << 23) * (p.scale < 0.f ? -1.f : 1.f);
+                    const float down = f * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);   // of row g
+                    fa = __shfl_sync(NONE, down, 8 * t); fb = __shfl_sync(NONE, down, 8 * t + 4);
 #pragma unroll
-                        for (uint32_t k = 0; k < NB; ++k) {
-                            const float4* v = reinterpret_cast<const float4*>(row + (k * 32 + 8 * t) * 4);
+                    for (uint32_t k = 0; k < NB; ++k) {
+                        const float4* v = reinterpret_cast<const float4*>(row + (k * 32 + 8 * t) * 4);
 #pragma unroll
-                            for (uint32_t h = 0; h < 2; ++h) {
-                                const float4 x = there ? v[h] : make_float4(0.f, 0.f, 0.f, 0.f);
-                                top = fmaxf(top, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-                            }
-                        }
-                        top = fmaxf(top, __shfl_xor_sync(NONE, top, 1));
-                        top = fmaxf(top, __shfl_xor_sync(NONE, top, 2));
-                        const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-                        const int shift = top > 0.f && e < 128 ? max(-115, min(40, 14 - e)) : 0;
-                        const float up = __uint_as_float(static_cast<uint32_t>(shift + 127) << 23) * (p.scale < 0.f ? -1.f : 1.f);
-                        const float down = f * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);   // of row g (+ 8)
-                        if constexpr (R == 8) { fa = __shfl_sync(NONE, down, 8 * t); fb = __shfl_sync(NONE, down, 8 * t + 4); }
-                        else if (half == 0) fa = down;
-                        else fb = down;
-#pragma unroll
-                        for (uint32_t k = 0; k < NB; ++k) {
-                            const float4* v = reinterpret_cast<const float4*>(row + (k * 32 + 8 * t) * 4);
-#pragma unroll
-                            for (uint32_t h = 0; h < 2; ++h) {
-                                const float4 x = there ? v[h] : make_float4(0.f, 0.f, 0.f, 0.f);
-                                const float y0 = x.x * up, y1 = x.y * up, y2 = x.z * up, y3 = x.w * up;
-                                const uint32_t h0 = h2_bits(__floats2half2_rn(y0, y1)), h1 = h2_bits(__floats2half2_rn(y2, y3));
-                                qf[0][2 * k + h][half] = h0; qf[0][2 * k + h][half + R / 8] = h1;
-                                qf[F16 ? 0 : 1][2 * k + h][half] = pack_low(y0, y1, h0); qf[F16 ? 0 : 1][2 * k + h][half + R / 8] = pack_low(y2, y3, h1);
-                            }
+                        for (uint32_t h = 0; h < 2; ++h) {
+                            const float4 x = there ? v[h] : make_float4(0.f, 0.f, 0.f, 0.f);
+                            const float y0 = x.x * up, y1 = x.y * up, y2 = x.z * up, y3 = x.w * up;
+                            const uint32_t h0 = h2_bits(__floats2half2_rn(y0, y1)), h1 = h2_bits(__floats2half2_rn(y2, y3));
+                            qf[0][2 * k + h][0] = h0; qf[0][2 * k + h][1] = h1;
+                            qf[F16 ? 0 : 1][2 * k + h][0] = pack_low(y0, y1, h0); qf[F16 ? 0 : 1][2 * k + h][1] = pack_low(y2, y3, h1);
                         }
                     }
                 }
                 if constexpr (Q8 && F16) {
 #pragma unroll
                     for (uint32_t k = 0; k < NB; ++k) {
-                        float sum[R / 8];
+                        float sum = 0.f;
 #pragma unroll
-                        for (uint32_t half = 0; half < R / 8; ++half) {
-                            sum[half] = 0.f;
+                        for (uint32_t h = 0; h < 2; ++h)
 #pragma unroll
-                            for (uint32_t h = 0; h < 2; ++h)
-#pragma unroll
-                                for (uint32_t j = 0; j < 2; ++j) {
-                                    const float2 v = __half22float2(bits_h2(qf[0][2 * k + h][half + j * (R / 8)]));
-                                    sum[half] += v.x + v.y;
-                                }
-                            sum[half] += __shfl_xor_sync(NONE, sum[half], 1);
-                            sum[half] += __shfl_xor_sync(NONE, sum[half], 2);
-                            sum[half] *= -1152.f;
-                        }
-                        if constexpr (R == 8) { start[k][0] = __shfl_sync(NONE, sum[0], 8 * t); start[k][1] = __shfl_sync(NONE, sum[0], 8 * t + 4); }
-                        else { start[k][0] = sum[0]; start[k][1] = sum[R / 8 - 1]; }
+                            for (uint32_t j = 0; j < 2; ++j) {
+                                const float2 v = __half22float2(bits_h2(qf[0][2 * k + h][j]));
+                                sum += v.x + v.y;
+                            }
+                        sum += __shfl_xor_sync(NONE, sum, 1);
+                        sum += __shfl_xor_sync(NONE, sum, 2);
+                        sum *= -1152.f;
+                        start[k][0] = __shfl_sync(NONE, sum, 8 * t); start[k][1] = __shfl_sync(NONE, sum, 8 * t + 4);
                     }
                 }
             }
 
-            // R = 16: [32 dims][n tile][c]: rows g, g + 8; dims 32 b + 8 i + 2 t, + 1. R = 8: [32 dims][m tile][c]: dims 32 b + 16 i + g, + 8; rows 2 t, + 1
-            float o[NB][NI][4];
+            // [32 dims][m tile][c]: dims 32 b + 16 i + g, + 8; rows 2 t, + 1
+            float o[NB][2][4];
 #pragma unroll
             for (uint32_t k = 0; k < NB; ++k)
 #pragma unroll
-                for (uint32_t i = 0; i < NI; ++i)
+                for (uint32_t i = 0; i < 2; ++i)
 #pragma unroll
                     for (uint32_t c = 0; c < 4; ++c) o[k][i][c] = 0.f;
             // A row's weight is 2^(score + ref), ref = lift - m: m, the score that was largest when the reference last moved; lift, Q8_0: the power of two
@@ -232,42 +222,24 @@ tree_attention_kernel(const AttnParams p) {
                                 else { codes_to_halves(x, kb[n][0], kb[n][1]); codes_to_halves(y, kb[n][2], kb[n][3]); }
                             } else { kb[n][0] = w[n].x; kb[n][1] = w[n].y; kb[n][2] = w[n].z; kb[n][3] = w[n].w; }
                         }
-                        float acc[NS / 4][4];
+                        float acc[4];
 #pragma unroll
-                        for (uint32_t n = 0; n < NS / 4; ++n)
+                        for (uint32_t h = 0; h < 2; ++h)
 #pragma unroll
-                            for (uint32_t h = 0; h < 2; ++h)
-#pragma unroll
-                                for (uint32_t part = 0; part < (F16 ? 1 : 2); ++part) {
-                                    const uint32_t (&q)[QR] = qf[part][2 * k + h];
-                                    const bool fresh = h == 0 && part == 0;
-                                    float c0 = 0.f, c1 = 0.f, c2 = 0.f, c3 = 0.f;
-                                    if constexpr (Q8 && F16) { c0 = start[k][0]; c1 = start[k][R == 8]; c2 = start[k][R != 8]; c3 = start[k][1]; }
-                                    if constexpr (R == 8) {
-                                        if (fresh) mma_f16_16816_from(acc[n], kb[0][0], kb[1][0], kb[0][1], kb[1][1], q[0], q[1], c0, c1, c2, c3);
-                                        else mma_f16_16816(acc[n], kb[0][2 * h], kb[1][2 * h], kb[0][2 * h + 1], kb[1][2 * h + 1], q[0], q[1]);
-                                    } else {
-                                        if (fresh) mma_f16_16816_from(acc[n], q[0], q[1], q[2 % QR], q[3 % QR], kb[n][0], kb[n][1], c0, c1, c2, c3);
-                                        else mma_f16_16816(acc[n], q[0], q[1], q[2 % QR], q[3 % QR], kb[n][2 * h], kb[n][2 * h + 1]);
-                                    }
-                                }
+                            for (uint32_t part = 0; part < (F16 ? 1 : 2); ++part) {
+                                const uint32_t (&q)[2] = qf[part][2 * k + h];
+                                if (h || part) mma_f16_16816(acc, kb[0][2 * h], kb[1][2 * h], kb[0][2 * h + 1], kb[1][2 * h + 1], q[0], q[1]);
+                                else if constexpr (Q8 && F16) mma_f16_16816_from(acc, kb[0][0], kb[1][0], kb[0][1], kb[1][1], q[0], q[1], start[k][0], start[k][1], start[k][0], start[k][1]);
+                                else mma_f16_16816_zero(acc, kb[0][0], kb[1][0], kb[0][1], kb[1][1], q[0], q[1]);
+                            }
                         if constexpr (Q8) {
                             const uint8_t* scales = keys + kKvGroup * D + k * kKvGroup * 2;
-                            if constexpr (R == 8) {
-                                const float d0 = __half2float(*reinterpret_cast<const __half*>(scales + g * 2)), d1 = __half2float(*reinterpret_cast<const __half*>(scales + g * 2 + 16));
-                                s[0] = fmaf(acc[0][0], d0, s[0]); s[1] = fmaf(acc[0][1], d0, s[1]);
-                                s[2] = fmaf(acc[0][2], d1, s[2]); s[3] = fmaf(acc[0][3], d1, s[3]);
-                            } else {
-#pragma unroll
-                                for (uint32_t n = 0; n < NS / 4; ++n) {
-                                    const float2 d = __half22float2(*reinterpret_cast<const __half2*>(scales + (8 * n + 2 * t) * 2));
-#pragma unroll
-                                    for (uint32_t c = 0; c < 4; ++c) s[4 * n + c] = fmaf(acc[n][c], c & 1 ? d.y : d.x, s[4 * n + c]);
-                                }
-                            }
+                            const float d0 = __half2float(*reinterpret_cast<const __half*>(scales + g * 2)), d1 = __half2float(*reinterpret_cast<const __half*>(scales + g * 2 + 16));
+                            s[0] = fmaf(acc[0], d0, s[0]); s[1] = fmaf(acc[1], d0, s[1]);
+                            s[2] = fmaf(acc[2], d1, s[2]); s[3] = fmaf(acc[3], d1, s[3]);
                         } else {
 #pragma unroll
-                            for (uint32_t i = 0; i < NS; ++i) s[i] += acc[i / 4][i % 4];
+                            for (uint32_t i = 0; i < NS; ++i) s[i] += acc[i];
                         }
                     }
                 }
@@ -310,26 +282,16 @@ tree_attention_kernel(const AttnParams p) {
                     for (uint32_t n = 0; n < 2; ++n)
                         keep[n] = (drop >> (8 * n + 2 * t) & 1 ? 0u : 0x0000ffffu) | (drop >> (8 * n + 2 * t) & 2 ? 0u : 0xffff0000u);
                 }
-                // value scales: R = 8, of slots g, g + 8; R = 16, of slots 2t, 2t + 1, 8 more
-                [[maybe_unused]] float dv[Q8 ? NB : 1][QR];
+                [[maybe_unused]] float dv[Q8 ? NB : 1][2];   // value scales of slots g, g + 8
                 float widest = 0.f;
                 if constexpr (Q8) {
 #pragma unroll
                     for (uint32_t k = 0; k < NB; ++k) {
                         const uint8_t* scales = values + kKvGroup * D + k * kKvGroup * 2;
-                        if constexpr (R == 8) {
-                            dv[k][0] = __half2float(*reinterpret_cast<const __half*>(scales + g * 2));
-                            dv[k][1] = __half2float(*reinterpret_cast<const __half*>(scales + g * 2 + 16));
-                            if constexpr (EDGE) { if (drop >> g & 1) dv[k][0] = 0.f; if (drop >> (g + 8) & 1) dv[k][1] = 0.f; }
-                        } else {
-#pragma unroll
-                            for (uint32_t n = 0; n < 2; ++n) {
-                                const float2 f = __half22float2(bits_h2(*reinterpret_cast<const uint32_t*>(scales + (8 * n + 2 * t) * 2) & keep[n]));
-                                dv[k][2 * n % QR] = f.x; dv[k][(2 * n + 1) % QR] = f.y;
-                            }
-                        }
-#pragma unroll
-                        for (uint32_t i = 0; i < QR; ++i) widest = fmaxf(widest, fabsf(dv[k][i]));
+                        dv[k][0] = __half2float(*reinterpret_cast<const __half*>(scales + g * 2));
+                        dv[k][1] = __half2float(*reinterpret_cast<const __half*>(scales + g * 2 + 16));
+                        if constexpr (EDGE) { if (drop >> g & 1) dv[k][0] = 0.f; if (drop >> (g + 8) & 1) dv[k][1] = 0.f; }
+                        widest = fmaxf(widest, fmaxf(fabsf(dv[k][0]), fabsf(dv[k][1])));
                     }
                 }
                 float xa = -INFINITY, xb = -INFINITY;
@@ -338,7 +300,7 @@ tree_attention_kernel(const AttnParams p) {
                 xa *= fa; xb *= fb;
                 if (__any_sync(NONE, xa > limit_a || xb > limit_b || widest > limit_v)) {
 #pragma unroll
-                    for (uint32_t x = R == 8 ? 4 : 1; x < (R == 8 ? 32 : 4); x *= 2) { xa = fmaxf(xa, __shfl_xor_sync(NONE, xa, x)); xb = fmaxf(xb, __shfl_xor_sync(NONE, xb, x)); }
+                    for (uint32_t x = 4; x < 32; x *= 2) { xa = fmaxf(xa, __shfl_xor_sync(NONE, xa, x)); xb = fmaxf(xb, __shfl_xor_sync(NONE, xb, x)); }
                     xa = fmaxf(xa, ma); xb = fmaxf(xb, mb);
                     float fall = 0.f;
                     if constexpr (Q8) {   // widest < 2^(e + 1): weights up to 2^kSlack times it times 2^lift stay below 2^15
@@ -356,7 +318,7 @@ tree_attention_kernel(const AttnParams p) {
 #pragma unroll
                     for (uint32_t k = 0; k < NB; ++k)
 #pragma unroll
-                        for (uint32_t i = 0; i < NI; ++i)
+                        for (uint32_t i = 0; i < 2; ++i)
 #pragma unroll
                             for (uint32_t c = 0; c < 4; ++c) o[k][i][c] *= second(c) ? r1 : r0;
                 }
@@ -366,17 +328,14 @@ tree_attention_kernel(const AttnParams p) {
                     pr[i] = exp2_approx(fmaf(s[i], second(i) ? fb : fa, second(i) ? ref_b : ref_a));
                     if (second(i)) lb += pr[i]; else la += pr[i];
                 }
-                uint32_t wf[QR];
-                [[maybe_unused]] uint32_t wl[QR];
-                auto split = [&](const float (&w)[NS]) {   // R = 16: A fragment (rows g, g + 8; slots 2t.., 8 more); R = 8: B fragment, slots 2t.., 8 more, row g
+                uint32_t wf[2];
+                [[maybe_unused]] uint32_t wl[2];
+                auto split = [&](const float (&w)[NS]) {   // B fragment: slots 2t.., 8 more, of row g
 #pragma unroll
-                    for (uint32_t r = 0; r < QR; ++r) {
-                        wf[r] = h2_bits(__floats2half2_rn(w[2 * r], w[2 * r + 1]));
-                        if constexpr (!F16) wl[r] = pack_low(w[2 * r], w[2 * r + 1], wf[r]);
-                        if constexpr (R == 8) {
-                            wf[r] = transposed(wf[r]);
-                            if constexpr (!F16) wl[r] = transposed(wl[r]);
-                        }
+                    for (uint32_t r = 0; r < 2; ++r) {
+                        const uint32_t high = h2_bits(__floats2half2_rn(w[2 * r], w[2 * r + 1]));
+                        if constexpr (!F16) wl[r] = transposed(pack_low(w[2 * r], w[2 * r + 1], high));
+                        wf[r] = transposed(high);
                     }
                 };
                 if constexpr (!Q8) split(pr);
@@ -389,7 +348,7 @@ tree_attention_kernel(const AttnParams p) {
                         codes_to_halves(w.z, vb[4], vb[5]); codes_to_halves(w.w, vb[6], vb[7]);
                         float w4[NS];
 #pragma unroll
-                        for (uint32_t i = 0; i < NS; ++i) w4[i] = pr[i] * dv[k][R == 8 ? i / 2 : i / 4 * 2 + i % 2];
+                        for (uint32_t i = 0; i < NS; ++i) w4[i] = pr[i] * dv[k][i / 2];
                         split(w4);
                     } else {
                         const uint4 w = *reinterpret_cast<const uint4*>(values + k * 1024 + lane * 16), x = *reinterpret_cast<const uint4*>(values + k * 1024 + 512 + lane * 16);
@@ -400,21 +359,13 @@ tree_attention_kernel(const AttnParams p) {
                         }
                     }
 #pragma unroll
-                    for (uint32_t i = 0; i < NI; ++i) {
-                        auto product = [&](float (&acc)[4], const uint32_t (&w)[QR], bool fresh) {
-                            if constexpr (R == 8) {
-                                if (fresh) mma_f16_16816_zero(acc, vb[4 * i % 8], vb[(4 * i + 2) % 8], vb[(4 * i + 1) % 8], vb[(4 * i + 3) % 8], w[0], w[1]);
-                                else mma_f16_16816(acc, vb[4 * i % 8], vb[(4 * i + 2) % 8], vb[(4 * i + 1) % 8], vb[(4 * i + 3) % 8], w[0], w[1]);
-                            } else {
-                                if (fresh) mma_f16_16816_zero(acc, w[0], w[1], w[2 % QR], w[3 % QR], vb[2 * i], vb[2 * i + 1]);
-                                else mma_f16_16816(acc, w[0], w[1], w[2 % QR], w[3 % QR], vb[2 * i], vb[2 * i + 1]);
-                            }
-                        };
-                        if constexpr (F16) product(o[k][i], wf, false);
+                    for (uint32_t i = 0; i < 2; ++i) {
+                        const uint32_t a0 = vb[4 * i], a1 = vb[4 * i + 2], a2 = vb[4 * i + 1], a3 = vb[4 * i + 3];
+                        if constexpr (F16) mma_f16_16816(o[k][i], a0, a1, a2, a3, wf[0], wf[1]);
                         else {   // the tensor core cuts its sums off: a chain of two products, added up rounded
                             float acc[4];
-                            product(acc, wf, true);
-                            product(acc, wl, false);
+                            mma_f16_16816_zero(acc, a0, a1, a2, a3, wf[0], wf[1]);
+                            mma_f16_16816(acc, a0, a1, a2, a3, wl[0], wl[1]);
 #pragma unroll
                             for (uint32_t c = 0; c < 4; ++c) o[k][i][c] += acc[c];
                         }
@@ -445,34 +396,34 @@ tree_attention_kernel(const AttnParams p) {
 
             // ---- end of the item or of the run
 #pragma unroll
-            for (uint32_t x = R == 8 ? 4 : 1; x < (R == 8 ? 32 : 4); x *= 2) { la += __shfl_xor_sync(NONE, la, x); lb += __shfl_xor_sync(NONE, lb, x); }
-            auto dim_of = [&](uint32_t k, uint32_t i, uint32_t c) { return R == 8 ? k * 32 + i * 16 + g + 8 * (c / 2) : k * 32 + i * 8 + 2 * t + c % 2; };
+            for (uint32_t x = 4; x < 32; x *= 2) { la += __shfl_xor_sync(NONE, la, x); lb += __shfl_xor_sync(NONE, lb, x); }
+            auto dim_of = [&](uint32_t k, uint32_t i, uint32_t c) { return k * 32 + i * 16 + g + 8 * (c / 2); };
             if (it.start >= a && it.end <= b) {   // the whole item: its rows go out
                 const float ia = la == 0.f ? 0.f : 1.f / la, ib = lb == 0.f ? 0.f : 1.f / lb;
                 uint32_t bad = 0;   // bit 0, 1: row ra, rb
 #pragma unroll
                 for (uint32_t k = 0; k < NB; ++k)
 #pragma unroll
-                    for (uint32_t i = 0; i < NI; ++i)
+                    for (uint32_t i = 0; i < 2; ++i)
 #pragma unroll
                         for (uint32_t c = 0; c < 4; ++c) {
                             o[k][i][c] *= second(c) ? ib : ia;
                             if (!(F16 ? fabsf(o[k][i][c]) < 65520.f : finite_f32(o[k][i][c]))) bad |= second(c) ? 2u : 1u;
                         }
 #pragma unroll
-                for (uint32_t x = R == 8 ? 4 : 1; x < (R == 8 ? 32 : 4); x *= 2) bad |= __shfl_xor_sync(NONE, bad, x);
+                for (uint32_t x = 4; x < 32; x *= 2) bad |= __shfl_xor_sync(NONE, bad, x);
 #pragma unroll
                 for (uint32_t side = 0; side < 2; ++side) {
                     const uint32_t r = side ? rb : ra;
                     if (r >= it.rows) continue;
                     const bool zero = dead || bad >> side & 1;
                     if (zero && !dead) raise_error(p.error, TSP_ERR_NONFINITE);
-                    const uint32_t flat = it.tile * R + r, node = flat / p.group, head = it.head * p.group + flat % p.group;
+                    const uint32_t flat = it.tile * kTile + r, node = flat / p.group, head = it.head * p.group + flat % p.group;
                     uint8_t* dst = p.out + static_cast<uint64_t>(it.row0 + node) * p.out_stride + head * D * (F16 ? 2u : 4u);
 #pragma unroll
                     for (uint32_t k = 0; k < NB; ++k)
 #pragma unroll
-                        for (uint32_t i = 0; i < NI; ++i)
+                        for (uint32_t i = 0; i < 2; ++i)
 #pragma unroll
                             for (uint32_t c = 0; c < 4; ++c)
                                 if (second(c) == (side != 0)) {
@@ -484,15 +435,15 @@ tree_attention_kernel(const AttnParams p) {
             } else {
                 const uint32_t which = stop == mine ? 1 : 0;   // 1: the run's last item, into the ring, where no copy is under way any more
                 float* part = which ? reinterpret_cast<float*>(sm.ring[warp]) : warp_part;
-                if (R == 8 ? g == 0 : t == 0) {
+                if (g == 0) {
                     part[ra] = ma == -INFINITY ? ma : -ref_a; part[rb] = mb == -INFINITY ? mb : -ref_b;
-                    part[16 + ra] = la; part[16 + rb] = lb;
+                    part[kTile + ra] = la; part[kTile + rb] = lb;
                 }
-                if (lane == 0) { sm.key[warp][which] = it.start; sm.item[warp][which] = it; part[32] = dead ? 1.f : 0.f; }
+                if (lane == 0) { sm.key[warp][which] = it.start; sm.item[warp][which] = it; part[2 * kTile] = dead ? 1.f : 0.f; }
 #pragma unroll
                 for (uint32_t k = 0; k < NB; ++k)
 #pragma unroll
-                    for (uint32_t i = 0; i < NI; ++i)
+                    for (uint32_t i = 0; i < 2; ++i)
 #pragma unroll
                         for (uint32_t c = 0; c < 4; ++c) {
                             const uint32_t r = second(c) ? rb : ra;
@@ -581,8 +532,8 @@ tree_attention_kernel(const AttnParams p) {
                 for (uint32_t i0 = 0; i0 < n; i0 += 32) {
                     const uint32_t i = i0 + lane, count = min(32u, n - i0);
                     const float* head = part_of(min(i, n - 1));
-                    float m = load_piece(head + r), l = load_piece(head + 16 + r);
-                    dead |= load_piece(head + 32) != 0.f;
+                    float m = load_piece(head + r), l = load_piece(head + kTile + r);
+                    dead |= load_piece(head + 2 * kTile) != 0.f;
                     if (i >= n) { m = -INFINITY; l = 0.f; }
                     float now = m;
 #pragma unroll
@@ -636,7 +587,7 @@ tree_attention_kernel(const AttnParams p) {
                     if (has_row)
 #pragma unroll
                         for (uint32_t k = 0; k < V; ++k) __stcg(reinterpret_cast<float4*>(part + kPartHead + r * D) + k * LANES + lane, y[k]);
-                    if (lane == 0) { __stcg(part + r, top); __stcg(part + 16 + r, sum); __stcg(part + 32, dead ? 1.f : 0.f); }
+                    if (lane == 0) { __stcg(part + r, top); __stcg(part + kTile + r, sum); __stcg(part + 2 * kTile, dead ? 1.f : 0.f); }
                 } else {
                     const float inv = sum == 0.f ? 0.f : 1.f / sum;
                     bool ok = sum == sum;
@@ -647,7 +598,7 @@ tree_attention_kernel(const AttnParams p) {
                     }
                     ok = __all_sync(NONE, ok);
                     if (!ok && !dead && lane == 0) raise_error(p.error, TSP_ERR_NONFINITE);
-                    const uint32_t flat = item->tile * R + r, node = flat / p.group, head = item->head * p.group + flat % p.group;
+                    const uint32_t flat = item->tile * kTile + r, node = flat / p.group, head = item->head * p.group + flat % p.group;
                     uint8_t* dst = p.out + static_cast<uint64_t>(item->row0 + node) * p.out_stride + head * D * (F16 ? 2u : 4u);
                     if (has_row)
 #pragma unroll
@@ -671,12 +622,12 @@ uint64_t tree_attention_scratch_bytes() {
     return kAttnMaxBlocks * sizeof(uint32_t) + (here > there ? here : there);
 }
 
-template <uint32_t D, bool Q8, bool F16, uint32_t R>
+template <uint32_t D, bool Q8, bool F16>
 static int launch_tree_attention_t(const AttnParams& p, cudaStream_t st) {
-    using S = AttnShape<D, Q8, R>;
-    using Smem = AttnSmem<D, Q8, F16, R>;
+    using S = AttnShape<D, Q8>;
+    using Smem = AttnSmem<D, Q8>;
     static_assert(sizeof(Smem) <= 232448, "shared memory of a block");
-    auto kernel = tree_attention_kernel<D, Q8, F16, R>;
+    auto kernel = tree_attention_kernel<D, Q8, F16>;
     static thread_local SmemAttrCache attr;
     TSP_CUDA(ensure_dynamic_smem(kernel, attr, sizeof(Smem)));
     const int sms = sm_count();
@@ -689,14 +640,11 @@ int launch_tree_mma(const AttnParams&, cudaStream_t);
 
 template <uint32_t D, bool Q8>
 static int launch_tree_attention_d(const AttnParams& p, bool f16, cudaStream_t st) {
-    // The narrow tile takes little more than half the instructions of the wide one; heads of 256 dims leave no registers for the wide one. More binary16
-    // rows than one wide tile: 128 of them cost the tensor cores what two wide tiles cost the warps.
-    if constexpr (D < 256) {
-        const uint32_t rows = p.max_rows * p.group;
-        if (f16 && rows > 16) return launch_tree_mma(p, st);
-        if (rows > 8) return f16 ? launch_tree_attention_t<D, Q8, true, 16>(p, st) : launch_tree_attention_t<D, Q8, false, 16>(p, st);
-    }
-    return f16 ? launch_tree_attention_t<D, Q8, true, 8>(p, st) : launch_tree_attention_t<D, Q8, false, 8>(p, st);
+    // Tiles of 128 binary16 rows on the tensor memory's MMAs once more than six narrow tiles would read the cache: 6 sequences over 6000 slots, 48 rows a kv
+    // head 43 us (these tiles) against 41 (narrow ones), 64 rows 44 against 46; one over 8000 slots, 128 rows 34 against 48.
+    if constexpr (D < 256)
+        if (f16 && p.max_rows * p.group > 48) return launch_tree_mma(p, st);
+    return f16 ? launch_tree_attention_t<D, Q8, true>(p, st) : launch_tree_attention_t<D, Q8, false>(p, st);
 }
 
 int launch_tree_attention(const tsp_kv_cache& cache, const tsp_kv_batch& batch, const void* q, uint64_t q_stride, const uint64_t* mask, uint32_t q_heads,

@@ -57,12 +57,6 @@ __device__ __forceinline__ void codes_to_halves(uint32_t w, uint32_t& a, uint32_
     a = h2_bits(__hsub2(bits_h2(__byte_perm(w, 0x64646464u, 0x4140)), bias));
     b = h2_bits(__hsub2(bits_h2(__byte_perm(w, 0x64646464u, 0x4342)), bias));
 }
-// 8 x 8 matrix of binary16 over a warp, transposed: lane (g, t) gives entries (g, 2t), (g, 2t + 1) and gets (2t, g), (2t + 1, g)
-__device__ __forceinline__ uint32_t transposed(uint32_t v) {
-    uint32_t r;
-    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-    return r;
-}
 // the same bytes as 1024 + code + 128, for products whose sum starts at -1152 times the sum of the other side
 __device__ __forceinline__ void biased_halves(uint32_t w, uint32_t& a, uint32_t& b) {
     a = __byte_perm(w, 0x64646464u, 0x4140);
@@ -78,7 +72,6 @@ __device__ __forceinline__ uint32_t pack_low(float u, float v, uint32_t high) { 
     return h2_bits(__floats2half2_rn(u - f.x, v - f.y));
 }
 __device__ __forceinline__ bool odd_half(uint32_t bits) { return (bits & 0x7c00u) == 0x7c00u; }
-
 
 // Geometry of a sequence: units of an item, row tiles
 template <uint32_t R, uint32_t UNIT = kKvGroup>
