@@ -23,7 +23,8 @@
 
 namespace tsp {
 
-constexpr uint32_t kTile = 8;       // rows
+constexpr uint32_t kTile = 8;          // rows
+constexpr uint32_t kLeastUnits = 8;    // of a block's run
 constexpr uint32_t kPartHead = 32;   // floats in front of a piece's rows: references, sums, a flag
 __host__ __device__ constexpr uint64_t part_floats() { return kPartHead + kTile * 256; }
 constexpr uint32_t kMaxWarps = 16;   // AttnParams::parts: [2 kAttnMaxBlocks] pieces of blocks, then [kAttnMaxBlocks][kMaxWarps] of warps
@@ -67,7 +68,7 @@ tree_attention_kernel(const AttnParams p) {
     unit_prefix<kTile, kKvGroup, S::kThreads>(p, sm.cum, sm.warp_sums);
     const uint64_t units = sm.cum[p.batch.sequences];
     if (!units) return;
-    const AttnRuns runs(p, units, item_of<kTile>(p, sm.cum, 0));
+    const AttnRuns runs(p, units, item_of<kTile>(p, sm.cum, 0), kLeastUnits);
     uint64_t u0, u1;
     runs.run(blockIdx.x, units, u0, u1);
     if (u0 >= u1) return;

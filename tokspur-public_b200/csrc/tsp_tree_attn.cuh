@@ -6,7 +6,6 @@
 namespace tsp {
 
 constexpr uint32_t kAttnMaxBlocks = 192;     // blocks (one per SM) that the scratch has room for
-constexpr uint32_t kLeastUnits = 8;          // units of a block's run at least
 // The reference of a row moves when a score passes it by more than 2^kSlack: weights (times value scales, times a power of two 2^lift) stay below 2^15 in
 // binary16, which then reaches down to 2^-31 of the reference.
 constexpr float kSlack = 8.f, kUp = 7.f;
@@ -157,13 +156,13 @@ struct AttnRuns {
     uint64_t quota, item;   // units of a block's run; of an item where items have blocks of their own, else 0
     uint32_t blocks;        // of an item then
 
-    __device__ __forceinline__ AttnRuns(const AttnParams& p, uint64_t units, const AttnItem& any) : item(0), blocks(0) {
+    __device__ __forceinline__ AttnRuns(const AttnParams& p, uint64_t units, const AttnItem& any, uint32_t least) : item(0), blocks(0) {
         const uint64_t each = any.end - any.start, items = units / each;
         if (p.batch.sequences == 1 && items <= gridDim.x) {
             item = each;
             blocks = gridDim.x / static_cast<uint32_t>(items);
-            quota = max(static_cast<uint64_t>(kLeastUnits), (each + blocks - 1) / blocks);
-        } else quota = max(static_cast<uint64_t>(kLeastUnits), (units + gridDim.x - 1) / gridDim.x);
+            quota = max(static_cast<uint64_t>(least), (each + blocks - 1) / blocks);
+        } else quota = max(static_cast<uint64_t>(least), (units + gridDim.x - 1) / gridDim.x);
     }
     __device__ __forceinline__ void run(uint32_t block, uint64_t units, uint64_t& u0, uint64_t& u1) const {
         if (item) {

@@ -16,6 +16,7 @@
 
 namespace tsp {
 
+constexpr uint32_t kTmLeastUnits = 4;   // of a block's run
 constexpr uint32_t kTmRows = 128, kTmUnit = 64, kTmGroups = kTmUnit / kKvGroup;
 constexpr uint32_t kTmSoftmax = 4, kTmTiles = 8, kTmTileWarps = 8, kTmThreads = 32 * (kTmTiles + kTmTileWarps);   // first softmax warp, first tile warp
 // Registers after the hand-over between the warpgroups (setmaxnreg): together no more than the count at launch (80) times the six warpgroups, or the softmax
@@ -50,6 +51,7 @@ struct TmSmem {
     // values are not finite; slots that count as zero
     uint32_t gone[8], k_lift[8], v_lift[8], odd[8][2], drop[8][2];
     uint32_t tmem, last[2], span[2][2], bad_rows[kTmRows / 32];
+    float tops[4][kTmRows];   // of the join
 };
 
 __device__ __forceinline__ void tm_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -94,6 +96,16 @@ __device__ __forceinline__ bool tm_wait(uint64_t* bar, uint32_t parity) {
                      : "=r"(done) : "r"(at), "r"(parity), "r"(1000000u) : "memory");
     return __all_sync(0xffffffffu, done != 0);
 }
+// Three at once: where all are complete, for the time of one. The third may be NULL.
+__device__ __forceinline__ bool tm_wait3(uint64_t* a, uint32_t a_parity, uint64_t* b, uint32_t b_parity, uint64_t* c, uint32_t c_parity) {
+    uint32_t x, y, z = 1;
+    auto test = [](uint64_t* bar, uint32_t parity, uint32_t& done) {
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    };
+    test(a, a_parity, x); test(b, b_parity, y);
+    if (c) test(c, c_parity, z);
+    return __all_sync(0xffffffffu, x & y & z) || (tm_wait(a, a_parity) && tm_wait(b, b_parity) && (!c || tm_wait(c, c_parity)));
+}
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {   // two FP32 operations in one
     float2 d;
     asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
@@ -120,7 +132,7 @@ tree_mma_kernel(const AttnParams p) {
     if (tid == 0) {
         for (uint32_t i = 0; i < S::kStages; ++i) { mbar_init(&sm.code_full[i], 1); mbar_init(&sm.code_known[i], 1); mbar_init(&sm.code_empty[i], kTmTileWarps); }
         for (uint32_t i = 0; i < 2; ++i) {
-            mbar_init(&sm.k_ready[i], kTmTileWarps); mbar_init(&sm.v_ready[i], kTmTileWarps); mbar_init(&sm.s_full[i], 2); mbar_init(&sm.s_free[i], 4);
+            mbar_init(&sm.k_ready[i], kTmTileWarps / 2); mbar_init(&sm.v_ready[i], kTmTileWarps / 2); mbar_init(&sm.s_full[i], 2); mbar_init(&sm.s_free[i], 4);
             mbar_init(&sm.p_ready[i], 4); mbar_init(&sm.pv_done[i], 1); mbar_init(&sm.q_ready[i], 4);
         }
         mbar_fence_init();
@@ -129,7 +141,7 @@ tree_mma_kernel(const AttnParams p) {
     unit_prefix<kTmRows, kTmUnit, kTmThreads>(p, sm.cum, sm.warp_sums);
     const uint64_t units = sm.cum[p.batch.sequences];
     if (!units) return;
-    const AttnRuns runs(p, units, item_of<kTmRows, kTmUnit>(p, sm.cum, 0));
+    const AttnRuns runs(p, units, item_of<kTmRows, kTmUnit>(p, sm.cum, 0), kTmLeastUnits);
     uint64_t u0, u1;
     runs.run(blockIdx.x, units, u0, u1);
     if (u0 >= u1) return;
@@ -299,71 +311,65 @@ tree_mma_kernel(const AttnParams p) {
     } else if (warp >= kTmTiles) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTmTileRegs));
         __syncthreads();
-        // ---- tiles: a warp takes every 16th row of 512 bytes of K, then of V
-        const uint32_t w = warp - kTmTiles, g = lane / 4, t = lane % 4;
-        for (uint32_t j = 0; j < n; ++j) {
-            const uint32_t st = j % S::kStages, buf = j & 1, turn = (j >> 1) & 1;
-            ok = tm_wait(&sm.code_known[st], (j / S::kStages) & 1) && tm_wait(&sm.code_full[st], (j / S::kStages) & 1) && (j < 2 || tm_wait(&sm.s_full[buf], turn ^ 1));   // QK of unit j - 2 has read this K tile
-            if (!ok) break;
-            const uint8_t* stage = sm.ring[st];
-            const bool gone = sm.gone[j % 8] != 0;
-            const float k_up = pow2(static_cast<int>(sm.k_lift[j % 8])), v_up = pow2(static_cast<int>(sm.v_lift[j % 8]));
-            if (!gone) {
-                // K: [64 dims][64 slots] rows of 128 bytes; a lane's 16 bytes are dims 8 t.. of both 32s (Q8_0) or 8 t.. of one (binary16) of slot 8 n + g
+        // ---- tiles: four warps make those of K, four those of V, each its group of 16 slots, so that one side's waits and fences lie under the other's work
+        const uint32_t gi = warp % 4, g = lane / 4, t = lane % 4;
+        if (warp < kTmTiles + 4) {
+            for (uint32_t j = 0; j < n; ++j) {
+                const uint32_t st = j % S::kStages, round = j / S::kStages, buf = j & 1, turn = (j >> 1) & 1;
+                ok = tm_wait3(&sm.code_known[st], round & 1, &sm.code_full[st], round & 1, j < 2 ? nullptr : &sm.s_full[buf], turn ^ 1);   // QK of unit j - 2 has read this tile
+                if (!ok) break;
+                const uint8_t* group = sm.ring[st] + gi * S::kGroupBytes;
+                const float k_up = pow2(static_cast<int>(sm.k_lift[j % 8]));
+                if (!sm.gone[j % 8]) {
+                    // [64 dims][64 slots] rows of 128 bytes; a lane's 16 bytes are dims 8 t.. of both 32s (Q8_0) or 8 t.. of one (binary16) of slot 8 n + g
 #pragma unroll
-                for (uint32_t i = 0; i < (K_LINES * kTmGroups + kTmTileWarps - 1) / kTmTileWarps; ++i) {
-                    constexpr uint32_t LINES = K_LINES;
-                    const uint32_t line = i * kTmTileWarps + w;
-                    if (line >= LINES * kTmGroups) break;   // head_dim 64: half of the warps
-                    const uint32_t gi = line / LINES, x = line % LINES, in = x % 2 * 8 + g, slot = gi * kKvGroup + in;
-                    const uint8_t* group = stage + gi * S::kGroupBytes;
-                    const uint4 c = *reinterpret_cast<const uint4*>(group + x * 512 + lane * 16);
-                    if constexpr (Q8) {
-                        // odd slots put their second half first: eight lanes on eight different 16 bytes
-                        const uint32_t panel = x / 2, turned = g & 1;
-                        const uint32_t words[4] = {turned ? c.z : c.x, turned ? c.w : c.y, turned ? c.x : c.z, turned ? c.y : c.w};
-                        const uint8_t* scales = group + kKvGroup * D + (2 * panel * kKvGroup + in) * 2;
-                        uint8_t* to = sm.k[buf][0] + panel * (kTmUnit * 128) + slot * 128;
+                    for (uint32_t x = 0; x < K_LINES; ++x) {
+                        const uint32_t in = x % 2 * 8 + g, slot = gi * kKvGroup + in;
+                        const uint4 c = *reinterpret_cast<const uint4*>(group + x * 512 + lane * 16);
+                        if constexpr (Q8) {
+                            // odd slots put their second half first: eight lanes on eight different 16 bytes
+                            const uint32_t panel = x / 2, turned = g & 1;
+                            const uint32_t words[4] = {turned ? c.z : c.x, turned ? c.w : c.y, turned ? c.x : c.z, turned ? c.y : c.w};
+                            const uint8_t* scales = group + kKvGroup * D + (2 * panel * kKvGroup + in) * 2;
+                            uint8_t* to = sm.k[buf][0] + panel * (kTmUnit * 128) + slot * 128;
 #pragma unroll
-                        for (uint32_t side = 0; side < 2; ++side) {
-                            const uint32_t h = side ^ turned;
-                            const __half2 d = __float2half2_rn(__half2float(*reinterpret_cast<const __half*>(scales + h * (kKvGroup * 2))) * k_up);
-                            uint32_t high[4], low[4];
+                            for (uint32_t side = 0; side < 2; ++side) {
+                                const uint32_t h = side ^ turned;
+                                const __half2 d = __float2half2_rn(__half2float(*reinterpret_cast<const __half*>(scales + h * (kKvGroup * 2))) * k_up);
+                                uint32_t high[4], low[4];
 #pragma unroll
-                            for (uint32_t x2 = 0; x2 < 2; ++x2) {
-                                uint32_t y[2];
-                                codes_to_halves(words[2 * side + x2], y[0], y[1]);
+                                for (uint32_t x2 = 0; x2 < 2; ++x2) {
+                                    uint32_t y[2];
+                                    codes_to_halves(words[2 * side + x2], y[0], y[1]);
 #pragma unroll
-                                for (uint32_t z = 0; z < 2; ++z) {
-                                    const __half2 v = __hmul2(bits_h2(y[z]), d);
-                                    high[2 * x2 + z] = h2_bits(v);
-                                    low[2 * x2 + z] = h2_bits(__hfma2(bits_h2(y[z]), d, __hneg2(v)));
+                                    for (uint32_t z = 0; z < 2; ++z) {
+                                        const __half2 v = __hmul2(bits_h2(y[z]), d);
+                                        high[2 * x2 + z] = h2_bits(v);
+                                        low[2 * x2 + z] = h2_bits(__hfma2(bits_h2(y[z]), d, __hneg2(v)));
+                                    }
                                 }
+                                const uint32_t at = ((4 * h + t) ^ (slot & 7)) << 4;
+                                *reinterpret_cast<uint4*>(to + at) = make_uint4(high[0], high[1], high[2], high[3]);
+                                *reinterpret_cast<uint4*>(to + (S::kParts - 1) * S::kKPart + at) = make_uint4(low[0], low[1], low[2], low[3]);
                             }
-                            const uint32_t at = ((4 * h + t) ^ (slot & 7)) << 4;
-                            *reinterpret_cast<uint4*>(to + at) = make_uint4(high[0], high[1], high[2], high[3]);
-                            *reinterpret_cast<uint4*>(to + (S::kParts - 1) * S::kKPart + at) = make_uint4(low[0], low[1], low[2], low[3]);
+                        } else {
+                            const uint32_t b = x / 2;   // 32 dims
+                            *reinterpret_cast<uint4*>(sm.k[buf][0] + b / 2 * (kTmUnit * 128) + slot * 128 + (((b % 2 * 4 + t) ^ (slot & 7)) << 4)) = c;
                         }
-                    } else {
-                        const uint32_t b = x / 2;   // 32 dims
-                        *reinterpret_cast<uint4*>(sm.k[buf][0] + b / 2 * (kTmUnit * 128) + slot * 128 + (((b % 2 * 4 + t) ^ (slot & 7)) << 4)) = c;
                     }
                 }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(&sm.k_ready[buf]); mbar_arrive(&sm.code_empty[st]); }
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.k_ready[buf]);
-            ok = j < 2 || tm_wait(&sm.pv_done[buf], turn ^ 1);   // PV of unit j - 2 has read this V tile
-            if (!ok) break;
-            if (!gone) {
-                // V: [dims][64 slots], rows of 128 bytes; a lane's 16 bytes are dims 8 i + g, slots 2 t, 2 t + 1, 8 more
-#pragma unroll
-                for (uint32_t i = 0; i < (K_LINES * kTmGroups + kTmTileWarps - 1) / kTmTileWarps; ++i) {
-                    const uint32_t line = i * kTmTileWarps + w, gi = line / K_LINES, x = line % K_LINES;
-                    if (line >= K_LINES * kTmGroups) break;
-                    const uint8_t* values = stage + gi * S::kGroupBytes + S::kHalf;
-                    const uint4 c = *reinterpret_cast<const uint4*>(values + x * 512 + lane * 16);
-                    const uint32_t words[4] = {c.x, c.y, c.z, c.w};
+        } else {
+            for (uint32_t j = 0; j < n; ++j) {
+                const uint32_t st = j % S::kStages, round = j / S::kStages, buf = j & 1, turn = (j >> 1) & 1;
+                ok = tm_wait3(&sm.code_known[st], round & 1, &sm.code_full[st], round & 1, j < 2 ? nullptr : &sm.pv_done[buf], turn ^ 1);   // PV of unit j - 2 has read this tile
+                if (!ok) break;
+                const uint8_t* values = sm.ring[st] + gi * S::kGroupBytes + S::kHalf;
+                const float v_up = pow2(static_cast<int>(sm.v_lift[j % 8]));
+                if (!sm.gone[j % 8]) {
                     uint32_t keep[2] = {NONE, NONE};
                     const uint32_t out = sm.drop[j % 8][gi / 2] >> (gi % 2 * kKvGroup) & 0xffffu;
                     if (out) {
@@ -373,35 +379,41 @@ tree_mma_kernel(const AttnParams p) {
                     auto put = [&](uint32_t part, uint32_t dim, uint32_t h, uint32_t pair) {   // slots gi * 16 + 8 h + 2 t, + 1 of a dim
                         *reinterpret_cast<uint32_t*>(sm.v[buf][part] + dim * 128 + (((2 * gi + h) ^ (dim & 7)) << 4) + 4 * t) = pair;
                     };
-                    if constexpr (Q8) {
-                        __half2 d[2];
+                    // [dims][64 slots], rows of 128 bytes; a lane's 16 bytes are dims 8 i + g, slots 2 t, 2 t + 1, 8 more
 #pragma unroll
-                        for (uint32_t h = 0; h < 2; ++h) {
-                            const float2 f = __half22float2(bits_h2(*reinterpret_cast<const uint32_t*>(values + kKvGroup * D + (x * kKvGroup + 8 * h + 2 * t) * 2) & keep[h]));
-                            d[h] = __floats2half2_rn(f.x * v_up, f.y * v_up);
-                        }
-#pragma unroll
-                        for (uint32_t q = 0; q < 4; ++q) {
-                            uint32_t y[2];
-                            codes_to_halves(words[q], y[0], y[1]);
+                    for (uint32_t x = 0; x < K_LINES; ++x) {
+                        const uint4 c = *reinterpret_cast<const uint4*>(values + x * 512 + lane * 16);
+                        const uint32_t words[4] = {c.x, c.y, c.z, c.w};
+                        if constexpr (Q8) {
+                            __half2 d[2];
 #pragma unroll
                             for (uint32_t h = 0; h < 2; ++h) {
-                                const __half2 v = __hmul2(bits_h2(y[h]), d[h]);
-                                put(0, 32 * x + 8 * q + g, h, h2_bits(v));
-                                put(S::kParts - 1, 32 * x + 8 * q + g, h, h2_bits(__hfma2(bits_h2(y[h]), d[h], __hneg2(v))));
+                                const float2 f = __half22float2(bits_h2(*reinterpret_cast<const uint32_t*>(values + kKvGroup * D + (x * kKvGroup + 8 * h + 2 * t) * 2) & keep[h]));
+                                d[h] = __floats2half2_rn(f.x * v_up, f.y * v_up);
                             }
+#pragma unroll
+                            for (uint32_t q = 0; q < 4; ++q) {
+                                uint32_t y[2];
+                                codes_to_halves(words[q], y[0], y[1]);
+#pragma unroll
+                                for (uint32_t h = 0; h < 2; ++h) {
+                                    const __half2 v = __hmul2(bits_h2(y[h]), d[h]);
+                                    put(0, 32 * x + 8 * q + g, h, h2_bits(v));
+                                    put(S::kParts - 1, 32 * x + 8 * q + g, h, h2_bits(__hfma2(bits_h2(y[h]), d[h], __hneg2(v))));
+                                }
+                            }
+                        } else {
+#pragma unroll
+                            for (uint32_t q = 0; q < 2; ++q)
+#pragma unroll
+                                for (uint32_t h = 0; h < 2; ++h) put(0, 16 * x + 8 * q + g, h, words[2 * q + h] & keep[h]);
                         }
-                    } else {
-#pragma unroll
-                        for (uint32_t q = 0; q < 2; ++q)
-#pragma unroll
-                            for (uint32_t h = 0; h < 2; ++h) put(0, 16 * x + 8 * q + g, h, words[2 * q + h] & keep[h]);
                     }
                 }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(&sm.v_ready[buf]); mbar_arrive(&sm.code_empty[st]); }
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) { mbar_arrive(&sm.v_ready[buf]); mbar_arrive(&sm.code_empty[st]); }
         }
         __syncwarp();
         __syncthreads();   // a warp that asked for registers now would keep asking until the others are done
@@ -592,7 +604,7 @@ tree_mma_kernel(const AttnParams p) {
                     tm_ld_wait();
 #pragma unroll
                     for (uint32_t i = 0; i < 8; ++i)
-                        __stcg(rows + (c * 8 + i) * kTmRows + r, make_float4(o[4 * i] * scale, o[4 * i + 1] * scale, o[4 * i + 2] * scale, o[4 * i + 3] * scale));
+                        if (r < it.rows) __stcg(rows + (c * 8 + i) * kTmRows + r, make_float4(o[4 * i] * scale, o[4 * i + 1] * scale, o[4 * i + 2] * scale, o[4 * i + 3] * scale));
                 }
             }
             tm_fence_before();   // the accumulator is read before the next item's first weights are said to be ready
@@ -636,15 +648,22 @@ tree_mma_kernel(const AttnParams p) {
         const float* part0 = part_at(c0, runs.at_run_start(it.start));
         const float* part1 = part_at(c0 + 1, true);
         auto part_of = [&](uint32_t i) { return i == 0 ? part0 : part1 + 2ull * (i - 1) * tm_part_floats(); };
+        // the reference of all pieces: each lot looks at every fourth
+        const bool on = lot < LOTS && r < it.rows;
         float top = -INFINITY, sum = 0.f;
         bool dead = false;
 #pragma unroll 4
-        for (uint32_t i = 0; i < (lot < LOTS ? pieces : 0); ++i) top = fmaxf(top, load_piece(part_of(i) + r));
+        for (uint32_t i = lot; i < (on ? pieces : 0); i += LOTS) top = fmaxf(top, load_piece(part_of(i) + r));
+        if (on) sm.tops[lot][r] = top;
+        __syncthreads();
+        if (on)
+#pragma unroll
+            for (uint32_t x = 0; x < LOTS; ++x) top = fmaxf(top, sm.tops[x][r]);
         float4 y[V];
 #pragma unroll
         for (uint32_t k = 0; k < V; ++k) y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-        for (uint32_t i = 0; i < (lot < LOTS ? pieces : 0); ++i) {
+#pragma unroll 2
+        for (uint32_t i = 0; i < (on ? pieces : 0); ++i) {
             const float* part = part_of(i);
             const float m = load_piece(part + r), l = load_piece(part + kTmRows + r), fi = weight_of(m, top);
             dead |= load_piece(part + 2 * kTmRows) != 0.f;
@@ -665,9 +684,9 @@ tree_mma_kernel(const AttnParams p) {
             y[k].x *= inv; y[k].y *= inv; y[k].z *= inv; y[k].w *= inv;
             good &= in_range<true>(y[k].x) && in_range<true>(y[k].y) && in_range<true>(y[k].z) && in_range<true>(y[k].w);
         }
-        if (!good && r < it.rows && lot < LOTS) atomicOr(&sm.bad_rows[r / 32], 1u << r % 32);
+        if (!good && on) atomicOr(&sm.bad_rows[r / 32], 1u << r % 32);
         __syncthreads();
-        if (r < it.rows && lot < LOTS) {
+        if (on) {
             const bool bad = sm.bad_rows[r / 32] >> r % 32 & 1;
             if (bad && !dead && lot == 0) raise_error(p.error, TSP_ERR_NONFINITE);
             const uint32_t flat = it.tile * kTmRows + r, node = flat / p.group, head = it.head * p.group + flat % p.group;
