@@ -3,8 +3,10 @@ import ctypes as C
 
 import numpy as np
 import pytest
+import torch
 
 import attention_ref as R
+from tokspur_public_b200 import attention as A
 from tokspur_public_b200 import capi
 
 
@@ -150,3 +152,31 @@ def test_accepted_arguments_reach_the_device():
         pytest.skip("would follow the pointers")
     for entry in ["norm"] + CACHE:
         assert getattr(Call(), entry)() == capi.E_CUDA, (entry, capi.last_error())
+
+
+def test_tensors_of_another_device_are_refused():
+    """Host memory beside a cache on a GPU (only its device index is set here): the library would follow the pointer on the wrong device."""
+    rows, heads, dim = 3, 2, 64
+    cache = A.KvCache(torch.zeros(4, A.page_bytes("q8_0", 16, heads, dim), dtype=torch.uint8), torch.zeros(1, 4, dtype=torch.int32), 16, heads, dim, "q8_0")
+    batch = A.KvBatch(torch.tensor([0, rows], dtype=torch.int32), torch.zeros(1, dtype=torch.int32), rows)
+    turn = A.QkNormRope(dim, dim, "halves", torch.ones(dim // 2))
+    k, words = torch.zeros(rows, heads, dim), torch.zeros(rows, dtype=torch.int32)
+    cache.device = 0
+    with pytest.raises(ValueError, match="row offsets: on cpu"):
+        A.kv_cache_append(cache, batch, k, k, None)
+    batch.device = 0
+    with pytest.raises(ValueError, match="k: on cpu"):
+        A.kv_cache_append(cache, batch, k, k, None)
+    with pytest.raises(ValueError, match="k_out: on cpu"):
+        A.kv_cache_read(cache, batch, k, None, None)
+    with pytest.raises(ValueError, match="accepted: on cpu"):
+        A.kv_cache_keep(cache, batch, words, words, None)
+    with pytest.raises(ValueError, match="frequencies on devices"):
+        A.qk_norm_rope_append(turn, cache, batch, k, k, k, words, k, None)
+    with pytest.raises(ValueError, match="q: on cpu"):
+        A.tree_attention(cache, batch, k, k, None, rows, 1.0, torch.zeros(1, dtype=torch.uint8), None)
+    with pytest.raises(ValueError, match="no rows"):
+        A.kv_cache_read(cache, batch, None, None, None)
+    k16 = k.to(torch.bfloat16)
+    with pytest.raises(ValueError, match="bfloat16"):
+        A.kv_cache_append(cache, batch, k16, k16, None)

@@ -19,21 +19,29 @@ def _refuse(name, t, dtype, heads, dim, least):
     raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device} does not hold {least} rows of {heads} densely packed heads of {dim} {dtype}")
 
 
-def _rows(name: str, t: torch.Tensor, dtype: torch.dtype, heads: int, dim: int, least: int) -> tuple[int, int]:
+def _elsewhere(name, t, device):
+    raise ValueError(f"{name}: on {t.device}, the call is for CUDA device {device}")
+
+
+def _rows(name: str, t: torch.Tensor, dtype: torch.dtype, heads: int, dim: int, least: int, device: int) -> tuple[int, int]:
     """Pointer and row stride in bytes of [rows, heads, dim], after the checks that the library cannot make. A call of a few microseconds is
     in good part these lines: they ask each tensor as little as they can."""
     stride = t.stride()
-    if len(stride) != 3 or stride[2] != 1 or (stride[1] != dim and heads > 1) or t.dtype is not dtype:
+    if len(stride) != 3 or stride[2] != 1 or (stride[1] != dim and heads > 1) or t.dtype is not dtype or dtype not in SIZES:
         _refuse(name, t, dtype, heads, dim, least)
+    if t.get_device() != device:
+        _elsewhere(name, t, device)
     rows, h, d = t.shape
     if h != heads or d != dim or rows < least:
         _refuse(name, t, dtype, heads, dim, least)
     return t.data_ptr(), stride[0] * SIZES[dtype]
 
 
-def _words(name: str, t: torch.Tensor, dtype: torch.dtype, least: int) -> int:
+def _words(name: str, t: torch.Tensor, dtype: torch.dtype, least: int, device: int) -> int:
     if t.dtype is not dtype or t.numel() < least or not t.is_contiguous():
         raise ValueError(f"{name}: {least} dense values of {dtype}")
+    if t.get_device() != device:
+        _elsewhere(name, t, device)
     return t.data_ptr()
 
 
@@ -42,17 +50,18 @@ _entries: dict = {}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-def _call(name: str, like: torch.Tensor, error: torch.Tensor | None, *args) -> None:
-    """The library's entry on the device of `like`, on torch's current stream there."""
+def _call(name: str, device: int, error: torch.Tensor | None, *args) -> None:
+    """The library's entry on a device, on torch's current stream there."""
     entry = _entries.get(name)
     if entry is None:
         entry = _entries[name] = getattr(capi.lib(), name)
-    device = like.get_device()
+    if error is not None and error.get_device() != device:
+        _elsewhere("error word", error, device)
     if device != torch.cuda.current_device():
         if device < 0:
-            raise ValueError(f"{name}: rows on {like.device}")
+            raise ValueError(f"{name}: tensors in host memory")
         with torch.cuda.device(device):
-            return _call(name, like, error, *args)
+            return _call(name, device, error, *args)
     rc = entry(*args, None if error is None else error.data_ptr(), _raw_stream(device))
     if rc:
         capi.check(rc)
@@ -68,6 +77,9 @@ class KvCache:
             raise ValueError("the page table is int32 [sequences, pages of a sequence]")
         if pages.shape[1] < page_bytes(type_, page_tokens, kv_heads, head_dim):
             raise ValueError("a page is smaller than its slots need")
+        self.device = pages.get_device()
+        if page_table.get_device() != self.device:
+            _elsewhere("page table", page_table, self.device)
         self.pages, self.page_table, self.kv_heads, self.head_dim, self.sequences = pages, page_table, kv_heads, head_dim, page_table.shape[0]
         # a row of the table may be part of a wider one: the stride is what the library walks by
         if page_table.shape[0] > 1 and page_table.stride(0) != page_table.shape[1]:
@@ -88,6 +100,9 @@ class KvBatch:
         if row_offsets.dtype != torch.int32 or lengths.dtype != torch.int32 or row_offsets.numel() != lengths.numel() + 1 \
                 or not row_offsets.is_contiguous() or not lengths.is_contiguous():
             raise ValueError("int32 row offsets of one more than the lengths")
+        self.device = lengths.get_device()
+        if row_offsets.get_device() != self.device:
+            _elsewhere("row offsets", row_offsets, self.device)
         self.row_offsets, self.lengths, self.rows, self.sequences = row_offsets, lengths, rows, lengths.numel()
         self.struct = capi.KvBatch(row_offsets.data_ptr(), lengths.data_ptr(), lengths.numel(), rows)
         self.ref = C.byref(self.struct)
@@ -102,66 +117,81 @@ class QkNormRope:
             if t is not None and (t.dtype != torch.float32 or t.numel() < n or not t.is_contiguous()):
                 raise ValueError("norm weights and frequencies are dense float32")
         self.tensors, self.head_dim = (inv_freq, q_norm, k_norm), head_dim
+        self.devices = {t.get_device() for t in self.tensors if t is not None}
         self.struct = capi.QkNormRope(*(None if t is None else t.data_ptr() for t in (q_norm, k_norm, inv_freq)), head_dim, rotary_dim, STYLES[style], eps, magnitude)
         self.ref = C.byref(self.struct)
 
 
-def _check_batch(cache: KvCache, batch: KvBatch):
+def _check_batch(cache: KvCache, batch: KvBatch) -> int:
+    """The device of both."""
     if batch.sequences > cache.sequences:
         raise ValueError("the page table has fewer sequences than the batch")
+    if batch.device != cache.device:
+        _elsewhere("row offsets", batch.row_offsets, cache.device)
+    return cache.device
+
+
+def _check_turn(turn: QkNormRope, device: int):
+    if turn.devices and turn.devices != {device}:
+        raise ValueError(f"norm weights and frequencies on devices {sorted(turn.devices)}, the call is for CUDA device {device}")
 
 
 def qk_norm_rope(turn: QkNormRope, q, k, positions, q_out, k_out, error):
     """q / k [rows, heads, head_dim] (either may be None) -> q_out / k_out of any of the two dtypes; positions int32 [rows]."""
     x, o, dim = (q, q_out, turn.head_dim) if q is not None else (k, k_out, turn.head_dim)
     rows, dt, ot = x.shape[0], x.dtype, o.dtype
+    device = x.get_device()
+    _check_turn(turn, device)
     hq = hk = qs = ks = qos = kos = 0
     qp = kp = qop = kop = None
     if q is not None:
         hq = q.shape[1]
-        qp, qs = _rows("q", q, dt, hq, dim, rows)
-        qop, qos = _rows("q_out", q_out, ot, hq, dim, rows)
+        qp, qs = _rows("q", q, dt, hq, dim, rows, device)
+        qop, qos = _rows("q_out", q_out, ot, hq, dim, rows, device)
     if k is not None:
         hk = k.shape[1]
-        kp, ks = _rows("k", k, dt, hk, dim, rows)
-        kop, kos = _rows("k_out", k_out, ot, hk, dim, rows)
-    _call("tsp_qk_norm_rope", x, error, turn.ref, qp, qs, kp, ks, int(dt is torch.float16), _words("positions", positions, torch.int32, rows), rows, hq, hk, qop, qos,
+        kp, ks = _rows("k", k, dt, hk, dim, rows, device)
+        kop, kos = _rows("k_out", k_out, ot, hk, dim, rows, device)
+    _call("tsp_qk_norm_rope", device, error, turn.ref, qp, qs, kp, ks, int(dt is torch.float16), _words("positions", positions, torch.int32, rows, device), rows, hq, hk, qop, qos,
           kop, kos, int(ot is torch.float16))
 
 
 def kv_cache_append(cache: KvCache, batch: KvBatch, k, v, error):
-    _check_batch(cache, batch)
+    device = _check_batch(cache, batch)
     dt = k.dtype
-    kp, ks = _rows("k", k, dt, cache.kv_heads, cache.head_dim, batch.rows)
-    vp, vs = _rows("v", v, dt, cache.kv_heads, cache.head_dim, batch.rows)
-    _call("tsp_kv_cache_append", k, error, cache.ref, batch.ref, kp, ks, vp, vs, int(dt is torch.float16))
+    kp, ks = _rows("k", k, dt, cache.kv_heads, cache.head_dim, batch.rows, device)
+    vp, vs = _rows("v", v, dt, cache.kv_heads, cache.head_dim, batch.rows, device)
+    _call("tsp_kv_cache_append", device, error, cache.ref, batch.ref, kp, ks, vp, vs, int(dt is torch.float16))
 
 
 def qk_norm_rope_append(turn: QkNormRope, cache: KvCache, batch: KvBatch, q, k, v, positions, q_out, error):
     """Norm and rotation of q into q_out; of k into the cache, beside v."""
-    _check_batch(cache, batch)
+    device = _check_batch(cache, batch)
+    _check_turn(turn, device)
     dt, ot, dim, heads, rows = q.dtype, q_out.dtype, cache.head_dim, q.shape[1], batch.rows
-    qp, qs = _rows("q", q, dt, heads, dim, rows)
-    kp, ks = _rows("k", k, dt, cache.kv_heads, dim, rows)
-    vp, vs = _rows("v", v, dt, cache.kv_heads, dim, rows)
-    op, os = _rows("q_out", q_out, ot, heads, dim, rows)
-    _call("tsp_qk_norm_rope_append", q, error, turn.ref, cache.ref, batch.ref, qp, qs, kp, ks, vp, vs, int(dt is torch.float16),
-          _words("positions", positions, torch.int32, rows), heads, op, os, int(ot is torch.float16))
+    qp, qs = _rows("q", q, dt, heads, dim, rows, device)
+    kp, ks = _rows("k", k, dt, cache.kv_heads, dim, rows, device)
+    vp, vs = _rows("v", v, dt, cache.kv_heads, dim, rows, device)
+    op, os = _rows("q_out", q_out, ot, heads, dim, rows, device)
+    _call("tsp_qk_norm_rope_append", device, error, turn.ref, cache.ref, batch.ref, qp, qs, kp, ks, vp, vs, int(dt is torch.float16),
+          _words("positions", positions, torch.int32, rows, device), heads, op, os, int(ot is torch.float16))
 
 
 def kv_cache_read(cache: KvCache, batch: KvBatch, k_out, v_out, error):
     """Either of k_out and v_out may be None."""
-    _check_batch(cache, batch)
+    device = _check_batch(cache, batch)
     x = k_out if k_out is not None else v_out
-    kp, ks = (None, 0) if k_out is None else _rows("k_out", k_out, x.dtype, cache.kv_heads, cache.head_dim, batch.rows)
-    vp, vs = (None, 0) if v_out is None else _rows("v_out", v_out, x.dtype, cache.kv_heads, cache.head_dim, batch.rows)
-    _call("tsp_kv_cache_read", x, error, cache.ref, batch.ref, kp, ks, vp, vs, int(x.dtype is torch.float16))
+    if x is None:
+        raise ValueError("kv_cache_read: no rows to read into")
+    kp, ks = (None, 0) if k_out is None else _rows("k_out", k_out, x.dtype, cache.kv_heads, cache.head_dim, batch.rows, device)
+    vp, vs = (None, 0) if v_out is None else _rows("v_out", v_out, x.dtype, cache.kv_heads, cache.head_dim, batch.rows, device)
+    _call("tsp_kv_cache_read", device, error, cache.ref, batch.ref, kp, ks, vp, vs, int(x.dtype is torch.float16))
 
 
 def kv_cache_keep(cache: KvCache, batch: KvBatch, accepted, counts, error):
     """accepted int32 [rows] (a sequence's accepted nodes from its row offset on, ascending), counts int32 [sequences]."""
-    _check_batch(cache, batch)
-    _call("tsp_kv_cache_keep", accepted, error, cache.ref, batch.ref, _words("accepted", accepted, torch.int32, batch.rows), _words("counts", counts, torch.int32, batch.sequences))
+    device = _check_batch(cache, batch)
+    _call("tsp_kv_cache_keep", device, error, cache.ref, batch.ref, _words("accepted", accepted, torch.int32, batch.rows, device), _words("counts", counts, torch.int32, batch.sequences, device))
 
 
 def tree_attention_scratch(device="cuda") -> torch.Tensor:
@@ -172,9 +202,11 @@ def tree_attention_scratch(device="cuda") -> torch.Tensor:
 
 def tree_attention(cache: KvCache, batch: KvBatch, q, out, tree_mask, max_rows: int, scale: float, scratch, error):
     """q [rows, q_heads, head_dim] -> out, the same shape and dtype; tree_mask int64 [rows] (bit i: the row sees token i of its step) or None (chain)."""
-    _check_batch(cache, batch)
+    device = _check_batch(cache, batch)
     dt, heads, dim, rows = q.dtype, q.shape[1], cache.head_dim, batch.rows
-    qp, qs = _rows("q", q, dt, heads, dim, rows)
-    op, os = _rows("out", out, dt, heads, dim, rows)
-    _call("tsp_tree_attention", q, error, cache.ref, batch.ref, qp, qs, None if tree_mask is None else _words("tree words", tree_mask, torch.int64, rows), heads, max_rows,
+    qp, qs = _rows("q", q, dt, heads, dim, rows, device)
+    op, os = _rows("out", out, dt, heads, dim, rows, device)
+    if scratch.get_device() != device:
+        _elsewhere("scratch", scratch, device)
+    _call("tsp_tree_attention", device, error, cache.ref, batch.ref, qp, qs, None if tree_mask is None else _words("tree words", tree_mask, torch.int64, rows, device), heads, max_rows,
           scale, op, os, int(dt is torch.float16), scratch.data_ptr(), scratch.numel())
