@@ -1,5 +1,5 @@
 /*
- * tsp_moe.h — C ABI of the B200 (sm_100a) routed-MoE FFN hot path.
+ * tsp_moe.h — C ABI of the B200 (sm_100a) routed-MoE FFN hot path and of the attention half of a verify / decode step.
  *
  * This is the boundary a tokspur maintainer binds in place of the Metal operator methods of
  * `MetalGraph` (native/include/tokspur/graph.hpp) that `encode_moe`, `encode_moe_mm_many` and

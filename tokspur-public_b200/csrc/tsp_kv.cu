@@ -102,13 +102,14 @@ __device__ __forceinline__ bool put_keys(uint8_t* half, uint32_t t, bool q8, uin
     return ok;
 }
 
-// 16 slots of a head's values, a warp: lane (g, t) takes dims 8 i + 2 t, + 1 of slots g and g + 8, in the order of an MMA fragment, and a transposing
-// move of 8 x 8 matrices puts four slots beside each other as the cache holds them: whole 512-byte rows go out. `rows`: slots of the group that are
-// written (bit i: slot i), `at(slot)`: a slot's values. (A warp per row and head, byte by byte: three prompts of 3000 rows 100 us, now 38.)
 __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+// 16 slots of a head's values, a warp: lane (g, t) takes dims 8 i + 2 t, + 1 of slots g and g + 8, in the order of an MMA fragment, and a transposing
+// move of 8 x 8 matrices puts four slots beside each other as the cache holds them: whole 512-byte rows go out. `rows`: slots of the group that are
+// written (bit i: slot i), `at(slot)`: a slot's values. (A warp per row and head, byte by byte: 4000 rows of three prompts with 32 + 8 + 8 heads of 128
+// dims, norm and rotation 100 us, and 39.5 now.)
 template <uint32_t D, bool IN16, typename At>
 __device__ __forceinline__ bool put_values(uint8_t* half, uint32_t rows, bool q8, uint32_t lane, At&& at) {
     const uint32_t g = lane / 4, t = lane % 4;
@@ -227,9 +228,6 @@ struct HeadRows {
     uint32_t q_heads, kv_heads;   // kv_heads: of k_out (no cache)
 };
 
-// Blocks of three kinds. Rows that go out as rows: a block takes RB rows and as many heads as its threads hold at eight dims each; the rows' values are under
-// way while the threads compute the rows' angles, one each. Keys that go into the cache: a block per row, a warp per head. Values that do: a
-// warp per group of 16 slots and head.
 template <bool F16> struct Raw4;   // four values as they lie in memory
 template <> struct Raw4<true> {
     uint2 w;
@@ -244,6 +242,11 @@ template <> struct Raw4<false> {
     __device__ __forceinline__ void load(const uint8_t* p) { w = *reinterpret_cast<const float4*>(p); }
     __device__ __forceinline__ void to(float (&v)[4]) const { v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w; }
 };
+// Blocks of three kinds. Rows that go out as rows: a block takes RB rows and as many heads as its threads hold at eight dims each; the rows' values are under
+// way while the threads compute the rows' angles, one each. Keys that go into the cache: a block per four slots, a warp per head. Values that do: a
+// warp per group of 16 slots and head. Measured, 32 + 8 heads of 128 dims: 8 FP32 rows 2.1 us, the pitch of launches; 4096 binary16 rows 18 us, 84 MB at 4.6 TB/s, from
+// the L2 in part, bound by instructions (71 % of the issue slots). Into a Q8_0 cache: 38 rows of six drafts 10.3 us, a chain of latencies; 4024 rows of
+// prompts 39.5 us, bound by the 64-bit arithmetic of the keys and by instructions (67 % of the issue slots), and without norm and rotation 17.8.
 template <uint32_t D, bool IN16, bool OUT16, uint32_t RB>
 __device__ __forceinline__ void turn_rows(const tsp_qk_norm_rope_args& a, const HeadRows& r, uint32_t pass, uint32_t row0, uint32_t end, uint32_t* error) {
     __shared__ __align__(16) float cs[RB][D / 2], sn[RB][D / 2];
@@ -427,8 +430,6 @@ append_rows_kernel(const tsp_qk_norm_rope_args a, const HeadRows r, const tsp_kv
     if (bad) raise_error(error, TSP_ERR_NONFINITE);
 }
 
-// A warp per group of 16 slots and head: every load is a whole 512-byte row of the group, all of them under way at once; K leaves in the order it lies in,
-// V through transposing moves as it came. (A warp per row and head, byte by byte: 60000 rows of 8 heads 238 us, now 63.)
 template <uint32_t D, bool OUT16>
 __device__ __forceinline__ void store8(uint8_t* row, uint32_t x, const float (&v)[8]) {   // eight dims from x on
     if constexpr (OUT16) *reinterpret_cast<uint4*>(row + x * 2) = make_uint4(half2_bits(v[0], v[1]), half2_bits(v[2], v[3]), half2_bits(v[4], v[5]), half2_bits(v[6], v[7]));
@@ -442,6 +443,9 @@ __device__ __forceinline__ void values_of(uint32_t a, uint32_t b, float d, float
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) v[i] = static_cast<float>(static_cast<int>((i < 4 ? a : b) >> (8 * (i % 4)) & 0xffu) - 128) * d;
 }
+// A warp per group of 16 slots and head: every load is a whole 512-byte row of the group, all of them under way at once; K leaves in the order it lies in,
+// V through transposing moves as it came. (A warp per row and head, byte by byte: 57000 rows of 8 heads of 128 dims 238 us, and 64 now: 361 MB at 5.6 TB/s, the
+// writes to memory bound it.)
 template <uint32_t D, bool OUT16, bool Q8>
 __global__ void __launch_bounds__(256)
 cache_read_kernel(const tsp_kv_cache cache, const tsp_kv_batch batch, uint8_t* k, uint64_t k_stride, uint8_t* v, uint64_t v_stride, uint32_t* error) {
@@ -539,7 +543,8 @@ cache_read_kernel(const tsp_kv_cache cache, const tsp_kv_batch batch, uint8_t* k
 }
 
 // A block per (sequence, head): every source slot is in shared memory before the first destination is written. Pieces of a slot: 16 bytes of K, the four
-// bytes (two halves) of V that a group of its 512-byte rows has of the slot, scales.
+// bytes (two halves) of V that a group of its 512-byte rows has of the slot, scales. Latencies one behind the other bound it (offsets, indices, table, source,
+// destination): one tree of 24 tokens 5.2 us, 64 sequences of up to 16 10.3.
 template <uint32_t D, bool Q8>
 __global__ void __launch_bounds__(256)
 cache_keep_kernel(const tsp_kv_cache cache, const tsp_kv_batch batch, const uint32_t* accepted, const uint32_t* counts, uint32_t* error) {

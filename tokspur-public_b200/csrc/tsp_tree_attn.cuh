@@ -151,7 +151,7 @@ __device__ __forceinline__ void unit_prefix(const AttnParams& p, uint64_t* cum, 
 
 // Which units a block runs over, and which blocks an item has. The units of a ragged batch are dealt in equal runs, whatever item they are of. A single
 // sequence's items (heads, row tiles) are all alike: where there are no more of them than blocks, every item gets the same number of blocks of its
-// own, so that no block has pieces of two to join (one row over 4096 slots: 19 us against 15).
+// own, so that no block has pieces of two to join (one token over 4096 slots 15.8 us, in equal runs 19).
 struct AttnRuns {
     uint64_t quota, item;   // units of a block's run; of an item where items have blocks of their own, else 0
     uint32_t blocks;        // of an item then

@@ -4,10 +4,15 @@
 // the M of tcgen05 MMAs: S = Q K^T (N = 64 slots, K = dims) and O += P V (N = dims, K = 64 slots), both with the left operand in tensor memory and the cache's
 // tile in shared memory. Units are 64 slots; they are dealt to the blocks as there, and pieces of items that span blocks are joined the same way.
 //
-// Roles of a block's 24 warps (one block per SM): 0 copies groups of 16 slots into a ring; 3 looks at what came; 1 issues the MMAs; 4..7 are the softmax, a thread per query row:
+// Roles of a block's 16 warps (one block per SM): 0 copies groups of 16 slots into a ring; 3 looks at what came; 1 issues the MMAs; 4..7 are the softmax, a thread per query row:
 // a score row from tensor memory to registers, weights back to tensor memory as binary16, reference, sum and the rare rescaling of the accumulator, and at an
-// item's end the accumulator's row; 8..15 turn codes into the MMAs' tiles. Scores, weights, query rows and tiles are double-buffered, so the QK of
-// one unit runs under the softmax of the one before and the PV of the one before that.
+// item's end the accumulator's row; 8..11 turn codes into the MMAs' tiles of K, 12..15 into those of V. Scores, weights, query rows and tiles are double-buffered, so
+// the QK of one unit runs under the softmax of the one before and the PV of the one before that.
+//
+// Measured: a tree of 64 tokens x 32 heads over 131072 slots of 8 kv heads, Q8_0, 128 dims: 283 us (867 with tiles of eight rows on the warps' MMAs; 293 with
+// K and V tiles by the same warps), the bytes alone 44 us, the products alone 84; four trees of 32 tokens over up to 20000 slots: 66 us (115). A unit takes about
+// 2050 cycles at 1.75 GHz, 1024 of them MMAs; without the tiles' arithmetic it takes 1850, without half of the MMAs 1880, without these, the softmax's and the
+// copies 1450: no stage alone but the hand-overs between them (barrier, fence, commit) bound it.
 //
 // Rounding: a Q8_0 value is code times scale, 18 bits. Tiles hold it as two binary16 numbers, high and low (exact, times a power of two that puts the unit's
 // largest scale at 2^7), and the MMAs run over both: what is left between the cache and a binary16 row is the weights' rounding, as on the warp MMAs. (High
@@ -16,11 +21,11 @@
 
 namespace tsp {
 
-constexpr uint32_t kTmLeastUnits = 4;   // of a block's run
+constexpr uint32_t kTmLeastUnits = 4;   // of a block's run: 13 tokens over 1000 slots 18.8 us, 22.5 with eight
 constexpr uint32_t kTmRows = 128, kTmUnit = 64, kTmGroups = kTmUnit / kKvGroup;
 constexpr uint32_t kTmSoftmax = 4, kTmTiles = 8, kTmTileWarps = 8, kTmThreads = 32 * (kTmTiles + kTmTileWarps);   // first softmax warp, first tile warp
-// Registers after the hand-over between the warpgroups (setmaxnreg): together no more than the count at launch (80) times the six warpgroups, or the softmax
-// would wait for ever; the launcher checks it. At the end all go back to that count.
+// Registers after the hand-over between the warpgroups (setmaxnreg): together no more than the count at launch times the four warpgroups, or the softmax
+// would wait for ever; the launcher checks that count. At the end all go back to that count.
 constexpr int kTmLaunchRegs = 128, kTmIssueRegs = 104, kTmSoftmaxRegs = 192, kTmTileRegs = 104;
 static_assert(kTmIssueRegs + kTmSoftmaxRegs + kTmTileWarps / 4 * kTmTileRegs <= (2 + kTmTileWarps / 4) * kTmLaunchRegs, "hand-over of registers");
 // piece of an item: references and sums of 128 rows, a flag, then the rows' dims four by four, rows side by side: [dim / 4][row][4]
@@ -30,7 +35,7 @@ __host__ __device__ constexpr uint64_t tm_part_floats() { return kTmPartHead + k
 template <uint32_t D, bool Q8>
 struct TmShape {
     static constexpr uint32_t kGroupBytes = kv_group_bytes(D, Q8), kHalf = kv_half_bytes(D, Q8), kStage = kTmGroups * kGroupBytes;
-    static constexpr uint32_t kStages = 3, kParts = Q8 ? 2 : 1;                      // parts: high, low
+    static constexpr uint32_t kStages = 3, kParts = Q8 ? 2 : 1;   // parts: high, low. Four stages: no faster over long contexts, 2 % slower over short ones
     static constexpr uint32_t kKPart = kTmUnit * D * 2, kVPart = kTmUnit * D * 2;      // bytes of a part of a K tile ([64 dims][64 slots][64]) and a V tile ([dims][64 slots])
     // tensor memory: query rows (two buffers), scores (two), weights (two), accumulator
     static constexpr uint32_t kQ = 0, kS = kQ + 2 * (D / 2), kP = kS + 2 * kTmUnit, kO = kP + 2 * (kTmUnit / 2), kCols = 512;
@@ -85,8 +90,8 @@ __device__ __forceinline__ void tm_mma64(uint32_t d, uint32_t a, uint32_t b_smem
 __device__ __forceinline__ void tm_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// Bounded wait by a whole warp. Every try may sleep for up to a millisecond: sixteen warps that asked again at once took a sixth of the issue slots from the
-// others. Two seconds in all, then the caller gives up.
+// Bounded wait by a whole warp. Every try may sleep for up to a millisecond: warps that asked again at once took issue slots and shared memory's time from the
+// others (the case above 323 us). Two seconds in all, then the caller gives up.
 __device__ __forceinline__ bool tm_wait(uint64_t* bar, uint32_t parity) {
     const uint32_t at = smem_u32(bar);
     uint32_t done = 0;

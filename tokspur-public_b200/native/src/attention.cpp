@@ -74,7 +74,7 @@ void encode_verify_attention(CudaGraph& g, const AttentionWeights& w, const KvCa
     const tsp_qk_norm_rope_args a{weight(g, w.q_norm, dim, "query norm"), weight(g, w.k_norm, dim, "key norm"), weight(g, w.inv_freq, w.rotary_dim / 2, "frequencies"),
                                   dim, w.rotary_dim, w.pairs ? TSP_ROPE_PAIRS : TSP_ROPE_HALVES, w.eps, w.magnitude};
     const uint32_t q_heads = q.columns / dim;
-    // both launches or none: what the second would refuse is refused before the first
+    // shapes that the second launch would refuse are refused before the first
     if (q_heads % cache.shape.kv_heads || q_heads / cache.shape.kv_heads > 64 || !most_rows || most_rows > TSP_KV_MAX_DRAFT || !std::isfinite(scale) ||
         scratch.join.bytes < tsp_tree_attention_scratch_bytes())
         throw FormatError("attention shape or scratch mismatch");
