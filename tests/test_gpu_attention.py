@@ -599,3 +599,62 @@ def test_long_runs(type_, dim, heads, group, counts, lengths, dtype):
         d = out[first[s]:first[s + 1]].double() - want
         num, den = num + float((d * d).sum()), den + float((want * want).sum())
     assert np.sqrt(num / den) <= (2e-3 if dtype == "f16" else 5e-6)
+
+
+# ---- more than 48 binary16 rows per key / value head: the tiles of 128 rows, at the same edges
+
+@pytest.mark.parametrize("type_,dim", [("q8_0", 128), ("q8_0", 64), ("f16", 128), ("f16", 64)])
+@pytest.mark.parametrize("rows", [47, 48, 49, 64])
+def test_rows_at_the_change_of_tiles(type_, dim, rows):
+    s = Step(rows + dim, type_, dim, 16, 2, 1, [rows, 3], [200, 1027], "f16", True)
+    out, err = s.run()
+    assert err == 0
+    s.check(out)
+
+
+@pytest.mark.parametrize("type_", ["q8_0", "f16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-12])
+def test_wide_tiles_scales(type_, dim, scale):
+    s = Step(17, type_, dim, 16, 2, 16, [5, 2], [237, 0], "f16", True)
+    s.mask[1] = 0
+    s.scale = scale
+    out, err = s.run()
+    assert err == 0
+    s.check(out)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_wide_tiles_sequences_out_of_range(dim):
+    s = Step(19, "q8_0", dim, 16, 2, 4, [3, 40, 20, 2], [50, 20, 170, 8], "f16", False)
+    out, err = s.run(most=32)                          # sequence 1 has more rows than the call says
+    assert err == capi.ERR_INDEX and (out[3:43] == 0).all()
+    s.check(out, skip=(1,))
+    s.p.table[2, 2] = 0x7fffffff                       # a page that does not exist
+    out, err = s.run()
+    assert err & capi.ERR_INDEX and (out[43:63] == 0).all()
+    s.check(out, skip=(2,))
+    s.batch.lengths[3] = 5000                          # slots that the table does not hold
+    out, err = s.run()
+    assert err & capi.ERR_INDEX and (out[63:65] == 0).all() and (out[43:63] == 0).all()
+    s.check(out, skip=(2, 3))
+
+
+@pytest.mark.parametrize("type_", ["q8_0", "f16"])
+@pytest.mark.parametrize("at", [2e4, 1e-4])
+def test_wide_tiles_large_scores_and_values(type_, at):
+    """Scores far apart, values near binary16's limits and far below one; a scale that grows and falls from slot to slot."""
+    s = Step(23, type_, 128, 16, 1, 4, [16], [190], "f16", False)
+    for j in range(206):
+        k, v = s.k[0][j] * (30 if j % 3 else 0.01), s.v[0][j] * (at / 6) * (1 if j % 5 else 1 / 64)
+        s.p.put(0, j, k, v)
+        s.k[0][j], s.v[0][j] = R.cached(k, type_), R.cached(v, type_)
+    out, err = s.run()
+    assert err == 0
+    got = out.cpu().numpy().astype(np.float64)
+    for j in range(16):
+        want, spread, vmax = R.attended(s.q[j], s.k[0], s.v[0], s.visible(0, j), s.scale)
+        e = (136 * U32 + U16) * spread
+        # weights, the low parts' and the result's rounding; 2^-25: half of binary16's smallest step
+        tol = vmax * (4 * e + 4 * U16) + U16 * np.abs(want) + 2.0 ** -25
+        assert (np.abs(got[j] - want) <= tol).all(), (type_, at, j)
