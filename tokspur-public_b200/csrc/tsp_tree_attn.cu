@@ -17,7 +17,7 @@
 // Measured, Q8_0 and binary16 rows of 32 heads over 8 kv heads of 128 dims: 64 sequences of up to 8192 slots, a token each, 128 us, 644 MB of cache at
 // 5.0 TB/s, bound by instructions (unpacking, 53 % of the issue slots) and by the ragged runs' ends; one token over 4096 slots 15.7 us, bound by a
 // chain of latencies (table, copy, cold instructions, the join of a head's blocks). FP32 rows, 6 chains of up to 8 tokens x 8 heads over 6000 slots
-// of binary16, 256 dims: 51 us, bound by the instructions of the split products (640 for the 64 MMAs of a unit and tile) at four warps an SM.
+// of binary16, 256 dims: 41.5 us, bound by the instructions of the split products (640 for the 64 MMAs of a unit and tile) at eight warps an SM.
 //
 // Codes enter the MMAs exactly (binary16 integers). The scale of a key block multiplies the FP32 partial score of its 32 dims, that of a value block the
 // FP32 weight before that is rounded to binary16: one rounding of 2^-11 on the whole path of binary16 rows. FP32 rows split the query (times a
@@ -37,10 +37,13 @@ constexpr uint32_t kMaxWarps = 16;   // AttnParams::parts: [2 kAttnMaxBlocks] pi
 template <uint32_t D, bool Q8>
 struct AttnShape {
     static constexpr uint32_t kGroupBytes = kv_group_bytes(D, Q8), kHalf = kv_half_bytes(D, Q8);
+    // A stage holds a group, or its keys or values alone where three groups for each of eight warps do not fit shared memory (256 dims of binary16: 51 us for six
+    // chains with four warps and whole groups, 41.5 so)
+    static constexpr uint32_t kPieces = 8 * 3 * kGroupBytes <= 212992 ? 1 : 2, kPiece = kGroupBytes / kPieces;
     // Warps: as many as the registers allow (128 a thread with sixteen) and as three stages each fit shared memory
-    static constexpr uint32_t kWarps = 16 * 3 * kGroupBytes <= 212992 ? 16 : 8 * 3 * kGroupBytes <= 212992 ? 8 : 4, kThreads = 32 * kWarps;
-    static constexpr uint32_t kStages = 212992 / (kWarps * kGroupBytes) < 6 ? 212992 / (kWarps * kGroupBytes) : 6;
-    static constexpr uint32_t kRing = kStages * kGroupBytes;   // a warp's
+    static constexpr uint32_t kWarps = 16 * 3 * kPiece <= 212992 && kPieces == 1 ? 16 : 8, kThreads = 32 * kWarps;
+    static constexpr uint32_t kStages = 212992 / (kWarps * kPiece) < 6 ? 212992 / (kWarps * kPiece) : 6;
+    static constexpr uint32_t kRing = kStages * kPiece;   // a warp's
     static_assert(kStages >= 3 && kRing >= (kTile * D + kPartHead) * 4, "a warp's last piece lies in its ring");
 };
 template <uint32_t D, bool Q8>
@@ -88,23 +91,25 @@ tree_attention_kernel(const AttnParams p) {
         // warps without a unit are the last ones: the pieces of an item lie in neighbouring rings
         const uint32_t n = static_cast<uint32_t>(u1 - u0), mine = n / W + (warp < n % W);
         const uint64_t a = u0 + warp * (n / W) + min(warp, n % W), b = a + mine;
+        constexpr uint32_t PIECES = S::kPieces;
         uint64_t src = 0;              // lane i: source of unit i of the 32 that `issued` is in
-        uint32_t issued = 0, gone = 0; // bit st: the unit in stage st has no page
+        uint32_t issued = 0, gone = 0; // issued: pieces; gone, bit st: the unit in stage st has no page
         auto issue = [&](uint32_t st) {
-            if (issued >= mine) return;
-            if (issued % 32 == 0) {
+            if (issued >= mine * PIECES) return;
+            if (issued % (32 * PIECES) == 0) {
                 src = 0;
-                const uint64_t u = a + issued + lane;
+                const uint64_t u = a + issued / PIECES + lane;
                 if (u < b) {
                     const AttnItem x = item_of<kTile>(p, sm.cum, u);
                     if (!x.dead) src = reinterpret_cast<uint64_t>(kv_group(p.cache, x.seq, (u - x.start) * kKvGroup, x.head, p.error));
                 }
             }
-            const uint64_t from = __shfl_sync(NONE, src, issued % 32);
+            uint64_t from = __shfl_sync(NONE, src, issued / PIECES % 32);
+            if (from) from += issued % PIECES * S::kPiece;
             gone = (gone & ~(1u << st)) | (from ? 0u : 1u << st);
             if (elect_one()) {
-                mbar_arrive_expect_tx(&sm.full[warp][st], from ? S::kGroupBytes : 0);
-                if (from) bulk_g2s(sm.ring[warp] + st * S::kGroupBytes, reinterpret_cast<const void*>(from), S::kGroupBytes, &sm.full[warp][st]);
+                mbar_arrive_expect_tx(&sm.full[warp][st], from ? S::kPiece : 0);
+                if (from) bulk_g2s(sm.ring[warp] + st * S::kPiece, reinterpret_cast<const void*>(from), S::kPiece, &sm.full[warp][st]);
             }
             __syncwarp();
             ++issued;
@@ -205,10 +210,24 @@ tree_attention_kernel(const AttnParams p) {
             float ref_a = 0.f, ref_b = 0.f, limit_a = -INFINITY, limit_b = -INFINITY, limit_v = Q8 ? 0x1p-13f : INFINITY;
             bool dead = false;
 
+            // false: the wait has run out, and no wait is tried again
+            auto arrived = [&]() {
+                const bool yes = __all_sync(NONE, !lost && (mbar_try_wait(&sm.full[warp][stage], phase) || mbar_wait(&sm.full[warp][stage], phase)));
+                if (!yes) {
+                    if (!lost && lane == 0) raise_error(p.error, TSP_ERR_TIMEOUT);
+                    lost = dead = true;
+                }
+                return yes;
+            };
+            auto pass = [&]() {   // the stage has been read: filled again
+                __syncwarp();
+                if (!lost) issue(stage);
+                if (++stage == P) { stage = 0; phase ^= 1; }
+            };
             // One unit; EDGE: it reaches past the context
-            auto unit = [&](auto edge_tag, const uint8_t* keys) {
+            auto unit = [&](auto edge_tag) {
                 constexpr bool EDGE = decltype(edge_tag)::value;
-                const uint8_t* values = keys + S::kHalf;
+                const uint8_t* keys = sm.ring[warp] + stage * S::kPiece;
                 float s[NS];
 #pragma unroll
                 for (uint32_t i = 0; i < NS; ++i) s[i] = 0.f;
@@ -249,6 +268,8 @@ tree_attention_kernel(const AttnParams p) {
                         }
                     }
                 }
+                if constexpr (PIECES == 2) { pass(); (void)arrived(); }
+                const uint8_t* values = PIECES == 2 ? sm.ring[warp] + stage * S::kPiece : keys + S::kHalf;
                 // At the end of the context: what a row does not see gets no weight. Drafted slots whose values are not finite give the rows that see
                 // them NaN through the weight, and count as zero themselves; slots behind the last count as zero, whatever they hold.
                 uint32_t keep[2] = {NONE, NONE};   // values of slots 2t, 2t + 1 and 8 more
@@ -380,25 +401,16 @@ tree_attention_kernel(const AttnParams p) {
             };
             const uint64_t plain = it.start + it.length / kKvGroup;   // units before this one lie in the context
             const uint32_t inner = plain <= a ? 0u : static_cast<uint32_t>(min(plain - a, static_cast<uint64_t>(stop)));
-            // false: the wait has run out, and no wait is tried again
-            auto arrived = [&](uint32_t st) { return !lost && (mbar_try_wait(&sm.full[warp][st], phase) || mbar_wait(&sm.full[warp][st], phase)); };
-            auto step = [&](uint32_t st, auto edge_tag) {
-                if (!__all_sync(NONE, arrived(st))) {
-                    if (!lost && lane == 0) raise_error(p.error, TSP_ERR_TIMEOUT);
-                    lost = dead = true;
-                } else if (gone >> st & 1) dead = true;
-                else unit(edge_tag, sm.ring[warp] + st * S::kGroupBytes);
-                __syncwarp();
-                if (!lost) issue(st);   // into the stage that was just read
+            auto step = [&](auto edge_tag) {
+                if (arrived() && !(gone >> stage & 1)) unit(edge_tag);
+                else {
+                    dead = true;
+                    if constexpr (PIECES == 2) { pass(); (void)arrived(); }
+                }
+                pass();
             };
-            for (; done < inner; ++done) {
-                step(stage, std::false_type{});
-                if (++stage == P) { stage = 0; phase ^= 1; }
-            }
-            for (; done < stop; ++done) {
-                step(stage, std::true_type{});
-                if (++stage == P) { stage = 0; phase ^= 1; }
-            }
+            for (; done < inner; ++done) step(std::false_type{});
+            for (; done < stop; ++done) step(std::true_type{});
 
             // ---- end of the item or of the run
 #pragma unroll
