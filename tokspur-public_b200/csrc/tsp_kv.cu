@@ -108,10 +108,10 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 }
 // 16 slots of a head's values, a warp: lane (g, t) takes dims 8 i + 2 t, + 1 of slots g and g + 8, in the order of an MMA fragment, and a transposing
 // move of 8 x 8 matrices puts four slots beside each other as the cache holds them: whole 512-byte rows go out. `rows`: slots of the group that are
-// written (bit i: slot i), `at(slot)`: a slot's values. (A warp per row and head, byte by byte: 4000 rows of three prompts with 32 + 8 + 8 heads of 128
+// written (bit i: slot i), b0 .. b1: blocks of 32 dims that are, `at(slot)`: a slot's values. (A warp per row and head, byte by byte: 4000 rows of three prompts with 32 + 8 + 8 heads of 128
 // dims, norm and rotation 100 us, and 39.5 now.)
 template <uint32_t D, bool IN16, typename At>
-__device__ __forceinline__ bool put_values(uint8_t* half, uint32_t rows, bool q8, uint32_t lane, At&& at) {
+__device__ __forceinline__ bool put_values(uint8_t* half, uint32_t rows, bool q8, uint32_t lane, uint32_t b0, uint32_t b1, At&& at) {
     const uint32_t g = lane / 4, t = lane % 4;
     bool fine = true;
     const bool on[2] = {(rows >> g & 1) != 0, (rows >> (g + 8) & 1) != 0};
@@ -138,7 +138,7 @@ __device__ __forceinline__ bool put_values(uint8_t* half, uint32_t rows, bool q8
     }
     // rolled: a step of a few rows waits for its instructions (unrolled, 24 rows took 13 us, half of it for those)
 #pragma unroll 1
-    for (uint32_t b = 0; b < D / 32; ++b) {
+    for (uint32_t b = b0; b < b1; ++b) {
         float v[2][8];
         uint32_t out[4][2];   // [i][slots 2t, 2t + 1 | 8 more]: binary16 values, or codes
 #pragma unroll
@@ -245,7 +245,7 @@ template <> struct Raw4<false> {
 // Blocks of three kinds. Rows that go out as rows: a block takes RB rows and as many heads as its threads hold at eight dims each; the rows' values are under
 // way while the threads compute the rows' angles, one each. Keys that go into the cache: a block per four slots, a warp per head. Values that do: a
 // warp per group of 16 slots and head. Measured, 32 + 8 heads of 128 dims: 8 FP32 rows 2.1 us, the pitch of launches; 4096 binary16 rows 18 us, 84 MB at 4.6 TB/s, from
-// the L2 in part, bound by instructions (71 % of the issue slots). Into a Q8_0 cache: 38 rows of six drafts 10.3 us, a chain of latencies; 4024 rows of
+// the L2 in part, bound by instructions (71 % of the issue slots). Into a Q8_0 cache: 38 rows of six drafts 6.6 us, a chain of latencies; 4024 rows of
 // prompts 39.5 us, bound by the 64-bit arithmetic of the keys and by instructions (67 % of the issue slots), and without norm and rotation 17.8.
 template <uint32_t D, bool IN16, bool OUT16, uint32_t RB>
 __device__ __forceinline__ void turn_rows(const tsp_qk_norm_rope_args& a, const HeadRows& r, uint32_t pass, uint32_t row0, uint32_t end, uint32_t* error) {
@@ -337,13 +337,12 @@ turn_rows_kernel(const tsp_qk_norm_rope_args a, const HeadRows r, uint32_t passe
     turn_rows<D, IN16, OUT16, RB>(a, r, blockIdx.x % passes, blockIdx.x / passes * RB, rows, error);
 }
 
-// Grid: value blocks, key blocks, then `passes` blocks for every RB query rows. A key block: four slots (a quarter of a group), a warp per head.
-constexpr uint32_t kKeyRows = 4;
+// Grid: value blocks (a warp per group, head and `parts`-th of its dims), key blocks, then `passes` blocks for every RB query rows. A key block: RB slots of a group (a row), a warp per head.
 template <uint32_t D, bool IN16, bool OUT16, uint32_t RB>
 __global__ void __launch_bounds__(kHeadThreads)
-append_rows_kernel(const tsp_qk_norm_rope_args a, const HeadRows r, const tsp_kv_cache cache, const tsp_kv_batch batch, uint32_t values, uint32_t keys, uint32_t passes,
-                   uint32_t* error) {
-    __shared__ double cs[kKeyRows][D / 2], sn[kKeyRows][D / 2], exchange[kHeadThreads / 32][D];
+append_rows_kernel(const tsp_qk_norm_rope_args a, const HeadRows r, const tsp_kv_cache cache, const tsp_kv_batch batch, uint32_t values, uint32_t parts, uint32_t keys,
+                   uint32_t passes, uint32_t* error) {
+    __shared__ double cs[RB][D / 2], sn[RB][D / 2], exchange[kHeadThreads / 32][D];
     pdl_launch_dependents();
     pdl_wait();
     const uint32_t tid = threadIdx.x, lane = tid % 32, warp = tid / 32, places = kv_group_places(batch.rows, batch.sequences);
@@ -357,21 +356,32 @@ append_rows_kernel(const tsp_qk_norm_rope_args a, const HeadRows r, const tsp_kv
     uint32_t seq, row0, mask;
     uint64_t slot0;
     if (blockIdx.x < values) {
-        const uint32_t task = blockIdx.x * (kHeadThreads / 32) + warp, place = task / cache.kv_heads, head = task % cache.kv_heads;
+        const uint32_t task = blockIdx.x * (kHeadThreads / 32) + warp, part = task % parts, place = task / parts / cache.kv_heads, head = task / parts % cache.kv_heads;
         if (place >= places || !kv_group_of_place(batch, place, lane, seq, slot0, row0, mask)) return;
         uint8_t* group = kv_group(cache, seq, slot0, head, error);
         if (!group) return;
-        const bool fine = put_values<D, IN16>(group + kv_half_bytes(D, q8), mask, q8, lane,
+        const bool fine = put_values<D, IN16>(group + kv_half_bytes(D, q8), mask, q8, lane, part * (D / 32 / parts), (part + 1) * (D / 32 / parts),
                                               [&](uint32_t t) { return r.v + static_cast<uint64_t>(row0 + t) * r.v_stride + head * D * (IN16 ? 2u : 4u); });
         if (!fine) raise_error(error, TSP_ERR_NONFINITE);
         return;
     }
-    constexpr uint32_t NV = D / 32, QUARTERS = kKvGroup / kKeyRows;
-    const uint32_t quarter = (blockIdx.x - values) % QUARTERS, half = a.rotary_dim / 2;
-    if (!kv_group_of_place(batch, (blockIdx.x - values) / QUARTERS, lane, seq, slot0, row0, mask)) return;
-    mask &= ((1u << kKeyRows) - 1) << (quarter * kKeyRows);
-    if (!mask) return;
-    const uint32_t t0 = __ffs(mask) - 1, t1 = 32 - __clz(mask);   // the quarter's slots of this step
+    constexpr uint32_t NV = D / 32, LOTS = kKvGroup / RB;
+    const uint32_t half = a.rotary_dim / 2;
+    if constexpr (RB == 1) {   // a block is a row
+        uint32_t node;
+        if (!kv_row(batch, blockIdx.x - values, lane, seq, node)) return;
+        const uint64_t slot = static_cast<uint64_t>(batch.d_lengths[seq]) + node;
+        const uint32_t t = static_cast<uint32_t>(slot % kKvGroup);
+        slot0 = slot - t;
+        row0 = blockIdx.x - values - t;   // modulo 2^32
+        mask = 1u << t;
+    } else {
+        const uint32_t lot = (blockIdx.x - values) % LOTS;
+        if (!kv_group_of_place(batch, (blockIdx.x - values) / LOTS, lane, seq, slot0, row0, mask)) return;
+        mask &= ((1u << RB) - 1) << (lot * RB);
+        if (!mask) return;
+    }
+    const uint32_t t0 = __ffs(mask) - 1, t1 = 32 - __clz(mask);   // the lot's slots of this step
     auto key_row = [&](uint32_t t, uint32_t h) { return r.k + static_cast<uint64_t>(row0 + t) * r.k_stride + h * D * (IN16 ? 2u : 4u); };
     float next[NV];
     if (warp < cache.kv_heads) load_run<IN16>(key_row(t0, warp), lane * NV, next);
@@ -604,8 +614,8 @@ cache_keep_kernel(const tsp_kv_cache cache, const tsp_kv_batch batch, const uint
     }
 }
 
-static uint32_t value_blocks(const tsp_kv_cache& c, const tsp_kv_batch& b) {
-    return (kv_group_places(b.rows, b.sequences) * c.kv_heads + kHeadThreads / 32 - 1) / (kHeadThreads / 32);
+static uint32_t value_blocks(const tsp_kv_cache& c, const tsp_kv_batch& b, uint32_t parts) {
+    return (kv_group_places(b.rows, b.sequences) * c.kv_heads * parts + kHeadThreads / 32 - 1) / (kHeadThreads / 32);
 }
 
 template <uint32_t D, bool IN16, bool OUT16>
@@ -620,12 +630,17 @@ static int launch_head_rows_d(const tsp_qk_norm_rope_args& a, const HeadRows& r,
         else TSP_CUDA(launch_pdl(turn_rows_kernel<D, IN16, OUT16, 4>, dim3(passes * ((rows + 3) / 4)), dim3(width), 0, st, a, r, passes, rows, error));
         return TSP_OK;
     }
-    const uint32_t values = value_blocks(*cache, *batch), passes = (lanes + threads - 1) / threads, at_least_one = passes ? passes : 1;
-    const uint32_t keys = kv_group_places(batch->rows, batch->sequences) * (kKvGroup / kKeyRows);
-    if (rows * passes <= 2 * sms)
-        TSP_CUDA(launch_pdl(append_rows_kernel<D, IN16, OUT16, 1>, dim3(values + keys + passes * rows), dim3(threads), 0, st, a, r, *cache, *batch, values, keys, at_least_one, error));
-    else
-        TSP_CUDA(launch_pdl(append_rows_kernel<D, IN16, OUT16, 4>, dim3(values + keys + passes * ((rows + 3) / 4)), dim3(threads), 0, st, a, r, *cache, *batch, values, keys, at_least_one, error));
+    // Few groups: a warp for each 32 dims of a group and head, which looks at the whole head but writes a quarter (of 128 dims): a warp's chain of latencies is the
+    // call's time. With the keys a row a block, 16 sequences of one token 6.7 us and 4.8 so, 772 rows of 64 (176 blocks without) 13.5 and 11.8; more blocks have
+    // enough warps without: 256 sequences of one token (528) 12.5 and 16.9 so.
+    const uint32_t parts = 4 * value_blocks(*cache, *batch, 1) <= 5 * sms ? D / 32 : 1, values = value_blocks(*cache, *batch, parts);
+    const uint32_t passes = (lanes + threads - 1) / threads, at_least_one = passes ? passes : 1;
+    if (rows * at_least_one <= 2 * sms) {
+        TSP_CUDA(launch_pdl(append_rows_kernel<D, IN16, OUT16, 1>, dim3(values + rows + passes * rows), dim3(threads), 0, st, a, r, *cache, *batch, values, parts, rows, at_least_one, error));
+    } else {
+        const uint32_t keys = kv_group_places(batch->rows, batch->sequences) * (kKvGroup / 4);
+        TSP_CUDA(launch_pdl(append_rows_kernel<D, IN16, OUT16, 4>, dim3(values + keys + passes * ((rows + 3) / 4)), dim3(threads), 0, st, a, r, *cache, *batch, values, parts, keys, at_least_one, error));
+    }
     return TSP_OK;
 }
 

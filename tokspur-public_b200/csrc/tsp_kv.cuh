@@ -33,6 +33,17 @@ __device__ __forceinline__ uint8_t* kv_group(const tsp_kv_cache& c, uint32_t seq
     return nullptr;
 }
 
+// Sequence of a row, by a whole warp in two steps of 32 offsets each (sequences <= 1024); false for a row of the padding
+__device__ __forceinline__ bool kv_row(const tsp_kv_batch& b, uint32_t row, uint32_t lane, uint32_t& seq, uint32_t& node) {
+    const uint32_t step = (b.sequences + 31) / 32;
+    const uint32_t a = __popc(__ballot_sync(0xffffffffu, (lane + 1) * step <= b.sequences && b.d_row_offsets[min((lane + 1) * step, b.sequences)] <= row)) * step;
+    seq = a + __popc(__ballot_sync(0xffffffffu, lane < step && a + lane + 1 <= b.sequences && b.d_row_offsets[min(a + lane + 1, b.sequences)] <= row));
+    if (seq >= b.sequences) return false;
+    const uint32_t first = b.d_row_offsets[seq], end = b.d_row_offsets[seq + 1];
+    node = row - first;
+    return first <= row && row < end && end <= b.rows;
+}
+
 // 8 x 8 matrix of binary16 over a warp, transposed: lane (g, t) gives entries (g, 2t), (g, 2t + 1) and gets (2t, g), (2t + 1, g)
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
     uint32_t r;
