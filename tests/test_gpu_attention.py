@@ -658,3 +658,62 @@ def test_wide_tiles_large_scores_and_values(type_, at):
         # weights, the low parts' and the result's rounding; 2^-25: half of binary16's smallest step
         tol = vmax * (4 * e + 4 * U16) + U16 * np.abs(want) + 2.0 ** -25
         assert (np.abs(got[j] - want) <= tol).all(), (type_, at, j)
+
+
+# ---- the cache write's other splits: many sequences (a warp for a whole head's values), more rows than two blocks an SM (four slots a key block)
+
+@pytest.mark.parametrize("type_", ["q8_0", "f16"])
+@pytest.mark.parametrize("counts", [[1] * 250, [1, 0, 2] * 133, [90, 7, 0, 260]])
+def test_append_of_many_rows_or_sequences(type_, counts):
+    dim, heads, page = 128, 8, 16
+    lengths = [(5 * i) % 23 for i in range(len(counts))]
+    rng = np.random.default_rng(len(counts))
+    p = R.Pages(rng, type_, page, heads, dim, [a + b for a, b in zip(counts, lengths)])
+    cache, (batch, off) = make_cache(p), make_batch(counts, lengths, rows=sum(counts) + 2)
+    k, v = (rng.normal(size=(batch.rows, heads, dim)).astype(np.float32) for _ in range(2))
+    k[3, 1, 7] = np.inf                                # one head of one row: zeros
+    v[5, 2, 9] = np.nan
+    err = error_word()
+    A.kv_cache_append(cache, batch, dev(k), dev(v), err)
+    assert int(err) == capi.ERR_NONFINITE
+    k[3, 1], v[5, 2] = 0, 0
+    for s in range(len(counts)):
+        for j in range(counts[s]):
+            p.put(s, lengths[s] + j, k[off[s] + j].astype(np.float64), v[off[s] + j].astype(np.float64))
+    assert np.array_equal(cache.pages.cpu().numpy(), p.data)
+
+
+@pytest.mark.parametrize("type_", ["q8_0", "f16"])
+@pytest.mark.parametrize("dim,rotary,style,dtype", [(64, 64, "pairs", "f16"), (128, 128, "halves", "f32"), (256, 128, "halves", "f32")])
+def test_fused_norm_rotation_and_append_of_many_rows(type_, dim, rotary, style, dtype):
+    rng = np.random.default_rng(dim + 1)
+    counts, lengths, heads, hq = [100, 0, 257, 1], [9, 3, 14, 0], 2, 4
+    rows = sum(counts)
+    p = R.Pages(rng, type_, 64, heads, dim, [a + b for a, b in zip(counts, lengths)])
+    cache, (batch, off) = make_cache(p), make_batch(counts, lengths, rows=rows + 3)
+    x = rng.normal(size=(rows + 3, hq + 2 * heads, dim)).astype(NP[dtype])
+    pos = rng.integers(0, 20000, rows + 3).astype(np.uint32)
+    wq, wk, f = (1 + 0.1 * rng.normal(size=dim)).astype(np.float32), (1 + 0.1 * rng.normal(size=dim)).astype(np.float32), inv_freq(rotary)
+    t, err = dev(x), error_word()
+    q_out = torch.full((rows + 3, hq, dim), 3.0, dtype=t.dtype, device="cuda")
+    A.qk_norm_rope_append(A.QkNormRope(dim, rotary, style, dev(f), dev(wq), dev(wk)), cache, batch, t[:, :hq], t[:, hq:hq + heads], t[:, hq + heads:], dev(pos), q_out, err)
+    assert int(err) == 0 and (q_out[rows:] == 3).all()
+    check_turned(q_out[:rows].cpu().numpy(), R.turned(x[:rows, :hq], wq, pos[:rows], f, rotary, style, 1e-6), dtype)
+    want = R.turned(x[:rows, hq:hq + heads], wk, pos[:rows], f, rotary, style, 1e-6)
+    for s in range(4):
+        for j in range(counts[s]):
+            p.put(s, lengths[s] + j, want[off[s] + j], x[off[s] + j, hq + heads:].astype(np.float64))
+    assert np.array_equal(cache.pages.cpu().numpy(), p.data)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_stages_of_halves_without_a_page(dtype):
+    """256 dims of binary16: keys and values arrive one after the other; a unit without a page passes both."""
+    s = Step(29, "f16", 256, 16, 2, 3, [5, 9, 2], [700, 350, 40], dtype, True)
+    out, err = s.run()
+    assert err == 0
+    s.check(out)
+    s.p.table[1, 3] = 0x7fffffff
+    out, err = s.run()
+    assert err & capi.ERR_INDEX and (out[5:14] == 0).all()
+    s.check(out, skip=(1,))

@@ -26,15 +26,16 @@ def _elsewhere(name, t, device):
 def _rows(name: str, t: torch.Tensor, dtype: torch.dtype, heads: int, dim: int, least: int, device: int) -> tuple[int, int]:
     """Pointer and row stride in bytes of [rows, heads, dim], after the checks that the library cannot make. A call of a few microseconds is
     in good part these lines: they ask each tensor as little as they can."""
-    stride = t.stride()
-    if len(stride) != 3 or stride[2] != 1 or (stride[1] != dim and heads > 1) or t.dtype is not dtype or dtype not in SIZES:
+    try:
+        (rows, h, d), (step, between, one) = t.shape, t.stride()
+        size = SIZES[dtype]
+    except (ValueError, KeyError):
+        _refuse(name, t, dtype, heads, dim, least)
+    if rows < least or h != heads or d != dim or one != 1 or (between != dim and h != 1) or t.dtype is not dtype:
         _refuse(name, t, dtype, heads, dim, least)
     if t.get_device() != device:
         _elsewhere(name, t, device)
-    rows, h, d = t.shape
-    if h != heads or d != dim or rows < least:
-        _refuse(name, t, dtype, heads, dim, least)
-    return t.data_ptr(), stride[0] * SIZES[dtype]
+    return t.data_ptr(), step * size
 
 
 def _words(name: str, t: torch.Tensor, dtype: torch.dtype, least: int, device: int) -> int:
@@ -46,6 +47,7 @@ def _words(name: str, t: torch.Tensor, dtype: torch.dtype, least: int, device: i
 
 
 _entries: dict = {}
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 # the current stream's handle without a Stream object around it (a microsecond less a call), where torch has it
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
@@ -57,7 +59,7 @@ def _call(name: str, device: int, error: torch.Tensor | None, *args) -> None:
         entry = _entries[name] = getattr(capi.lib(), name)
     if error is not None and error.get_device() != device:
         _elsewhere("error word", error, device)
-    if device != torch.cuda.current_device():
+    if device != _current_device():
         if device < 0:
             raise ValueError(f"{name}: tensors in host memory")
         with torch.cuda.device(device):
@@ -117,7 +119,10 @@ class QkNormRope:
             if t is not None and (t.dtype != torch.float32 or t.numel() < n or not t.is_contiguous()):
                 raise ValueError("norm weights and frequencies are dense float32")
         self.tensors, self.head_dim = (inv_freq, q_norm, k_norm), head_dim
-        self.devices = {t.get_device() for t in self.tensors if t is not None}
+        devices = {t.get_device() for t in self.tensors if t is not None}
+        if len(devices) > 1:
+            raise ValueError(f"norm weights and frequencies on devices {sorted(devices)}")
+        self.device = devices.pop() if devices else None
         self.struct = capi.QkNormRope(*(None if t is None else t.data_ptr() for t in (q_norm, k_norm, inv_freq)), head_dim, rotary_dim, STYLES[style], eps, magnitude)
         self.ref = C.byref(self.struct)
 
@@ -132,8 +137,8 @@ def _check_batch(cache: KvCache, batch: KvBatch) -> int:
 
 
 def _check_turn(turn: QkNormRope, device: int):
-    if turn.devices and turn.devices != {device}:
-        raise ValueError(f"norm weights and frequencies on devices {sorted(turn.devices)}, the call is for CUDA device {device}")
+    if turn.device is not None and turn.device != device:
+        raise ValueError(f"norm weights and frequencies on devices {[turn.device]}, the call is for CUDA device {device}")
 
 
 def qk_norm_rope(turn: QkNormRope, q, k, positions, q_out, k_out, error):
