@@ -19,7 +19,7 @@ def turned(x, weight, positions, inv_freq, rotary, style, eps, magnitude=1.0):
 
 def quantised(x):
     """[..., dim] -> (codes int, scales float16 [..., dim/32]) of the Q8_0 rule, in float64."""
-    blocks = x.astype(np.float64).reshape(*x.shape[:-1], -1, 32)
+    blocks = x.astype(np.float64).reshape(*x.shape[:-1], x.shape[-1] // 32, 32)
     d = (np.abs(blocks).max(-1) / 127).astype(np.float32).astype(np.float16)
     df = d.astype(np.float64)[..., None]
     q = np.where(df > 0, np.clip(np.rint(blocks / np.where(df > 0, df, 1)), -127, 127), 0)

@@ -717,3 +717,57 @@ def test_stages_of_halves_without_a_page(dtype):
     out, err = s.run()
     assert err & capi.ERR_INDEX and (out[5:14] == 0).all()
     s.check(out, skip=(1,))
+
+
+# ---- calls that the documentation allows: the most sequences, none at all, two at once
+
+@pytest.mark.parametrize("group,dtype", [(2, "f32"), (4, "f16"), (64, "f16")])
+def test_the_most_sequences(group, dtype):
+    n = capi.KV_MAX_SEQUENCES
+    s = Step(31, "q8_0", 64, 16, 1, group, [1] * (n - 3) + [0, 2, 3], [i % 19 for i in range(n)], dtype, True)
+    out, err = s.run()
+    assert err == 0
+    s.check(out)
+
+
+@pytest.mark.parametrize("group,dtype", [(2, "f32"), (32, "f16")])
+def test_a_step_without_rows(group, dtype):
+    """Three sequences, none with a token, in buffers of four rows: nothing is touched."""
+    s = Step(33, "q8_0", 128, 16, 2, group, [0, 0, 0], [5, 0, 40], dtype, False, pad_rows=4)
+    cache = make_cache(s.p)
+    before, err = cache.pages.clone(), error_word()
+    out, code = s.run(cache, most=4)
+    assert code == 0 and (out == 11).all()
+    k = torch.ones(s.batch.rows, 2, 128, device="cuda")
+    A.kv_cache_append(cache, s.batch, k, k, err)
+    A.kv_cache_keep(cache, s.batch, torch.zeros(s.batch.rows, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda"), err)
+    q = torch.full((s.batch.rows, 4, 128), 2.0, device="cuda")
+    A.qk_norm_rope_append(A.QkNormRope(128, 0, "halves", None), cache, s.batch, q, k, k, torch.zeros(s.batch.rows, dtype=torch.int32, device="cuda"), q, err)
+    A.kv_cache_read(cache, s.batch, k, None, err)
+    assert int(err) == 0 and torch.equal(cache.pages, before) and (k == 1).all() and (q == 2).all()
+
+
+@pytest.mark.parametrize("group", [4, 32])
+def test_two_captured_calls_at_once_with_a_workspace_each(group):
+    steps = [Step(seed, "q8_0", 128, 32, 2, group, [3, 2], [1900, 700], "f16", True) for seed in (35, 36)]
+    wants, graphs, outs, errs, keep = [], [], [], [], []
+    for s in steps:
+        want, err = s.run()
+        assert err == 0
+        s.check(want)
+        wants.append(want)
+        cache, q, mask, scratch, err, out = make_cache(s.p), dev(s.q), dev(s.mask), A.tree_attention_scratch(), error_word(), torch.full_like(want, 11.0)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(8):
+                A.tree_attention(cache, s.batch, q, out, mask, s.most, s.scale, scratch, err)
+        graphs.append(graph); outs.append(out); errs.append(err); keep.append((cache, q, mask, scratch))
+    streams = [torch.cuda.Stream() for _ in steps]
+    for _ in range(6):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for want, out, err in zip(wants, outs, errs):
+        assert int(err) == 0 and torch.equal(out, want)
