@@ -220,6 +220,7 @@ tree_attention_kernel(const AttnParams p) {
                 return yes;
             };
             auto pass = [&]() {   // the stage has been read: filled again
+                fence_async_smem();
                 __syncwarp();
                 if (!lost) issue(stage);
                 if (++stage == P) { stage = 0; phase ^= 1; }

@@ -30,6 +30,9 @@ struct AttnItem {
     bool dead;               // out of range: zeros
 };
 
+// Between a thread's reads (or writes) of shared memory and what asynchronous copies (or MMAs) do to it next: the copies write through another proxy, so that
+// neither a warp barrier nor an arrival alone keeps them behind reads whose values nobody has used yet. Every thread that has read fences, then the warp meets.
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -363,7 +363,7 @@ tree_mma_kernel(const AttnParams p) {
                         }
                     }
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                fence_async_smem();
                 __syncwarp();
                 if (lane == 0) { mbar_arrive(&sm.k_ready[buf]); mbar_arrive(&sm.code_empty[st]); }
             }
@@ -415,7 +415,7 @@ tree_mma_kernel(const AttnParams p) {
                         }
                     }
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                fence_async_smem();
                 __syncwarp();
                 if (lane == 0) { mbar_arrive(&sm.v_ready[buf]); mbar_arrive(&sm.code_empty[st]); }
             }
