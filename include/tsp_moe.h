@@ -340,7 +340,7 @@ int tsp_kv_cache_keep(const tsp_kv_cache* cache, const tsp_kv_batch* batch, cons
  *   tokens 0..i of the step. A row that sees nothing gets zeros. One token per sequence is plain decode.
  * The step's keys and values have to be in the cache (append first). max_rows: the most rows of a sequence in this batch, 1..TSP_KV_MAX_DRAFT; a
  * sequence with more raises TSP_ERR_INDEX, as do slots or pages out of range: its rows are then zeros. Slots that a row does not see
- * never reach its result, whatever they hold; a result that is not finite is written as zeros for that head and raises TSP_ERR_NONFINITE.
+ * have no part in its result, whatever they hold (they may move its last rounding, as any other tiling of the sum does); a result that is not finite is written as zeros for that head and raises TSP_ERR_NONFINITE.
  * q and out rows have one dtype. FP32 rows are computed with FP32 accuracy (products of exact parts, FP32 sums); binary16 rows with
  * binary16 products and FP32 sums.
  * d_scratch: tsp_tree_attention_scratch_bytes() (for the current device), 16-byte aligned, zero before its first use; every call leaves what the next one needs.

@@ -29,3 +29,84 @@ def test_many_refills_give_the_same_bits(type_, dim, group, dtype):
         for out in outs:
             differing += (out != want).sum()
     assert int(differing) == 0 and int(err) == 0
+
+
+# ---- slots that a row does not see: finite or not, large or not, they cost it nothing
+
+def check_row(s, out, r, seq, j, k, v):
+    """Step.check's bound for one row over the slots k, v of its sequence; returns the squares of error and value."""
+    vis = s.visible(seq, j)
+    want, spread, vmax = R.attended(s.q[r], k, v, vis, s.scale)
+    e = ((s.dim + 8) * U32 + (U16 if s.dtype == "f16" else 0)) * spread
+    tol = vmax * (4 * e + (4 * U16 if s.dtype == "f16" else (len(vis) + 64) * U32)) + (U16 * np.abs(want) + 2.0 ** -25 if s.dtype == "f16" else 0)
+    d = np.abs(out[r] - want)
+    assert (d <= tol).all(), (seq, j, float((d / tol).max()), float(d.max()))
+    return float((d * d).sum()), float((want * want).sum())
+
+
+def poked(s, hidden, which, value):
+    """Rewrites the scales (binary16 cache: the values) of token `hidden[seq]` of every sequence's step."""
+    for seq, token in enumerate(hidden):
+        s.p.poke_scale(seq, s.lengths[seq] + token, value, which=which)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("type_,dim,group", [("q8_0", 128, 2), ("q8_0", 64, 3), ("q8_0", 256, 2), ("f16", 128, 2), ("q8_0", 128, 32), ("q8_0", 64, 32), ("f16", 64, 32)])
+@pytest.mark.parametrize("which,value", [((1,), 6e4), ((1,), 512.0), ((0,), 6e4), ((0,), np.inf), ((0,), np.nan), ((1,), -np.inf), ((0, 1), 6e4)])
+@pytest.mark.parametrize("small", [1.0, 2.0 ** -6])
+def test_hidden_slots_cost_the_other_rows_nothing(dtype, type_, dim, group, which, value, small):
+    """Token 1 of every step holds a scale (binary16: values) far above the others', or none that is finite; rows whose word hides it have the bounds of a
+    step without it. The third step's tokens span units of both kernels, and units behind the token's own."""
+    s = Step(43, type_, dim, 16, 2, group, [6, 12, 40], [0, 57, 300], dtype, True)
+    if small != 1:                                     # the other slots' values and keys; the same scores
+        s.q = (s.q.astype(np.float64) / small).astype(s.q.dtype)
+        for seq in range(3):
+            for j in range(len(s.k[seq])):
+                k, v = s.k[seq][j] * small, s.v[seq][j] * small
+                s.p.put(seq, j, k, v)
+                s.k[seq][j], s.v[seq][j] = R.cached(k, type_), R.cached(v, type_)
+    s.mask |= np.uint64(1)                             # a row of a short step sees something
+    s.mask[::2] &= ~np.uint64(2)
+    poked(s, [1, 1, 1], which, value)
+    out, err = s.run()
+    assert np.isfinite(value) or err == capi.ERR_NONFINITE
+    got = out.cpu().numpy().astype(np.float64)
+    assert np.isfinite(got).all()
+    num = den = 0.0
+    for seq in range(3):
+        for j in range(s.counts[seq]):
+            r = s.off[seq] + j
+            if not int(s.mask[r]) & 2:
+                x, y = check_row(s, got, r, seq, j, s.k[seq], s.v[seq])
+                num, den = num + x, den + y
+    assert np.sqrt(num / den) <= (2e-3 if dtype == "f16" else 5e-6), np.sqrt(num / den)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("group", [2, 32])
+@pytest.mark.parametrize("which,value", [((1,), 512.0), ((0,), 64.0), ((0, 1), 256.0)])
+def test_rows_that_see_such_a_slot(dtype, group, which, value):
+    """The rows on the other side, against sums over what the cache then holds (finite scales, results within binary16's range)."""
+    s = Step(47, "q8_0", 128, 16, 2, group, [6, 12, 40], [0, 57, 300], dtype, True)
+    s.mask |= np.uint64(3)
+    for seq in range(3):                               # codes small enough that binary16 holds the results
+        at = s.lengths[seq] + 1
+        k, v = s.k[seq][at], np.clip(s.v[seq][at], -0.5, 0.5)
+        s.p.put(seq, at, k, v)
+    poked(s, [1, 1, 1], which, value)
+    for seq in range(3):
+        s.k[seq][s.lengths[seq] + 1], s.v[seq][s.lengths[seq] + 1] = s.p.get(seq, s.lengths[seq] + 1)
+    out, err = s.run()
+    got = out.cpu().numpy().astype(np.float64)
+    limit = 65504 if dtype == "f16" else np.inf
+    for seq in range(3):
+        for j in range(s.counts[seq]):
+            r = s.off[seq] + j
+            want, _, _ = R.attended(s.q[r], s.k[seq], s.v[seq], s.visible(seq, j), s.scale)
+            fits = [h for h in range(s.hq) if np.abs(want[h]).max() < 0.9 * limit]
+            vis = s.visible(seq, j)
+            for h in fits:
+                w, spread, vmax = R.attended(s.q[r][h:h + 1], s.k[seq][:, h // group][:, None], s.v[seq][:, h // group][:, None], vis, s.scale)
+                e = ((s.dim + 8) * U32 + (U16 if dtype == "f16" else 0)) * spread
+                tol = vmax * (4 * e + (4 * U16 if dtype == "f16" else (len(vis) + 64) * U32)) + (U16 * np.abs(w[0]) + 2.0 ** -25 if dtype == "f16" else 0)
+                assert (np.abs(got[r][h] - w[0]) <= tol).all(), (seq, j, h, float((np.abs(got[r][h] - w[0]) / tol).max()))

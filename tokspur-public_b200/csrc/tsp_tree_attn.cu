@@ -205,8 +205,9 @@ tree_attention_kernel(const AttnParams p) {
 #pragma unroll
                     for (uint32_t c = 0; c < 4; ++c) o[k][i][c] = 0.f;
             // A row's weight is 2^(score + ref), ref = lift - m: m, the score that was largest when the reference last moved; lift, Q8_0: the power of two
-            // that keeps weights times value scales below 2^15 (it only falls), else kUp
-            float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f, lift = Q8 ? 20.f : kUp;
+            // that keeps weights times the value scales of the slots that the row has seen below 2^15 (it only falls), else kUp. limit_v: the value scale that the
+            // higher of the two lifts allows
+            float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f, lift_a = Q8 ? 20.f : kUp, lift_b = lift_a;
             float ref_a = 0.f, ref_b = 0.f, limit_a = -INFINITY, limit_b = -INFINITY, limit_v = Q8 ? 0x1p-13f : INFINITY;
             bool dead = false;
 
@@ -311,7 +312,9 @@ tree_attention_kernel(const AttnParams p) {
                         keep[n] = (drop >> (8 * n + 2 * t) & 1 ? 0u : 0x0000ffffu) | (drop >> (8 * n + 2 * t) & 2 ? 0u : 0xffff0000u);
                 }
                 [[maybe_unused]] float dv[Q8 ? NB : 1][2];   // value scales of slots g, g + 8
-                float widest = 0.f;
+                // largest value scale that a row sees: not that of a slot hidden from it, which would push the weights of the others under binary16's
+                // smallest numbers. Inside the context both rows see every slot.
+                float widest_a = 0.f, widest_b = 0.f;
                 if constexpr (Q8) {
 #pragma unroll
                     for (uint32_t k = 0; k < NB; ++k) {
@@ -319,30 +322,45 @@ tree_attention_kernel(const AttnParams p) {
                         dv[k][0] = __half2float(*reinterpret_cast<const __half*>(scales + g * 2));
                         dv[k][1] = __half2float(*reinterpret_cast<const __half*>(scales + g * 2 + 16));
                         if constexpr (EDGE) { if (drop >> g & 1) dv[k][0] = 0.f; if (drop >> (g + 8) & 1) dv[k][1] = 0.f; }
-                        widest = fmaxf(widest, fmaxf(fabsf(dv[k][0]), fabsf(dv[k][1])));
+                        if constexpr (EDGE) {
+#pragma unroll
+                            for (uint32_t n = 0; n < 2; ++n) {
+                                if (s[2 * n] != -INFINITY) widest_a = fmaxf(widest_a, fabsf(dv[k][n]));
+                                if (s[2 * n + 1] != -INFINITY) widest_b = fmaxf(widest_b, fabsf(dv[k][n]));
+                            }
+                        } else widest_a = fmaxf(widest_a, fmaxf(fabsf(dv[k][0]), fabsf(dv[k][1])));
                     }
+                    if constexpr (!EDGE) widest_b = widest_a;
                 }
                 float xa = -INFINITY, xb = -INFINITY;
 #pragma unroll
                 for (uint32_t i = 0; i < NS; ++i) { if (second(i)) xb = fmaxf(xb, s[i]); else xa = fmaxf(xa, s[i]); }
                 xa *= fa; xb *= fb;
-                if (__any_sync(NONE, xa > limit_a || xb > limit_b || widest > limit_v)) {
+                if (__any_sync(NONE, xa > limit_a || xb > limit_b || fmaxf(widest_a, widest_b) > limit_v)) {
 #pragma unroll
                     for (uint32_t x = 4; x < 32; x *= 2) { xa = fmaxf(xa, __shfl_xor_sync(NONE, xa, x)); xb = fmaxf(xb, __shfl_xor_sync(NONE, xb, x)); }
                     xa = fmaxf(xa, ma); xb = fmaxf(xb, mb);
-                    float fall = 0.f;
+                    float fall_a = 0.f, fall_b = 0.f;
                     if constexpr (Q8) {   // widest < 2^(e + 1): weights up to 2^kSlack times it times 2^lift stay below 2^15
-                        const uint32_t bits = __reduce_max_sync(NONE, __float_as_uint(widest));
-                        const float now = fminf(lift, 6.f - static_cast<float>(static_cast<int>(min(bits >> 23, 143u)) - 127));
-                        fall = now - lift;
-                        lift = now;
-                        limit_v = exp2f(7.f - lift);
+                        uint32_t wa, wb;
+                        if constexpr (EDGE) {
+#pragma unroll
+                            for (uint32_t x = 4; x < 32; x *= 2) {
+                                widest_a = fmaxf(widest_a, __shfl_xor_sync(NONE, widest_a, x)); widest_b = fmaxf(widest_b, __shfl_xor_sync(NONE, widest_b, x));
+                            }
+                            wa = __float_as_uint(widest_a); wb = __float_as_uint(widest_b);
+                        } else wa = wb = __reduce_max_sync(NONE, __float_as_uint(widest_a));
+                        auto lowered = [](float lift, uint32_t bits) { return fminf(lift, 6.f - static_cast<float>(static_cast<int>(min(bits >> 23, 143u)) - 127)); };
+                        const float now_a = lowered(lift_a, wa), now_b = lowered(lift_b, wb);
+                        fall_a = now_a - lift_a; fall_b = now_b - lift_b;
+                        lift_a = now_a; lift_b = now_b;
+                        limit_v = exp2f(7.f - fmaxf(lift_a, lift_b));
                     }
-                    const float r0 = ma == -INFINITY ? 0.f : exp2_approx(ma - xa + fall), r1 = mb == -INFINITY ? 0.f : exp2_approx(mb - xb + fall);
+                    const float r0 = ma == -INFINITY ? 0.f : exp2_approx(ma - xa + fall_a), r1 = mb == -INFINITY ? 0.f : exp2_approx(mb - xb + fall_b);
                     la *= ma == -INFINITY ? 1.f : r0; lb *= mb == -INFINITY ? 1.f : r1;   // a NaN stays
                     ma = xa; mb = xb;
                     limit_a = ma + kSlack; limit_b = mb + kSlack;
-                    ref_a = ma == -INFINITY ? 0.f : lift - ma; ref_b = mb == -INFINITY ? 0.f : lift - mb;
+                    ref_a = ma == -INFINITY ? 0.f : lift_a - ma; ref_b = mb == -INFINITY ? 0.f : lift_b - mb;
 #pragma unroll
                     for (uint32_t k = 0; k < NB; ++k)
 #pragma unroll

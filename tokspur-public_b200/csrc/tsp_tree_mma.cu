@@ -17,11 +17,19 @@
 // Rounding: a Q8_0 value is code times scale, 18 bits. Tiles hold it as two binary16 numbers, high and low (exact, times a power of two that puts the unit's
 // largest scale at 2^7), and the MMAs run over both: what is left between the cache and a binary16 row is the weights' rounding, as on the warp MMAs. (High
 // parts alone: errors against 64 bits 4.1e-4 instead of 2.9e-4, half the MMAs.) A binary16 cache needs no low parts.
+// That power of two goes by all slots of the unit, also by drafted ones that some rows do not see. Up to 2^kTmSpread between their scales this costs such a
+// row nothing: values are exact up to 2^20, and weights reach down to 2^-24 of the row's largest. Beyond ("wild", at the end of the context only), warp 3
+// raises every slot's scales to the largest one's octave; its scores go back down by as much, its weights as far as the row's accumulator asks, both in
+// tensor memory and in rolled loops that no other unit enters (on the registers of the ordinary path they took 18 % of every call).
+#include <type_traits>
+
 #include "tsp_tree_attn.cuh"
 
 namespace tsp {
 
 constexpr uint32_t kTmLeastUnits = 4;   // of a block's run: 13 tokens over 1000 slots 18.8 us, 22.5 with eight
+// Octaves between the largest scales of two slots of a unit above which, at the end of the context, every slot gets a power of two of its own
+constexpr uint32_t kTmSpread = 8;
 constexpr uint32_t kTmRows = 128, kTmUnit = 64, kTmGroups = kTmUnit / kKvGroup;
 constexpr uint32_t kTmSoftmax = 4, kTmTiles = 8, kTmTileWarps = 8, kTmThreads = 32 * (kTmTiles + kTmTileWarps);   // first softmax warp, first tile warp
 // Registers after the hand-over between the warpgroups (setmaxnreg): together no more than the count at launch times the four warpgroups, or the softmax
@@ -55,6 +63,8 @@ struct TmSmem {
     // per unit (mod 8: the copies are four units ahead of the softmax at most): no page; the tiles' powers of two; drafted slots whose
     // values are not finite; slots that count as zero
     uint32_t gone[8], k_lift[8], v_lift[8], odd[8][2], drop[8][2];
+    uint32_t wild[8];                                     // units at the end of the context; bit 0: of keys, 1: of values
+    uint8_t k_raised[8][kTmUnit], v_raised[8][kTmUnit];   // octaves, by slot
     uint32_t tmem, last[2], span[2][2], bad_rows[kTmRows / 32];
     float tops[4][kTmRows];   // of the join
 };
@@ -68,6 +78,12 @@ __device__ __forceinline__ void tm_ld32(uint32_t at, float (&v)[32]) {
                    "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
                  : "r"(at));
 }
+__device__ __forceinline__ uint32_t tm_ld1(uint32_t at) {
+    uint32_t v;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void tm_st1(uint32_t at, uint32_t v) { asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(at), "r"(v) : "memory"); }
 __device__ __forceinline__ void tm_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_st32(uint32_t at, const uint32_t (&r)[32]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
@@ -257,57 +273,96 @@ tree_mma_kernel(const AttnParams p) {
                 const uint32_t st = j % S::kStages;
                 ok = tm_wait(&sm.code_full[st], (j / S::kStages) & 1);
                 if (!ok) break;
-                const uint8_t* stage = sm.ring[st];
+                uint8_t* stage = sm.ring[st];
                 const uint64_t slot0 = (u0 + j - start) * kTmUnit;
-                uint64_t drop = 0, odd_slots = 0;
-                const bool gone = sm.gone[j % 8] != 0, edge = slot0 + kTmUnit > length;
-                if (edge && !gone) {
-                    const uint64_t there = total - slot0 >= 64 ? ~0ull : (1ull << (total - slot0)) - 1;
-                    const uint64_t drafted = slot0 >= length ? ~0ull : ~0ull << (length - slot0);
-                    uint32_t odd[2] = {0, 0};
-                    if constexpr (Q8) {
-                        for (uint32_t i = lane; i < kTmGroups * NB * kKvGroup; i += 32) {
-                            const uint32_t gi = i / (NB * kKvGroup), x = i % (NB * kKvGroup), slot = gi * kKvGroup + x % kKvGroup;
-                            const uint32_t is = (*reinterpret_cast<const uint16_t*>(stage + gi * S::kGroupBytes + S::kHalf + kKvGroup * D + x * 2) & 0x7c00u) == 0x7c00u;
-                            if (slot < 32) odd[0] |= is << slot; else odd[1] |= is << (slot - 32);
+                // Two copies of the code, as the softmax has: what the end of the context needs delays no unit inside it (one copy: 8 % more)
+                auto look = [&](auto edge_tag) {
+                    constexpr bool EDGE = decltype(edge_tag)::value;
+                    uint64_t drop = 0, odd_slots = 0;
+                    const bool gone = EDGE && sm.gone[j % 8] != 0;
+                    if (EDGE && !gone) {
+                        const uint64_t there = total - slot0 >= 64 ? ~0ull : (1ull << (total - slot0)) - 1;
+                        const uint64_t drafted = slot0 >= length ? ~0ull : ~0ull << (length - slot0);
+                        uint32_t odd[2] = {0, 0};
+                        if constexpr (Q8) {
+                            for (uint32_t i = lane; i < kTmGroups * NB * kKvGroup; i += 32) {
+                                const uint32_t gi = i / (NB * kKvGroup), x = i % (NB * kKvGroup), slot = gi * kKvGroup + x % kKvGroup;
+                                const uint32_t is = (*reinterpret_cast<const uint16_t*>(stage + gi * S::kGroupBytes + S::kHalf + kKvGroup * D + x * 2) & 0x7c00u) == 0x7c00u;
+                                if (slot < 32) odd[0] |= is << slot; else odd[1] |= is << (slot - 32);
+                            }
+                        } else {
+                            for (uint32_t i = lane; i < kTmUnit * D; i += 32) {   // halves of V: [group][32 dims][m][g][t][i][e]
+                                const uint32_t gi = i / (kKvGroup * D), x = i % (kKvGroup * D), e = x % 4, tt = x / 8 % 4, slot = gi * kKvGroup + 2 * tt + (e & 1) + 8 * (e >> 1);
+                                const uint32_t is = (*reinterpret_cast<const uint16_t*>(stage + gi * S::kGroupBytes + S::kHalf + x * 2) & 0x7c00u) == 0x7c00u;
+                                if (slot < 32) odd[0] |= is << slot; else odd[1] |= is << (slot - 32);
+                            }
                         }
-                    } else {
-                        for (uint32_t i = lane; i < kTmUnit * D; i += 32) {   // halves of V: [group][32 dims][m][g][t][i][e]
-                            const uint32_t gi = i / (kKvGroup * D), x = i % (kKvGroup * D), e = x % 4, tt = x / 8 % 4, slot = gi * kKvGroup + 2 * tt + (e & 1) + 8 * (e >> 1);
-                            const uint32_t is = (*reinterpret_cast<const uint16_t*>(stage + gi * S::kGroupBytes + S::kHalf + x * 2) & 0x7c00u) == 0x7c00u;
-                            if (slot < 32) odd[0] |= is << slot; else odd[1] |= is << (slot - 32);
+                        odd_slots = (static_cast<uint64_t>(__reduce_or_sync(NONE, odd[1])) << 32 | __reduce_or_sync(NONE, odd[0])) & drafted & there;
+                        drop = odd_slots | ~there;
+                    }
+                    int ek = 21, ev = 21;
+                    [[maybe_unused]] uint32_t wild = 0;
+                    if constexpr (Q8) {   // largest scales: below 2^(e - 14), e the binary16 exponent; the tiles are times 2^(21 - e), codes times scales below 2^14
+                        uint32_t top[2];
+                        [[maybe_unused]] uint32_t low[2];   // smallest scales that are not zero, less one
+#pragma unroll
+                        for (uint32_t side = 0; side < 2; ++side) {
+                            constexpr uint32_t EACH = NB * 2;   // 16-byte pieces of a group's scales: eight slots of a block of 32 dims
+                            const uint32_t gi = lane / EACH % kTmGroups, x = lane % EACH;   // head_dim 64: the upper lanes look at the same again
+                            const uint4 d = *reinterpret_cast<const uint4*>(stage + gi * S::kGroupBytes + side * S::kHalf + kKvGroup * D + x * 16);
+                            uint32_t words[4] = {d.x & 0x7fff7fffu, d.y & 0x7fff7fffu, d.z & 0x7fff7fffu, d.w & 0x7fff7fffu};
+                            if constexpr (EDGE) {
+                                const uint32_t out = static_cast<uint32_t>(drop >> (gi * kKvGroup + x % 2 * 8));
+                                uint32_t least = 0xffffffffu;
+#pragma unroll
+                                for (uint32_t c = 0; c < 4; ++c) {
+                                    words[c] &= (out >> (2 * c) & 1 ? 0u : 0x0000ffffu) | (out >> (2 * c) & 2 ? 0u : 0xffff0000u);
+                                    least = __vminu2(least, __vsub2(words[c], 0x00010001u));   // zero wraps
+                                }
+                                low[side] = min(least & 0xffffu, least >> 16);
+                            }
+                            const uint32_t most = __vmaxu2(__vmaxu2(words[0], words[1]), __vmaxu2(words[2], words[3]));
+                            top[side] = max(most & 0xffffu, most >> 16);
+                        }
+                        ek = static_cast<int>(min(max(__reduce_max_sync(NONE, top[0]) >> 10, 1u), 30u));
+                        ev = static_cast<int>(min(max(__reduce_max_sync(NONE, top[1]) >> 10, 1u), 30u));
+                        if constexpr (EDGE) {
+                            // no two blocks so far apart: no two slots
+                            auto far = [&](uint32_t side) { return static_cast<uint32_t>(side ? ev : ek) > max((side ? low[1] : low[0]) >> 10, 1u) + kTmSpread; };
+                            if (__any_sync(NONE, far(0) || far(1)) && !gone) {
+#pragma unroll 1
+                                for (uint32_t side = 0; side < 2; ++side) {
+                                    if (!__any_sync(NONE, far(side))) continue;
+                                    wild |= 1u << side;
+                                    auto scale_of = [&](uint32_t slot, uint32_t b) {
+                                        return reinterpret_cast<__half*>(stage + slot / kKvGroup * S::kGroupBytes + side * S::kHalf + kKvGroup * D) + b * kKvGroup + slot % kKvGroup;
+                                    };
+#pragma unroll 1
+                                    for (uint32_t slot = lane; slot < kTmUnit; slot += 32) {
+                                        uint32_t own = 0;
+#pragma unroll 1
+                                        for (uint32_t b = 0; b < NB; ++b) own = max(own, __half_as_ushort(*scale_of(slot, b)) & 0x7fffu);
+                                        const uint32_t up = drop >> slot & 1 || !own ? 0u : static_cast<uint32_t>(side ? ev : ek) - min(max(own >> 10, 1u), 30u);
+                                        (side ? sm.v_raised : sm.k_raised)[j % 8][slot] = static_cast<uint8_t>(up);
+#pragma unroll 1
+                                        for (uint32_t b = 0; up && b < NB; ++b) *scale_of(slot, b) = __float2half_rn(__half2float(*scale_of(slot, b)) * pow2(static_cast<int>(up)));
+                                    }
+                                }
+                                fence_async_smem();   // the lanes' writes, before the copy that fills the stage next
+                                __syncwarp();
+                            }
                         }
                     }
-                    odd_slots = (static_cast<uint64_t>(__reduce_or_sync(NONE, odd[1])) << 32 | __reduce_or_sync(NONE, odd[0])) & drafted & there;
-                    drop = odd_slots | ~there;
-                }
-                int ek = 21, ev = 21;
-                if constexpr (Q8) {   // largest scales: below 2^(e - 14), e the binary16 exponent; the tiles are times 2^(21 - e), codes times scales below 2^14
-                    uint32_t top[2];
-#pragma unroll
-                    for (uint32_t side = 0; side < 2; ++side) {
-                        constexpr uint32_t EACH = NB * 2;   // 16-byte pieces of a group's scales: eight slots of a block of 32 dims
-                        const uint32_t gi = lane / EACH % kTmGroups, x = lane % EACH;   // head_dim 64: the upper lanes look at the same again
-                        const uint4 d = *reinterpret_cast<const uint4*>(stage + gi * S::kGroupBytes + side * S::kHalf + kKvGroup * D + x * 16);
-                        uint32_t words[4] = {d.x & 0x7fff7fffu, d.y & 0x7fff7fffu, d.z & 0x7fff7fffu, d.w & 0x7fff7fffu};
-                        if (edge) {
-                            const uint32_t out = static_cast<uint32_t>(drop >> (gi * kKvGroup + x % 2 * 8));
-#pragma unroll
-                            for (uint32_t c = 0; c < 4; ++c) words[c] &= (out >> (2 * c) & 1 ? 0u : 0x0000ffffu) | (out >> (2 * c) & 2 ? 0u : 0xffff0000u);
-                        }
-                        const uint32_t most = __vmaxu2(__vmaxu2(words[0], words[1]), __vmaxu2(words[2], words[3]));
-                        top[side] = max(most & 0xffffu, most >> 16);
+                    if (lane == 0) {
+                        sm.k_lift[j % 8] = 21 - ek; sm.v_lift[j % 8] = 21 - ev;
+                        if constexpr (EDGE) sm.wild[j % 8] = wild;
+                        sm.odd[j % 8][0] = static_cast<uint32_t>(odd_slots); sm.odd[j % 8][1] = static_cast<uint32_t>(odd_slots >> 32);
+                        sm.drop[j % 8][0] = static_cast<uint32_t>(drop); sm.drop[j % 8][1] = static_cast<uint32_t>(drop >> 32);
+                        mbar_arrive(&sm.code_known[st]);
                     }
-                    ek = static_cast<int>(min(max(__reduce_max_sync(NONE, top[0]) >> 10, 1u), 30u));
-                    ev = static_cast<int>(min(max(__reduce_max_sync(NONE, top[1]) >> 10, 1u), 30u));
-                }
-                if (lane == 0) {
-                    sm.k_lift[j % 8] = 21 - ek; sm.v_lift[j % 8] = 21 - ev;
-                    sm.odd[j % 8][0] = static_cast<uint32_t>(odd_slots); sm.odd[j % 8][1] = static_cast<uint32_t>(odd_slots >> 32);
-                    sm.drop[j % 8][0] = static_cast<uint32_t>(drop); sm.drop[j % 8][1] = static_cast<uint32_t>(drop >> 32);
-                    mbar_arrive(&sm.code_known[st]);
-                }
-                __syncwarp();
+                    __syncwarp();
+                };
+                if (slot0 + kTmUnit > length) look(std::true_type{}); else look(std::false_type{});
             }
         }
         __syncwarp();
@@ -469,13 +524,24 @@ tree_mma_kernel(const AttnParams p) {
                 if (stop < n) load_q(item_at(stop), item + 1);   // that buffer's last readers, the scores of the item before this one, are done
             }
             float m = -INFINITY, l = 0.f, ref = 0.f, limit = -INFINITY;
-            int lift = 64;   // of the V tiles: the accumulator is at the smallest so far
+            int lift = 64;   // of the V tiles: the row's accumulator is at the smallest so far of what it sees
             bool dead = false;
-            for (; j < stop; ++j) {
+            // One unit; EDGE: it reaches past the context. Two copies of the code, so that the units inside run past none of what only the others need
+            // (one copy: 5 % more). False: a wait has run out.
+            auto unit = [&](auto edge_tag) {
+                constexpr bool EDGE = decltype(edge_tag)::value;
                 const uint32_t buf = j & 1, turn = (j >> 1) & 1;
                 ok = tm_wait(&sm.s_full[buf], turn);
-                if (!ok) break;
+                if (!ok) return false;
                 tm_fence_after();
+                if (Q8 && EDGE && (sm.wild[j % 8] & 1)) {   // scores of raised keys
+#pragma unroll 1
+                    for (uint32_t c = 0; c < kTmUnit; ++c) {
+                        const uint32_t at = base + S::kS + buf * kTmUnit + c;
+                        tm_st1(at, __float_as_uint(__uint_as_float(tm_ld1(at)) * pow2(-static_cast<int>(sm.k_raised[j % 8][c]))));
+                    }
+                    tm_st_wait();
+                }
                 float s[2][32];
                 tm_ld32(base + S::kS + buf * kTmUnit, s[0]);
                 tm_ld32(base + S::kS + buf * kTmUnit + 32, s[1]);
@@ -486,7 +552,8 @@ tree_mma_kernel(const AttnParams p) {
                 dead |= sm.gone[j % 8] != 0;
                 const int k_lift = Q8 ? static_cast<int>(sm.k_lift[j % 8]) : 0, v_lift = Q8 ? static_cast<int>(sm.v_lift[j % 8]) : 0;
                 const float fj = Q8 ? f * pow2(-k_lift) : f;
-                if (j >= inner) {
+                int v_row = v_lift;   // the power of two that the row's accumulator has to be at: of the slots that it sees, if it sees any
+                if constexpr (EDGE) {
                     const AttnItem it = item_at(j);
                     const uint64_t slot0 = (u0 + j - it.start) * kTmUnit;
                     uint64_t word = 0;
@@ -499,6 +566,14 @@ tree_mma_kernel(const AttnParams p) {
                     const uint64_t there = it.total - slot0 >= 64 ? ~0ull : (1ull << (it.total - slot0)) - 1;
                     uint64_t seen = slot0 >= it.length ? word >> (slot0 - it.length) : (word << (it.length - slot0)) | ((1ull << (it.length - slot0)) - 1);
                     seen &= there;
+                    if (Q8 && (sm.wild[j % 8] & 2)) {
+                        uint32_t least = 64;
+#pragma unroll 1
+                        for (uint32_t c = 0; c < kTmUnit; ++c)
+                            if (seen >> c & 1) least = min(least, static_cast<uint32_t>(sm.v_raised[j % 8][c]));
+                        v_row += static_cast<int>(least);
+                    }
+                    if (Q8 && !seen) v_row = 64;
 #pragma unroll
                     for (uint32_t c = 0; c < 64; ++c) {
                         if (!(seen >> c & 1)) s[c / 32][c % 32] = -INFINITY;
@@ -510,7 +585,7 @@ tree_mma_kernel(const AttnParams p) {
                 for (uint32_t c = 0; c < 64; ++c) x4[c % 4] = fmaxf(x4[c % 4], s[c / 32][c % 32]);
                 const float x = fmaxf(fmaxf(x4[0], x4[1]), fmaxf(x4[2], x4[3])) * fj;
                 const bool fresh = j == first;
-                if (__any_sync(NONE, x > limit) || v_lift < lift) {
+                if (__any_sync(NONE, x > limit || v_row < lift)) {
                     float old = 1.f;
                     if (x > limit) {
                         old = m == -INFINITY ? 0.f : exp2_approx(m - x);
@@ -520,9 +595,9 @@ tree_mma_kernel(const AttnParams p) {
                     if (!fresh) {   // the accumulator, once the products so far are in it
                         const uint32_t last = j - 1;
                         ok = tm_wait(&sm.pv_done[last & 1], (last >> 1) & 1);
-                        if (!ok) break;
+                        if (!ok) return false;
                         tm_fence_after();
-                        if (v_lift < lift) old *= pow2(max(v_lift - lift, -120));
+                        if (v_row < lift) old *= pow2(max(v_row - lift, -120));
 #pragma unroll 1
                         for (uint32_t c = 0; c < D / 32; ++c) {
                             float o[32];
@@ -535,10 +610,10 @@ tree_mma_kernel(const AttnParams p) {
                         }
                         tm_st_wait();
                     }
-                    lift = min(lift, v_lift);
+                    lift = min(lift, v_row);
                 }
                 // V tiles at a higher power of two than the accumulator: the weights take what is between, and the sum gives it back
-                const float shift = Q8 ? max(static_cast<float>(lift - v_lift), -100.f) : 0.f;
+                const float shift = Q8 ? static_cast<float>(min(max(lift - v_lift, -100), 0)) : 0.f;   // above 0: raised slots, or none that the row sees
                 uint32_t w[32];
                 float2 sum[4] = {};
                 const float2 fj2 = make_float2(fj, fj), ref2 = make_float2(ref + shift, ref + shift);
@@ -552,14 +627,27 @@ tree_mma_kernel(const AttnParams p) {
                 sum[0] = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
                 l = fmaf(sum[0].x + sum[0].y, Q8 ? exp2_approx(-shift) : 1.f, l);
                 ok = j < 2 || tm_wait(&sm.pv_done[buf], turn ^ 1);   // PV of unit j - 2 has read this buffer
-                if (!ok) break;
+                if (!ok) return false;
                 tm_fence_after();
                 tm_st32(base + S::kP + buf * (kTmUnit / 2), w);
                 tm_st_wait();
+                if (Q8 && EDGE && (sm.wild[j % 8] & 2)) {   // weights of raised values
+                    const int above = max(lift - v_lift, 0);
+#pragma unroll 1
+                    for (uint32_t c = 0; c < kTmUnit / 2; ++c) {
+                        const uint32_t at = base + S::kP + buf * (kTmUnit / 2) + c;
+                        const float2 y = __half22float2(bits_h2(tm_ld1(at)));
+                        tm_st1(at, h2_bits(__floats2half2_rn(y.x * pow2(min(above - sm.v_raised[j % 8][2 * c], 0)), y.y * pow2(min(above - sm.v_raised[j % 8][2 * c + 1], 0)))));
+                    }
+                    tm_st_wait();
+                }
                 tm_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.p_ready[buf]);
-            }
+                return true;
+            };
+            for (; j < inner && unit(std::false_type{});) ++j;
+            for (; ok && j < stop && unit(std::true_type{});) ++j;
             if (!ok) break;
             const uint32_t last = j - 1;
             ok = tm_wait(&sm.pv_done[last & 1], (last >> 1) & 1);
