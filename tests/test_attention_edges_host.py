@@ -23,3 +23,18 @@ def test_refills_stand_behind_the_reads_of_what_they_overwrite():
     assert len(releases) == 2                               # tiles of keys, tiles of values
     for at in releases:
         assert re.search(r"fence_async_smem\(\);\s*__syncwarp\(\);\s*if \(lane == 0\) \{[^}]*$", wide[:at]), wide[at - 200:at]
+
+
+def test_norm_shuffles_are_reached_by_whole_warps():
+    """turn_rows: eight dims a lane, so that a warp holds 32 / (dim / 8) heads and may hold the last query heads beside the first key heads, of which one side may have
+    no norm. The sum of squares goes round the whole warp, so the warp decides as a whole whether it is formed."""
+    for dim in (64, 128):
+        lanes = dim // 8
+        mixed = [(hq, hk) for hq in range(1, 9) for hk in range(1, 9) if any(len({h >= hq for h in range(w, min(w + 32 // lanes, hq + hk))}) == 2
+                                                                            for w in range(0, hq + hk, 32 // lanes))]
+        assert (7, 2) in mixed                              # such calls exist
+    body = re.search(r"__device__ __forceinline__ void turn_rows\(.*?\n\}\n", source("tsp_kv.cu"), re.S).group(0)
+    before = body[:body.index("__shfl_xor_sync")]
+    branch = re.findall(r"if \((\w+)\) \{", before)[-1]
+    declared = re.search(r"const bool %s = ([^;]*);" % branch, body)
+    assert declared and declared.group(1).startswith("__any_sync(0xffffffffu, "), branch      # one answer for the warp

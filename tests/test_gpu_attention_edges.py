@@ -110,3 +110,26 @@ def test_rows_that_see_such_a_slot(dtype, group, which, value):
                 e = ((s.dim + 8) * U32 + (U16 if dtype == "f16" else 0)) * spread
                 tol = vmax * (4 * e + (4 * U16 if dtype == "f16" else (len(vis) + 64) * U32)) + (U16 * np.abs(w[0]) + 2.0 ** -25 if dtype == "f16" else 0)
                 assert (np.abs(got[r][h] - w[0]) <= tol).all(), (seq, j, h, float((np.abs(got[r][h] - w[0]) / tol).max()))
+
+
+# ---- norm and rotation
+
+def inv_freq(rotary):
+    return (1e4 ** (-np.arange(rotary // 2) / max(1, rotary // 2))).astype(np.float32)
+
+
+@pytest.mark.parametrize("dim,hq,hk", [(64, 1, 1), (64, 7, 2), (64, 3, 6), (128, 1, 1), (128, 7, 3), (256, 3, 2)])
+@pytest.mark.parametrize("sides", ["q", "k", "none", "both"])
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("rows", [1, 700])
+def test_norm_of_one_side_where_a_warp_holds_heads_of_both(dim, hq, hk, sides, dtype, rows):
+    rng = np.random.default_rng(dim + hq)
+    q, k = (rng.normal(size=(rows, h, dim)).astype(np.float32 if dtype == "f32" else np.float16) for h in (hq, hk))
+    pos, f = rng.integers(0, 9000, rows).astype(np.uint32), inv_freq(dim)
+    wq, wk = ((1 + 0.2 * rng.normal(size=dim)).astype(np.float32) if sides in (s, "both") else None for s in ("q", "k"))
+    turn = A.QkNormRope(dim, dim, "halves", dev(f), None if wq is None else dev(wq), None if wk is None else dev(wk), eps=1e-5)
+    qo, ko, err = torch.empty_like(dev(q)), torch.empty_like(dev(k)), error_word()
+    A.qk_norm_rope(turn, dev(q), dev(k), dev(pos), qo, ko, err)
+    assert int(err) == 0
+    for x, w, o in ((q, wq, qo), (k, wk, ko)):
+        check_turned(o.cpu().numpy(), R.turned(x, w, pos, f, dim, "halves", 1e-5), dtype)

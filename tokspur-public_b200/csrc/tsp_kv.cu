@@ -268,6 +268,7 @@ __device__ __forceinline__ void turn_rows(const tsp_qk_norm_rope_args& a, const 
         if (row0 + j < end) { ru[j].load(in + j * in_stride); rv[j].load(in + j * in_stride + iv); }
     const float* w = is_k ? a.d_k_norm : a.d_q_norm;
     Raw4<false> wu, wv;
+    wu.w = wv.w = make_float4(1.f, 1.f, 1.f, 1.f);
     if (w) { wu.load(reinterpret_cast<const uint8_t*>(w + xu)); wv.load(reinterpret_cast<const uint8_t*>(w + xv)); }
     if (half) {
         for (uint32_t i = tid; i < RB * half; i += blockDim.x) {
@@ -281,20 +282,21 @@ __device__ __forceinline__ void turn_rows(const tsp_qk_norm_rope_args& a, const 
         __syncthreads();
     }
     bool bad = false;
+    const bool normed = __any_sync(0xffffffffu, w != nullptr);   // a warp may hold heads of both sides, one without a norm, and all of it shuffles
     const uint32_t group = LANES == 32 ? 0xffffffffu : ((1u << (LANES % 32)) - 1) << (lane / LANES * LANES);
 #pragma unroll
     for (uint32_t j = 0; j < RB; ++j) {
         if (row0 + j >= end) break;
         float u[4], v[4];
         ru[j].to(u); rv[j].to(v);
-        if (w) {
+        if (normed) {
             float ss = 0.f, fu[4], fv[4];
             wu.to(fu); wv.to(fv);
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) ss = fmaf(u[i], u[i], fmaf(v[i], v[i], ss));
 #pragma unroll
             for (uint32_t o = LANES / 2; o; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const float inv = rsqrtf(ss * (1.f / D) + a.eps);
+            const float inv = w ? rsqrtf(ss * (1.f / D) + a.eps) : 1.f;   // a side without a norm: times one
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) { u[i] = u[i] * inv * fu[i]; v[i] = v[i] * inv * fv[i]; }
         }
