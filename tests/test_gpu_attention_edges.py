@@ -133,3 +133,46 @@ def test_norm_of_one_side_where_a_warp_holds_heads_of_both(dim, hq, hk, sides, d
     assert int(err) == 0
     for x, w, o in ((q, wq, qo), (k, wk, ko)):
         check_turned(o.cpu().numpy(), R.turned(x, w, pos, f, dim, "halves", 1e-5), dtype)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("eps", [0.0, 1e-38, 1e-6])
+@pytest.mark.parametrize("rows", [3, 600])
+def test_norms_of_heads_whose_squares_leave_fp32(dim, eps, rows):
+    """Finite heads around 1e19 and up (their squares overflow) and down to 1e-38 (they vanish); beside them heads of ordinary size, in the same warp."""
+    rng = np.random.default_rng(dim)
+    x = rng.normal(size=(rows, 7, dim))
+    at = np.array([1.0, 1e19, 1e-20, 3e37, 1e-24, 1e-37, 1e30])
+    x = (x * at[None, :, None]).astype(np.float32)
+    x[1, 2] = 0
+    x[1, 2, 5] = 1e-40                                 # one subnormal value
+    if eps == 0:
+        x[2, 4, :] = 0
+        x[2, 4, 0] = -3e38                             # one value, near the largest
+    pos, f, w = rng.integers(0, 9000, rows).astype(np.uint32), inv_freq(dim), (1 + 0.2 * rng.normal(size=dim)).astype(np.float32)
+    t, err = dev(x), error_word()
+    qo, ko = torch.empty_like(t[:, :4]), torch.empty_like(t[:, 4:])
+    A.qk_norm_rope(A.QkNormRope(dim, dim, "halves", dev(f), dev(w), dev(w), eps=eps), t[:, :4], t[:, 4:], dev(pos), qo, ko, err)
+    assert int(err) == 0
+    want = R.turned(x, w, pos, f, dim, "halves", eps)
+    got = np.concatenate([qo.cpu().numpy(), ko.cpu().numpy()], 1)
+    # 2^-19 of the head's largest value as elsewhere; 2^-149: where values themselves are subnormal
+    top = np.abs(want).max(-1, keepdims=True)
+    assert (np.abs(got.astype(np.float64) - want) <= top * 2.0 ** -19 + 2.0 ** -149).all()
+
+
+def test_the_key_in_the_cache_and_the_query_of_one_row_agree_on_large_heads():
+    """The fused call: query rows normed in FP32, the same values as keys in 64 bits on their way into the cache."""
+    dim = 128
+    x = (np.random.default_rng(8).normal(size=(5, 3, dim)) * 1e19).astype(np.float32)
+    p = R.Pages(np.random.default_rng(0), "f16", 16, 1, dim, [5])
+    cache, err = make_cache(p), error_word()
+    batch = A.KvBatch(dev(np.array([0, 5], np.uint32)), dev(np.zeros(1, np.uint32)), 5)
+    t, q = dev(x), torch.empty(5, 1, dim, device="cuda")
+    w, pos = np.ones(dim, np.float32), np.arange(5, dtype=np.uint32)
+    A.qk_norm_rope_append(A.QkNormRope(dim, dim, "halves", dev(inv_freq(dim)), dev(w), dev(w)), cache, batch, t[:, :1], t[:, :1], dev(x[:, 2:] / np.float32(1e19)), dev(pos), q, err)
+    k = torch.empty_like(q)
+    A.kv_cache_read(cache, batch, k, None, err)
+    assert int(err) == 0
+    check_turned(q.cpu().numpy(), R.turned(x[:, :1], w, pos, inv_freq(dim), dim, "halves", 1e-6), "f32")
+    check_turned(k.cpu().numpy(), R.turned(x[:, :1], w, pos, inv_freq(dim), dim, "halves", 1e-6), "f16")

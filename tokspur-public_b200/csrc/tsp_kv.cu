@@ -247,6 +247,26 @@ template <> struct Raw4<false> {
 // warp per group of 16 slots and head. Measured, 32 + 8 heads of 128 dims: 8 FP32 rows 2.1 us, the pitch of launches; 4096 binary16 rows 18 us, 84 MB at 4.6 TB/s, from
 // the L2 in part, bound by instructions (71 % of the issue slots). Into a Q8_0 cache: 38 rows of six drafts 6.6 us, a chain of latencies; 4024 rows of
 // prompts 39.5 us, bound by the 64-bit arithmetic of the keys and by instructions (67 % of the issue slots), and without norm and rotation 17.8.
+// A head whose squares overflow FP32, or vanish beside an eps that does not make up for them: the head and sqrt(eps) times a power of two that puts the larger
+// of them near one, and 1 / sqrt(mean + eps) of that. By whole warps; a group of LANES whose head needs none of it (`on` false) keeps what it has.
+template <uint32_t LANES>
+__device__ __noinline__ void scaled_norm(bool on, float eps, float (&u)[4], float (&v)[4], float& inv) {
+    float top = sqrtf(eps), ss = 0.f, x[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(u[i]), fabsf(v[i])));
+#pragma unroll
+    for (uint32_t o = LANES / 2; o; o /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const int e = max(-126, min(126, static_cast<int>(__float_as_uint(top) >> 23) - 127));
+    const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) { x[i] = (i < 4 ? u[i % 4] : v[i % 4]) * down; ss = fmaf(x[i], x[i], ss); }
+#pragma unroll
+    for (uint32_t o = LANES / 2; o; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (!on) return;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) { u[i] = x[i]; v[i] = x[i + 4]; }
+    inv = rsqrtf(ss * (1.f / (8 * LANES)) + eps * down * down);
+}
 template <uint32_t D, bool IN16, bool OUT16, uint32_t RB>
 __device__ __forceinline__ void turn_rows(const tsp_qk_norm_rope_args& a, const HeadRows& r, uint32_t pass, uint32_t row0, uint32_t end, uint32_t* error) {
     __shared__ __align__(16) float cs[RB][D / 2], sn[RB][D / 2];
@@ -296,7 +316,10 @@ __device__ __forceinline__ void turn_rows(const tsp_qk_norm_rope_args& a, const 
             for (uint32_t i = 0; i < 4; ++i) ss = fmaf(u[i], u[i], fmaf(v[i], v[i], ss));
 #pragma unroll
             for (uint32_t o = LANES / 2; o; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const float inv = w ? rsqrtf(ss * (1.f / D) + a.eps) : 1.f;   // a side without a norm: times one
+            const float mean = ss * (1.f / D) + a.eps;
+            float inv = w ? rsqrtf(mean) : 1.f;   // a side without a norm: times one
+            if constexpr (!IN16)   // squares that leave FP32, which those of binary16 rows cannot
+                if (__any_sync(0xffffffffu, w && !(mean >= 0x1p-90f && mean < INFINITY))) scaled_norm<LANES>(w && !(mean >= 0x1p-90f && mean < INFINITY), a.eps, u, v, inv);
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) { u[i] = u[i] * inv * fu[i]; v[i] = v[i] * inv * fv[i]; }
         }
