@@ -176,3 +176,15 @@ def test_the_key_in_the_cache_and_the_query_of_one_row_agree_on_large_heads():
     assert int(err) == 0
     check_turned(q.cpu().numpy(), R.turned(x[:, :1], w, pos, inv_freq(dim), dim, "halves", 1e-6), "f32")
     check_turned(k.cpu().numpy(), R.turned(x[:, :1], w, pos, inv_freq(dim), dim, "halves", 1e-6), "f16")
+
+
+@pytest.mark.parametrize("type_,dim,group", [("q8_0", 128, 4), ("f16", 64, 16), ("f16", 256, 2)])
+@pytest.mark.parametrize("scale,at", [(1e-30, 1e29), (1e-37, 1e36), (-3e-34, 1e33), (1e-30, 1.0), (4e3, 1e-5), (1e30, 1e-31)])
+def test_scales_far_from_one_with_rows_that_make_up_for_them(type_, dim, group, scale, at):
+    """FP32 rows: any finite scale, and the scores are what they are."""
+    s = Step(53, type_, dim, 16, 2, group, [5, 2], [200, 0], "f32", True)
+    s.q = (s.q * np.float32(at)).astype(np.float32)
+    s.scale = float(np.float32(scale))
+    out, err = s.run()
+    assert err == 0
+    s.check(out)

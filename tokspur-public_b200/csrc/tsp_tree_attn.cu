@@ -132,8 +132,9 @@ tree_attention_kernel(const AttnParams p) {
                 head = it.head * p.group + flat % p.group;
             };
             {
-                const float f = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-25f);   // not 0: it multiplies minus infinity
-                fa = fb = f;
+                // Not 0: it multiplies minus infinity. Sums of products of binary16 rows are below 2^47, those of FP32 rows with their power of two below 2^46: no weight
+                // shows what these floors add.
+                if constexpr (F16) fa = fb = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 0x1p-83f);
                 uint32_t node, head;
                 row_of(g, node, head);   // the fragments' row
                 const uint8_t* row = p.q + static_cast<uint64_t>(it.row0 + node) * p.q_stride + head * D * (F16 ? 2u : 4u);
@@ -160,9 +161,9 @@ tree_attention_kernel(const AttnParams p) {
                     top = fmaxf(top, __shfl_xor_sync(NONE, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(NONE, top, 2));
                     const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-                    const int shift = top > 0.f && e < 128 ? max(-115, min(40, 14 - e)) : 0;
+                    const int shift = top > 0.f && e < 128 ? max(-115, min(126, 14 - e)) : 0;
                     const float up = __uint_as_float(static_cast<uint32_t>(shift + 127) << 23) * (p.scale < 0.f ? -1.f : 1.f);
-                    const float down = f * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);   // of row g
+                    const float down = fmaxf(fabsf(p.scale) * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23) * 1.4426950408889634f, 0x1p-120f);   // of row g
                     fa = __shfl_sync(NONE, down, 8 * t); fb = __shfl_sync(NONE, down, 8 * t + 4);
 #pragma unroll
                     for (uint32_t k = 0; k < NB; ++k) {

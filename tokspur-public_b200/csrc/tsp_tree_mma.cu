@@ -483,7 +483,7 @@ tree_mma_kernel(const AttnParams p) {
         __syncthreads();
         // ---- softmax: a thread per query row
         const uint32_t quarter = warp - kTmSoftmax, r = quarter * 32 + lane, base = tmem + (quarter << 21);   // the warp's lanes of tensor memory
-        const float f = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-25f);   // not 0: it multiplies minus infinity
+        const float f = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 0x1p-83f);   // as on the warps' MMAs
         auto place = [&](const AttnItem& it, uint32_t& node, uint32_t& head) {
             const uint32_t flat = it.tile * kTmRows + r;
             node = flat / p.group;
