@@ -247,11 +247,12 @@ template <> struct Raw4<false> {
 // warp per group of 16 slots and head. Measured, 32 + 8 heads of 128 dims: 8 FP32 rows 2.1 us, the pitch of launches; 4096 binary16 rows 18 us, 84 MB at 4.6 TB/s, from
 // the L2 in part, bound by instructions (71 % of the issue slots). Into a Q8_0 cache: 38 rows of six drafts 6.6 us, a chain of latencies; 4024 rows of
 // prompts 39.5 us, bound by the 64-bit arithmetic of the keys and by instructions (67 % of the issue slots), and without norm and rotation 17.8.
-// A head whose squares overflow FP32, or vanish beside an eps that does not make up for them: the head and sqrt(eps) times a power of two that puts the larger
-// of them near one, and 1 / sqrt(mean + eps) of that. By whole warps; a group of LANES whose head needs none of it (`on` false) keeps what it has.
+// Squares of FP32 heads may leave FP32: whether the mean of a head's, with eps, says what it should
+__device__ __forceinline__ bool mean_in_range(float mean) { return __float_as_uint(mean) - 0x12800000u < 0x7f800000u - 0x12800000u; }   // [2^-90, infinity)
+// The norm of a head where it does not: the head and sqrt(eps) times a power of two that puts the larger of them near one. By whole warps.
 template <uint32_t LANES>
-__device__ __noinline__ void scaled_norm(bool on, float eps, float (&u)[4], float (&v)[4], float& inv) {
-    float top = sqrtf(eps), ss = 0.f, x[8];
+__device__ __forceinline__ void scaled_norm(float eps, float (&u)[4], float (&v)[4]) {
+    float top = sqrtf(eps), ss = 0.f;
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(u[i]), fabsf(v[i])));
 #pragma unroll
@@ -259,13 +260,12 @@ __device__ __noinline__ void scaled_norm(bool on, float eps, float (&u)[4], floa
     const int e = max(-126, min(126, static_cast<int>(__float_as_uint(top) >> 23) - 127));
     const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) { x[i] = (i < 4 ? u[i % 4] : v[i % 4]) * down; ss = fmaf(x[i], x[i], ss); }
+    for (uint32_t i = 0; i < 4; ++i) { u[i] *= down; v[i] *= down; ss = fmaf(u[i], u[i], fmaf(v[i], v[i], ss)); }
 #pragma unroll
     for (uint32_t o = LANES / 2; o; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (!on) return;
+    const float inv = rsqrtf(ss * (1.f / (8 * LANES)) + eps * down * down);
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) { u[i] = x[i]; v[i] = x[i + 4]; }
-    inv = rsqrtf(ss * (1.f / (8 * LANES)) + eps * down * down);
+    for (uint32_t i = 0; i < 4; ++i) { u[i] *= inv; v[i] *= inv; }
 }
 template <uint32_t D, bool IN16, bool OUT16, uint32_t RB>
 __device__ __forceinline__ void turn_rows(const tsp_qk_norm_rope_args& a, const HeadRows& r, uint32_t pass, uint32_t row0, uint32_t end, uint32_t* error) {
@@ -304,53 +304,79 @@ __device__ __forceinline__ void turn_rows(const tsp_qk_norm_rope_args& a, const 
     bool bad = false;
     const bool normed = __any_sync(0xffffffffu, w != nullptr);   // a warp may hold heads of both sides, one without a norm, and all of it shuffles
     const uint32_t group = LANES == 32 ? 0xffffffffu : ((1u << (LANES % 32)) - 1) << (lane / LANES * LANES);
+    float fu[4], fv[4];
+    wu.to(fu); wv.to(fv);
+    auto turn = [&](uint32_t j, float (&u)[4], float (&v)[4]) {
+        if (!turned) return;
+        const float4 c4 = *reinterpret_cast<const float4*>(cs[j] + p0), n4 = *reinterpret_cast<const float4*>(sn[j] + p0);
+        const float c[4] = {c4.x, c4.y, c4.z, c4.w}, n[4] = {n4.x, n4.y, n4.z, n4.w};
+        if (pairs) {
+            float t[4] = {u[0], u[2], v[0], v[2]}, s[4] = {u[1], u[3], v[1], v[3]};
 #pragma unroll
-    for (uint32_t j = 0; j < RB; ++j) {
-        if (row0 + j >= end) break;
-        float u[4], v[4];
-        ru[j].to(u); rv[j].to(v);
-        if (normed) {
-            float ss = 0.f, fu[4], fv[4];
-            wu.to(fu); wv.to(fv);
+            for (uint32_t i = 0; i < 4; ++i) { const float x = t[i]; t[i] = x * c[i] - s[i] * n[i]; s[i] = s[i] * c[i] + x * n[i]; }
+            u[0] = t[0]; u[1] = s[0]; u[2] = t[1]; u[3] = s[1]; v[0] = t[2]; v[1] = s[2]; v[2] = t[3]; v[3] = s[3];
+        } else {
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) ss = fmaf(u[i], u[i], fmaf(v[i], v[i], ss));
-#pragma unroll
-            for (uint32_t o = LANES / 2; o; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const float mean = ss * (1.f / D) + a.eps;
-            float inv = w ? rsqrtf(mean) : 1.f;   // a side without a norm: times one
-            if constexpr (!IN16)   // squares that leave FP32, which those of binary16 rows cannot
-                if (__any_sync(0xffffffffu, w && !(mean >= 0x1p-90f && mean < INFINITY))) scaled_norm<LANES>(w && !(mean >= 0x1p-90f && mean < INFINITY), a.eps, u, v, inv);
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) { u[i] = u[i] * inv * fu[i]; v[i] = v[i] * inv * fv[i]; }
+            for (uint32_t i = 0; i < 4; ++i) { const float x = u[i]; u[i] = x * c[i] - v[i] * n[i]; v[i] = v[i] * c[i] + x * n[i]; }
         }
-        if (turned) {
-            const float4 c4 = *reinterpret_cast<const float4*>(cs[j] + p0), n4 = *reinterpret_cast<const float4*>(sn[j] + p0);
-            const float c[4] = {c4.x, c4.y, c4.z, c4.w}, n[4] = {n4.x, n4.y, n4.z, n4.w};
-            if (pairs) {
-                float t[4] = {u[0], u[2], v[0], v[2]}, s[4] = {u[1], u[3], v[1], v[3]};
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) { const float x = t[i]; t[i] = x * c[i] - s[i] * n[i]; s[i] = s[i] * c[i] + x * n[i]; }
-                u[0] = t[0]; u[1] = s[0]; u[2] = t[1]; u[3] = s[1]; v[0] = t[2]; v[1] = s[2]; v[2] = t[3]; v[3] = s[3];
-            } else {
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) { const float x = u[i]; u[i] = x * c[i] - v[i] * n[i]; v[i] = v[i] * c[i] + x * n[i]; }
-            }
-        }
+    };
+    auto put = [&](uint32_t j, float (&u)[4], float (&v)[4], bool mine) {
         // magnitudes as integers: NaN lies above infinity
         uint32_t top = 0;
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) top = max(top, max(__float_as_uint(u[i]) & 0x7fffffffu, __float_as_uint(v[i]) & 0x7fffffffu));
         const bool ok = (__ballot_sync(0xffffffffu, top < (OUT16 ? 0x477ff000u : 0x7f800000u)) & group) == group;   // 65520 rounds to infinity in binary16
+        mine &= h0 < heads;
         if (!ok) {
-            bad |= h0 < heads;
+            bad |= mine;
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) u[i] = v[i] = 0.f;
         }
-        if (h0 < heads) {
+        if (mine) {
             store4<OUT16>(out + j * out_stride, 0, u);
             store4<OUT16>(out + j * out_stride + ov, 0, v);
         }
+    };
+    uint32_t again = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < RB; ++j) {
+        if (row0 + j >= end) break;
+        float u[4], v[4];
+        ru[j].to(u); rv[j].to(v);
+        bool odd = false;
+        if (normed) {
+            float ss = 0.f;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) ss = fmaf(u[i], u[i], fmaf(v[i], v[i], ss));
+#pragma unroll
+            for (uint32_t o = LANES / 2; o; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const float mean = ss * (1.f / D) + a.eps;
+            const float inv = w ? rsqrtf(mean) : 1.f;   // a side without a norm: times one
+            if constexpr (!IN16) odd = w && !mean_in_range(mean);
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) { u[i] = u[i] * inv * fu[i]; v[i] = v[i] * inv * fv[i]; }
+        }
+        turn(j, u, v);
+        put(j, u, v, !odd);
+        again |= static_cast<uint32_t>(odd) << j;
     }
+    // Heads whose squares leave FP32, which those of binary16 rows cannot: nothing of them has been written. (A branch beside the sums, or in front of the stores,
+    // keeps the rows from overlapping: 4096 FP32 rows of 40 heads 29 us, and 33 so.)
+    if constexpr (!IN16)
+        if (__any_sync(0xffffffffu, again != 0))
+#pragma unroll 1
+            for (uint32_t j = 0; j < RB && row0 + j < end; ++j) {
+                float u[4], v[4];
+                uint32_t row = row0 + j;
+                asm volatile("" : "+r"(row));   // the address anew: kept from the loads above it would cost the loop two registers
+                const uint8_t* from = (is_k ? r.k : r.q) + row * (is_k ? r.k_stride : r.q_stride) + (hh * D + xu) * IE;
+                load4<IN16>(from, 0, u); load4<IN16>(from + (xv - xu) * IE, 0, v);
+                scaled_norm<LANES>(a.eps, u, v);
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) { u[i] *= fu[i]; v[i] *= fv[i]; }
+                turn(j, u, v);
+                put(j, u, v, again >> j & 1);
+            }
     if (bad) raise_error(error, TSP_ERR_NONFINITE);
 }
 
@@ -364,7 +390,7 @@ turn_rows_kernel(const tsp_qk_norm_rope_args a, const HeadRows r, uint32_t passe
 
 // Grid: value blocks (a warp per group, head and `parts`-th of its dims), key blocks, then `passes` blocks for every RB query rows. A key block: RB slots of a group (a row), a warp per head.
 template <uint32_t D, bool IN16, bool OUT16, uint32_t RB>
-__global__ void __launch_bounds__(kHeadThreads)
+__global__ void __launch_bounds__(kHeadThreads, D < 256 ? 4 : 1)   // 64 registers (left alone, 76 for FP32 rows of 128 dims: 4024 rows into the cache and back 70 us, and 65)
 append_rows_kernel(const tsp_qk_norm_rope_args a, const HeadRows r, const tsp_kv_cache cache, const tsp_kv_batch batch, uint32_t values, uint32_t parts, uint32_t keys,
                    uint32_t passes, uint32_t* error) {
     __shared__ double cs[RB][D / 2], sn[RB][D / 2], exchange[kHeadThreads / 32][D];
