@@ -349,6 +349,11 @@ uint64_t tsp_tree_attention_scratch_bytes(void);
 int tsp_tree_attention(const tsp_kv_cache* cache, const tsp_kv_batch* batch, const void* d_q, uint64_t q_stride_bytes, const uint64_t* d_tree_mask,
                        uint32_t q_heads, uint32_t max_rows, float scale, void* d_out, uint64_t out_stride_bytes, uint32_t dtype, void* d_scratch,
                        uint64_t scratch_bytes, uint32_t* d_error, void* stream);
+/* What tsp_tree_attention would answer to these arguments on the current device, without a launch: for hosts that launch the step's cache write (which may turn
+ * the query rows in place) before it and want to be refused before either. */
+int tsp_tree_attention_check(const tsp_kv_cache* cache, const tsp_kv_batch* batch, const void* d_q, uint64_t q_stride_bytes, const uint64_t* d_tree_mask,
+                             uint32_t q_heads, uint32_t max_rows, float scale, const void* d_out, uint64_t out_stride_bytes, uint32_t dtype, const void* d_scratch,
+                             uint64_t scratch_bytes);
 
 /* ---- data preparation (device side) ----------------------------------------------------------------
  * tsp_synth_weights: seeded N(0, sigma) values quantised to GGUF blocks of `type` (Q4_K, Q8_0) or written

@@ -38,3 +38,19 @@ def test_norm_shuffles_are_reached_by_whole_warps():
     branch = re.findall(r"if \((\w+)\) \{", before)[-1]
     declared = re.search(r"const bool %s = ([^;]*);" % branch, body)
     assert declared and declared.group(1).startswith("__any_sync(0xffffffffu, "), branch      # one answer for the warp
+
+
+def test_the_check_answers_what_the_call_would():
+    """tsp_tree_attention_check, without a device: refusals of arguments come before anything that needs one."""
+    import ctypes as C
+    from test_attention_host import Call
+    from tokspur_public_b200 import capi
+
+    def check(c):
+        return capi.lib().tsp_tree_attention_check(C.byref(c.cache), C.byref(c.batch), c.q, c.qs, c.mask, c.q_heads, c.max_rows, c.scale, c.out, c.os, c.dtype, c.scratch,
+                                                   c.scratch_bytes)
+    for change in (dict(q_heads=33), dict(max_rows=0), dict(max_rows=65), dict(scale=float("inf")), dict(mask=(1 << 26) + 4), dict(scratch=(6 << 40) + 8), dict(scratch_bytes=0),
+                   dict(out=1 << 40), dict(out=1 << 32), dict(out=(4 << 40) + 4), dict(scratch=1 << 40), dict(scratch=4 << 40), dict(scratch=1 << 32), dict(os=16368), dict(q=None)):
+        c = Call()
+        vars(c).update(change)
+        assert check(c) == capi.E_ARG == c.attend(), change

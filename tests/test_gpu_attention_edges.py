@@ -1,5 +1,8 @@
 """The attention operators where buffers, scales and sizes meet their edges, against 64-bit restatements (attention_ref.py). Tolerances are those of
 test_gpu_attention.py, derived there."""
+import os
+import subprocess
+
 import numpy as np
 import pytest
 
@@ -188,3 +191,15 @@ def test_scales_far_from_one_with_rows_that_make_up_for_them(type_, dim, group, 
     out, err = s.run()
     assert err == 0
     s.check(out)
+
+
+# ---- the C++ host layer
+
+def test_the_host_layer_refuses_before_it_launches():
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    binary = os.path.join(root, "tokspur-public_b200", "native", "tests", "test_attention_refusals")
+    if not os.path.exists(binary):
+        subprocess.run(["make", "-s", "-C", os.path.dirname(os.path.dirname(binary))], check=True)
+    r = subprocess.run([binary], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
+    assert "attention refusal checks passed" in r.stdout

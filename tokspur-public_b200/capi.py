@@ -109,6 +109,7 @@ SIGNATURES = {
     "tsp_kv_cache_read": (_i, [_KV, _KB, _vp, _u64, _vp, _u64, _u32, _vp, _vp]),
     "tsp_kv_cache_keep": (_i, [_KV, _KB, _vp, _vp, _vp, _vp]),
     "tsp_tree_attention_scratch_bytes": (_u64, []),
+    "tsp_tree_attention_check": (_i, [_KV, _KB, _vp, _u64, _vp, _u32, _u32, C.c_float, _vp, _u64, _u32, _vp, _u64]),
     "tsp_tree_attention": (_i, [_KV, _KB, _vp, _u64, _vp, _u32, _u32, C.c_float, _vp, _u64, _u32, _vp, _u64, _vp, _vp]),
     "tsp_rows_f16_to_f32": (_i, [_vp, _u64, _vp, _u64, _u32, _u32, _vp]),
     "tsp_moe_layer_decode": (_i, [C.POINTER(MoeWeights), C.POINTER(MoeScratch), _vp, _u64, _u32, _vp, _u64, _u32, _u32, _u32,

@@ -173,4 +173,15 @@ int tsp_tree_attention(const tsp_kv_cache* cache, const tsp_kv_batch* batch, con
                                  static_cast<cudaStream_t>(stream));
 }
 
+int tsp_tree_attention_check(const tsp_kv_cache* cache, const tsp_kv_batch* batch, const void* d_q, uint64_t q_stride, const uint64_t* d_tree_mask, uint32_t q_heads,
+                             uint32_t max_rows, float scale, const void* d_out, uint64_t out_stride, uint32_t dtype, const void* d_scratch, uint64_t scratch_bytes) {
+    LaunchCount& count = launch_count();
+    const LaunchCount before = count;
+    count.dry = true;
+    const int rc = tsp_tree_attention(cache, batch, d_q, q_stride, d_tree_mask, q_heads, max_rows, scale, const_cast<void*>(d_out), out_stride, dtype,
+                                      const_cast<void*>(d_scratch), scratch_bytes, nullptr, nullptr);
+    count = before;
+    return rc;
+}
+
 }  // extern "C"

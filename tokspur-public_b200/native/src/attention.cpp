@@ -1,8 +1,6 @@
 // Encoders of the attention sub-layer: view checks, then the C ABI entries.
 #include "tokspur_b200/attention.hpp"
 
-#include <cmath>
-
 namespace tokspur_b200 {
 namespace {
 void check(int rc) { if (rc != TSP_OK) throw FormatError(tsp_last_error()); }
@@ -74,16 +72,11 @@ void encode_verify_attention(CudaGraph& g, const AttentionWeights& w, const KvCa
     const tsp_qk_norm_rope_args a{weight(g, w.q_norm, dim, "query norm"), weight(g, w.k_norm, dim, "key norm"), weight(g, w.inv_freq, w.rotary_dim / 2, "frequencies"),
                                   dim, w.rotary_dim, w.pairs ? TSP_ROPE_PAIRS : TSP_ROPE_HALVES, w.eps, w.magnitude};
     const uint32_t q_heads = q.columns / dim;
-    // shapes that the second launch would refuse are refused before the first
-    if (q_heads % cache.shape.kv_heads || q_heads / cache.shape.kv_heads > 64 || !most_rows || most_rows > TSP_KV_MAX_DRAFT || !std::isfinite(scale) ||
-        scratch.join.bytes < tsp_tree_attention_scratch_bytes())
-        throw FormatError("attention shape or scratch mismatch");
     void *qp = g.device_pointer(q.view, true), *op = g.device_pointer(out.view, true), *sp = g.device_pointer(scratch.join, true);
     const void *kp = g.device_pointer(k.view), *vp = g.device_pointer(v.view);
     const auto* words = tree.bytes ? static_cast<const uint64_t*>(g.device_pointer(tree)) : nullptr;
-    const auto span = [](const void* p, const GpuRowsF32& r) { return std::pair{reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + r.view.bytes}; };
-    const auto a0 = span(op, out), b0 = span(qp, q);
-    if (a0.first < b0.second && b0.first < a0.second) throw FormatError("attention output overlaps the query rows");
+    // what the second launch would refuse is refused before the first, which turns the query rows in place
+    check(tsp_tree_attention_check(&kc, &kb, qp, q.stride_bytes, words, q_heads, most_rows, scale, op, out.stride_bytes, 0, sp, scratch.join.bytes));
     check(tsp_qk_norm_rope_append(&a, &kc, &kb, qp, q.stride_bytes, kp, k.stride_bytes, vp, v.stride_bytes, 0, static_cast<const uint32_t*>(g.device_pointer(positions)), q_heads, qp,
                                   q.stride_bytes, 0, g.error_word(), g.stream()));
     check(tsp_tree_attention(&kc, &kb, qp, q.stride_bytes, words, q_heads, most_rows, scale, op, out.stride_bytes, 0, sp, scratch.join.bytes, g.error_word(), g.stream()));
