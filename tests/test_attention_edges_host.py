@@ -54,3 +54,23 @@ def test_the_check_answers_what_the_call_would():
         c = Call()
         vars(c).update(change)
         assert check(c) == capi.E_ARG == c.attend(), change
+
+
+def test_wide_tiles_are_left_where_their_registers_do_not_fit(tmp_path):
+    """The rule that chooses a kernel, compiled on its own: another register count of the wide kernel sends its calls to the narrow one, and refuses none."""
+    import subprocess
+    main = tmp_path / "rule.cpp"
+    main.write_text('#include <initializer_list>\n#include "tsp_tree_rule.h"\n'
+                    'using tsp::wide_tiles;\n'
+                    'int main() {\n'
+                    '    for (unsigned dim : {64u, 128u}) {\n'
+                    '        if (!wide_tiles(dim, true, 49, 128) || wide_tiles(dim, true, 48, 128) || wide_tiles(dim, false, 4096, 128)) return 1;\n'
+                    '        for (int regs : {96, 120, 126, 127, 129, 168}) if (wide_tiles(dim, true, 4096, regs)) return 2;\n'
+                    '    }\n'
+                    '    return wide_tiles(256, true, 4096, 128) ? 3 : 0;\n'
+                    '}\n')
+    subprocess.run(["g++", "-std=c++17", "-I", CSRC, "-o", str(tmp_path / "rule"), str(main)], check=True)
+    assert subprocess.run([str(tmp_path / "rule")]).returncode == 0
+    calls = source("tsp_tree_attn.cu")
+    assert re.search(r"tree_mma_registers\(p, registers\)\) return rc;\s*if \(wide_tiles\(D, f16, rows, registers\)\) return launch_tree_mma\(p, st\);", calls)
+    assert "numRegs" not in re.search(r"static int launch_tree_mma_t\(.*?\n\}\n", source("tsp_tree_mma.cu"), re.S).group(0)     # nothing refused there

@@ -30,7 +30,7 @@ def sources() -> list[str]:
 
 def _digest() -> str:
     h = hashlib.sha256()
-    for path in sources() + sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".cuh")) + \
+    for path in sources() + sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))) + \
             [os.path.join(ROOT, "include", "tsp_moe.h")]:
         with open(path, "rb") as f:
             h.update(os.path.relpath(path, ROOT).encode())

@@ -675,13 +675,16 @@ static int launch_tree_attention_t(const AttnParams& p, cudaStream_t st) {
 }
 
 int launch_tree_mma(const AttnParams&, cudaStream_t);
+int tree_mma_registers(const AttnParams&, int&);
 
 template <uint32_t D, bool Q8>
 static int launch_tree_attention_d(const AttnParams& p, bool f16, cudaStream_t st) {
-    // Tiles of 128 binary16 rows on the tensor memory's MMAs once more than six narrow tiles would read the cache: 6 sequences over 6000 slots, 48 rows a kv
-    // head 43 us (these tiles) against 41 (narrow ones), 64 rows 44 against 46; one over 8000 slots, 128 rows 34 against 48.
-    if constexpr (D < 256)
-        if (f16 && p.max_rows * p.group > 48) return launch_tree_mma(p, st);
+    const uint64_t rows = static_cast<uint64_t>(p.max_rows) * p.group;
+    if (wide_tiles(D, f16, rows, kTmLaunchRegs)) {   // if the registers of that kernel are right, that is
+        int registers;
+        if (int rc = tree_mma_registers(p, registers)) return rc;
+        if (wide_tiles(D, f16, rows, registers)) return launch_tree_mma(p, st);
+    }
     return f16 ? launch_tree_attention_t<D, Q8, true>(p, st) : launch_tree_attention_t<D, Q8, false>(p, st);
 }
 

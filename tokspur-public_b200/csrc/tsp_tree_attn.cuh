@@ -2,6 +2,7 @@
 #pragma once
 
 #include "tsp_kv.cuh"
+#include "tsp_tree_rule.h"
 
 namespace tsp {
 

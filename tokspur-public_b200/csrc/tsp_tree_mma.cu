@@ -33,8 +33,8 @@ constexpr uint32_t kTmSpread = 8;
 constexpr uint32_t kTmRows = 128, kTmUnit = 64, kTmGroups = kTmUnit / kKvGroup;
 constexpr uint32_t kTmSoftmax = 4, kTmTiles = 8, kTmTileWarps = 8, kTmThreads = 32 * (kTmTiles + kTmTileWarps);   // first softmax warp, first tile warp
 // Registers after the hand-over between the warpgroups (setmaxnreg): together no more than the count at launch times the four warpgroups, or the softmax
-// would wait for ever; the launcher checks that count. At the end all go back to that count.
-constexpr int kTmLaunchRegs = 128, kTmIssueRegs = 104, kTmSoftmaxRegs = 192, kTmTileRegs = 104;
+// would wait for ever; a kernel of another count is not launched (tsp_tree_rule.h). At the end all go back to that count.
+constexpr int kTmIssueRegs = 104, kTmSoftmaxRegs = 192, kTmTileRegs = 104;
 static_assert(kTmIssueRegs + kTmSoftmaxRegs + kTmTileWarps / 4 * kTmTileRegs <= (2 + kTmTileWarps / 4) * kTmLaunchRegs, "hand-over of registers");
 // piece of an item: references and sums of 128 rows, a flag, then the rows' dims four by four, rows side by side: [dim / 4][row][4]
 constexpr uint32_t kTmPartHead = 288;
@@ -800,19 +800,29 @@ template <uint32_t D, bool Q8>
 static int launch_tree_mma_t(const AttnParams& p, cudaStream_t st) {
     constexpr size_t smem = sizeof(TmSmem<D, Q8>) + 1024;
     static_assert(smem <= 232448, "shared memory of a block");
-    static thread_local int regs_ok = -1;
-    if (regs_ok < 0) {
-        cudaFuncAttributes fa;
-        TSP_CUDA(cudaFuncGetAttributes(&fa, tree_mma_kernel<D, Q8>));
-        regs_ok = fa.numRegs == kTmLaunchRegs;
-    }
-    if (!regs_ok) return fail(TSP_E_CUDA, "attention: the kernel's register count does not allow its hand-over");
     static thread_local SmemAttrCache attr;
     TSP_CUDA(ensure_dynamic_smem(tree_mma_kernel<D, Q8>, attr, smem));
     const int sms = sm_count();
     const uint32_t blocks = sms < 1 ? 1 : sms < static_cast<int>(kAttnMaxBlocks) ? sms : kAttnMaxBlocks;
     TSP_CUDA(launch_pdl(tree_mma_kernel<D, Q8>, dim3(blocks), dim3(kTmThreads), smem, st, p));
     return TSP_OK;
+}
+
+template <uint32_t D, bool Q8>
+static int tree_mma_registers_t(int& registers) {
+    static thread_local int known = 0;
+    if (!known) {
+        cudaFuncAttributes fa;
+        TSP_CUDA(cudaFuncGetAttributes(&fa, tree_mma_kernel<D, Q8>));
+        known = fa.numRegs;
+    }
+    registers = known;
+    return TSP_OK;
+}
+int tree_mma_registers(const AttnParams& p, int& registers) {
+    const bool q8 = p.cache.type == TSP_TYPE_Q8_0;
+    if (p.cache.head_dim == 64) return q8 ? tree_mma_registers_t<64, true>(registers) : tree_mma_registers_t<64, false>(registers);
+    return q8 ? tree_mma_registers_t<128, true>(registers) : tree_mma_registers_t<128, false>(registers);
 }
 
 int launch_tree_mma(const AttnParams& p, cudaStream_t st) {   // binary16 rows, head_dim 64 or 128
