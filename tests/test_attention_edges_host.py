@@ -2,6 +2,8 @@
 import os
 import re
 
+import pytest
+
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "tokspur-public_b200", "csrc")
 
 
@@ -74,3 +76,24 @@ def test_wide_tiles_are_left_where_their_registers_do_not_fit(tmp_path):
     calls = source("tsp_tree_attn.cu")
     assert re.search(r"tree_mma_registers\(p, registers\)\) return rc;\s*if \(wide_tiles\(D, f16, rows, registers\)\) return launch_tree_mma\(p, st\);", calls)
     assert "numRegs" not in re.search(r"static int launch_tree_mma_t\(.*?\n\}\n", source("tsp_tree_mma.cu"), re.S).group(0)     # nothing refused there
+
+
+def objects(rows=3, heads=2, dim=64):
+    """Cache, batch and rows in host memory: what is wrong with a tensor is said before anybody asks for a device."""
+    import torch
+    from tokspur_public_b200 import attention as A
+    cache = A.KvCache(torch.zeros(4, A.page_bytes("q8_0", 16, heads, dim), dtype=torch.uint8), torch.zeros(1, 4, dtype=torch.int32), 16, heads, dim, "q8_0")
+    batch = A.KvBatch(torch.tensor([0, rows], dtype=torch.int32), torch.zeros(1, dtype=torch.int32), rows)
+    return A, torch, cache, batch, torch.zeros(rows, heads, dim), torch.zeros(rows, dtype=torch.int32)
+
+
+def test_a_workspace_or_error_word_without_memory_of_its_own_is_refused():
+    """numel() of an expanded tensor says nothing of the memory behind it, and the library writes as much as it was told."""
+    A, torch, cache, batch, x, _ = objects()
+    size = 1 << 24
+    for scratch in (torch.zeros(1, dtype=torch.uint8).expand(size), torch.zeros(2 * size, dtype=torch.uint8)[::2], torch.zeros(size, dtype=torch.float32)):
+        with pytest.raises(ValueError, match="scratch"):
+            A.tree_attention(cache, batch, x, x.clone(), None, 3, 1.0, scratch, None)
+    for error in (torch.zeros(1, dtype=torch.uint8), torch.zeros(0, dtype=torch.int32), torch.zeros(1, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="error word: one int32"):
+            A.kv_cache_append(cache, batch, x, x, error)

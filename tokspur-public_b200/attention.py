@@ -57,8 +57,11 @@ def _call(name: str, device: int, error: torch.Tensor | None, *args) -> None:
     entry = _entries.get(name)
     if entry is None:
         entry = _entries[name] = getattr(capi.lib(), name)
-    if error is not None and error.get_device() != device:
-        _elsewhere("error word", error, device)
+    if error is not None:
+        if error.dtype is not torch.int32 or error.numel() < 1:
+            raise ValueError("error word: one int32")
+        if error.get_device() != device:
+            _elsewhere("error word", error, device)
     if device != _current_device():
         if device < 0:
             raise ValueError(f"{name}: tensors in host memory")
@@ -211,7 +214,6 @@ def tree_attention(cache: KvCache, batch: KvBatch, q, out, tree_mask, max_rows: 
     dt, heads, dim, rows = q.dtype, q.shape[1], cache.head_dim, batch.rows
     qp, qs = _rows("q", q, dt, heads, dim, rows, device)
     op, os = _rows("out", out, dt, heads, dim, rows, device)
-    if scratch.get_device() != device:
-        _elsewhere("scratch", scratch, device)
+    workspace = _words("scratch", scratch, torch.uint8, 1, device)   # dense: its size is what the library may write
     _call("tsp_tree_attention", device, error, cache.ref, batch.ref, qp, qs, None if tree_mask is None else _words("tree words", tree_mask, torch.int64, rows, device), heads, max_rows,
-          scale, op, os, int(dt is torch.float16), scratch.data_ptr(), scratch.numel())
+          scale, op, os, int(dt is torch.float16), workspace, scratch.numel())
