@@ -97,3 +97,18 @@ def test_a_workspace_or_error_word_without_memory_of_its_own_is_refused():
     for error in (torch.zeros(1, dtype=torch.uint8), torch.zeros(0, dtype=torch.int32), torch.zeros(1, dtype=torch.int64)):
         with pytest.raises(ValueError, match="error word: one int32"):
             A.kv_cache_append(cache, batch, x, x, error)
+
+
+def test_positions_and_rows_that_are_left_out():
+    """What the C entry accepts (no positions where nothing is rotated) goes through to it, here as far as the missing device; what it does not is a ValueError."""
+    A, torch, cache, batch, x, words = objects()
+    still, turned = A.QkNormRope(64, 0, "halves", None), A.QkNormRope(64, 64, "halves", torch.ones(32))
+    for call in (lambda: A.qk_norm_rope(still, x, None, None, x, None, None), lambda: A.qk_norm_rope_append(still, cache, batch, x, x, x, None, x, None)):
+        with pytest.raises(ValueError, match="tensors in host memory"):
+            call()
+    for call in (lambda: A.qk_norm_rope(turned, x, None, None, x, None, None), lambda: A.qk_norm_rope_append(turned, cache, batch, x, x, x, None, x, None)):
+        with pytest.raises(ValueError, match="positions: 3 dense values"):
+            call()
+    for rows in ((None, None, None, None), (x, None, None, None), (None, x, None, None), (x, x, x, None)):
+        with pytest.raises(ValueError, match="rows of queries, keys or both"):
+            A.qk_norm_rope(still, rows[0], rows[1], None, rows[2], rows[3], None)

@@ -203,3 +203,11 @@ def test_the_host_layer_refuses_before_it_launches():
     r = subprocess.run([binary], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout + r.stderr
     assert "attention refusal checks passed" in r.stdout
+
+
+def test_rows_without_rotation_need_no_positions():
+    x, w = np.random.default_rng(1).normal(size=(4, 3, 64)).astype(np.float32), np.ones(64, np.float32)
+    out, err = torch.empty(4, 3, 64, device="cuda"), error_word()
+    A.qk_norm_rope(A.QkNormRope(64, 0, "halves", None, dev(w)), dev(x), None, None, out, None, err)
+    assert int(err) == 0
+    check_turned(out.cpu().numpy(), R.turned(x, w, np.zeros(4), np.ones(1), 0, "halves", 1e-6), "f32")

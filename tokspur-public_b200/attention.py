@@ -39,7 +39,7 @@ def _rows(name: str, t: torch.Tensor, dtype: torch.dtype, heads: int, dim: int, 
 
 
 def _words(name: str, t: torch.Tensor, dtype: torch.dtype, least: int, device: int) -> int:
-    if t.dtype is not dtype or t.numel() < least or not t.is_contiguous():
+    if t is None or t.dtype is not dtype or t.numel() < least or not t.is_contiguous():
         raise ValueError(f"{name}: {least} dense values of {dtype}")
     if t.get_device() != device:
         _elsewhere(name, t, device)
@@ -62,9 +62,9 @@ def _call(name: str, device: int, error: torch.Tensor | None, *args) -> None:
             raise ValueError("error word: one int32")
         if error.get_device() != device:
             _elsewhere("error word", error, device)
+    if device < 0:
+        raise ValueError(f"{name}: tensors in host memory")
     if device != _current_device():
-        if device < 0:
-            raise ValueError(f"{name}: tensors in host memory")
         with torch.cuda.device(device):
             return _call(name, device, error, *args)
     rc = entry(*args, None if error is None else error.data_ptr(), _raw_stream(device))
@@ -144,9 +144,15 @@ def _check_turn(turn: QkNormRope, device: int):
         raise ValueError(f"norm weights and frequencies on devices {[turn.device]}, the call is for CUDA device {device}")
 
 
+def _positions(turn: QkNormRope, positions, rows: int, device: int):
+    return None if positions is None and not turn.struct.rotary_dim else _words("positions", positions, torch.int32, rows, device)
+
+
 def qk_norm_rope(turn: QkNormRope, q, k, positions, q_out, k_out, error):
-    """q / k [rows, heads, head_dim] (either may be None) -> q_out / k_out of any of the two dtypes; positions int32 [rows]."""
+    """q / k [rows, heads, head_dim] (one may be None) -> q_out / k_out of any of the two dtypes; positions int32 [rows], None where nothing is rotated."""
     x, o, dim = (q, q_out, turn.head_dim) if q is not None else (k, k_out, turn.head_dim)
+    if x is None or o is None or (q is not None and k is not None and k_out is None):
+        raise ValueError("qk_norm_rope: rows of queries, keys or both, and as many outputs")
     rows, dt, ot = x.shape[0], x.dtype, o.dtype
     device = x.get_device()
     _check_turn(turn, device)
@@ -160,7 +166,7 @@ def qk_norm_rope(turn: QkNormRope, q, k, positions, q_out, k_out, error):
         hk = k.shape[1]
         kp, ks = _rows("k", k, dt, hk, dim, rows, device)
         kop, kos = _rows("k_out", k_out, ot, hk, dim, rows, device)
-    _call("tsp_qk_norm_rope", device, error, turn.ref, qp, qs, kp, ks, int(dt is torch.float16), _words("positions", positions, torch.int32, rows, device), rows, hq, hk, qop, qos,
+    _call("tsp_qk_norm_rope", device, error, turn.ref, qp, qs, kp, ks, int(dt is torch.float16), _positions(turn, positions, rows, device), rows, hq, hk, qop, qos,
           kop, kos, int(ot is torch.float16))
 
 
@@ -182,7 +188,7 @@ def qk_norm_rope_append(turn: QkNormRope, cache: KvCache, batch: KvBatch, q, k, 
     vp, vs = _rows("v", v, dt, cache.kv_heads, dim, rows, device)
     op, os = _rows("q_out", q_out, ot, heads, dim, rows, device)
     _call("tsp_qk_norm_rope_append", device, error, turn.ref, cache.ref, batch.ref, qp, qs, kp, ks, vp, vs, int(dt is torch.float16),
-          _words("positions", positions, torch.int32, rows, device), heads, op, os, int(ot is torch.float16))
+          _positions(turn, positions, rows, device), heads, op, os, int(ot is torch.float16))
 
 
 def kv_cache_read(cache: KvCache, batch: KvBatch, k_out, v_out, error):
