@@ -112,3 +112,11 @@ def test_positions_and_rows_that_are_left_out():
     for rows in ((None, None, None, None), (x, None, None, None), (None, x, None, None), (x, x, x, None)):
         with pytest.raises(ValueError, match="rows of queries, keys or both"):
             A.qk_norm_rope(still, rows[0], rows[1], None, rows[2], rows[3], None)
+
+
+def test_a_page_table_that_is_part_of_a_wider_one_is_refused():
+    A, torch, cache, batch, x, _ = objects()
+    wide = torch.zeros(2, 8, dtype=torch.int32)
+    with pytest.raises(ValueError, match="not next to one another"):
+        A.KvCache(cache.pages, wide[:, :4], 16, 2, 64, "q8_0")
+    assert A.KvCache(cache.pages, wide[:1, :4], 16, 2, 64, "q8_0").struct.table_stride == 4      # one row of it has no next

@@ -86,9 +86,9 @@ class KvCache:
         if page_table.get_device() != self.device:
             _elsewhere("page table", page_table, self.device)
         self.pages, self.page_table, self.kv_heads, self.head_dim, self.sequences = pages, page_table, kv_heads, head_dim, page_table.shape[0]
-        # a row of the table may be part of a wider one: the stride is what the library walks by
+        # The library has one number for the words between two rows and for the pages of a sequence: columns of a wider table would pass for pages of this one
         if page_table.shape[0] > 1 and page_table.stride(0) != page_table.shape[1]:
-            raise ValueError("the page table is densely packed")
+            raise ValueError("the rows of the page table are not next to one another")
         self.struct = capi.KvCache(pages.data_ptr(), pages.stride(0), page_table.data_ptr(), page_table.shape[1], pages.shape[0], page_tokens, kv_heads,
                                    head_dim, TYPES[type_])
         self.ref = C.byref(self.struct)
