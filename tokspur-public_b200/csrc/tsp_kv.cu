@@ -108,8 +108,8 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 }
 // 16 slots of a head's values, a warp: lane (g, t) takes dims 8 i + 2 t, + 1 of slots g and g + 8, in the order of an MMA fragment, and a transposing
 // move of 8 x 8 matrices puts four slots beside each other as the cache holds them: whole 512-byte rows go out. `rows`: slots of the group that are
-// written (bit i: slot i), b0 .. b1: blocks of 32 dims that are, `at(slot)`: a slot's values. (A warp per row and head, byte by byte: 4000 rows of three prompts with 32 + 8 + 8 heads of 128
-// dims, norm and rotation 100 us, and 39.5 now.)
+// written (bit i: slot i), b0 .. b1: blocks of 32 dims that are, `at(slot)`: a slot's values. (A warp per row and head, byte by byte: 4024 rows of three prompts with 32 + 8 + 8 heads of 128
+// dims, normed, rotated, written and read back, 100 us, and 76 so; 49 with all later changes.)
 template <uint32_t D, bool IN16, typename At>
 __device__ __forceinline__ bool put_values(uint8_t* half, uint32_t rows, bool q8, uint32_t lane, uint32_t b0, uint32_t b1, At&& at) {
     const uint32_t g = lane / 4, t = lane % 4;
@@ -244,7 +244,7 @@ template <> struct Raw4<false> {
 };
 // Blocks of three kinds. Rows that go out as rows: a block takes RB rows and as many heads as its threads hold at eight dims each; the rows' values are under
 // way while the threads compute the rows' angles, one each. Keys that go into the cache: a block per four slots, a warp per head. Values that do: a
-// warp per group of 16 slots and head. Measured, 32 + 8 heads of 128 dims: 8 FP32 rows 2.1 us, the pitch of launches; 4096 binary16 rows 18 us, 84 MB at 4.6 TB/s, from
+// warp per group of 16 slots and head. Measured, 32 + 8 heads of 128 dims: 8 FP32 rows 2.1 us, the pitch of launches; 4096 binary16 rows 18 us (FP32 rows 29 among other calls), 84 MB at 4.6 TB/s, from
 // the L2 in part, bound by instructions (71 % of the issue slots). Into a Q8_0 cache: 38 rows of six drafts 6.6 us, a chain of latencies; 4024 rows of
 // prompts 39.5 us, bound by the 64-bit arithmetic of the keys and by instructions (67 % of the issue slots), and without norm and rotation 17.8.
 // Squares of FP32 heads may leave FP32: whether the mean of a head's, with eps, says what it should

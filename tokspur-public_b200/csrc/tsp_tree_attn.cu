@@ -12,12 +12,13 @@
 // piece), keeps reference, sum and accumulators in registers, and writes the rows of an item that lies within its run. Pieces of items
 // that do not (two a warp at most) meet at the end of the block, and what still is a piece there goes to the scratch, where the last block of the
 // item to arrive joins them, in order: the same bits every time. (Warps that took the units of one item in turn and met at its end: a ragged
-// batch of 64 contexts 187 us, and 128 now.)
+// batch of 64 contexts 187 us, and 128 so.) Every lane fences the asynchronous proxy between its reads of a stage and the copy that fills it again: no time in
+// these figures but 1 % of the chains of 256 dims, whose units are two stages.
 //
 // Measured, Q8_0 and binary16 rows of 32 heads over 8 kv heads of 128 dims: 64 sequences of up to 8192 slots, a token each, 128 us, 644 MB of cache at
-// 5.0 TB/s, bound by instructions (unpacking, 53 % of the issue slots) and by the ragged runs' ends; one token over 4096 slots 15.7 us, bound by a
+// 5.0 TB/s, bound by instructions (unpacking, 53 % of the issue slots) and by the ragged runs' ends; FP32 rows 139. One token over 4096 slots 15.8 us, bound by a
 // chain of latencies (table, copy, cold instructions, the join of a head's blocks). FP32 rows, 6 chains of up to 8 tokens x 8 heads over 6000 slots
-// of binary16, 256 dims: 41.5 us, bound by the instructions of the split products (640 for the 64 MMAs of a unit and tile) at eight warps an SM.
+// of binary16, 256 dims: 41.8 us, bound by the instructions of the split products (640 for the 64 MMAs of a unit and tile) at eight warps an SM.
 //
 // Codes enter the MMAs exactly (binary16 integers). The scale of a key block multiplies the FP32 partial score of its 32 dims, that of a value block the
 // FP32 weight before that is rounded to binary16: one rounding of 2^-11 on the whole path of binary16 rows. FP32 rows split the query (times a

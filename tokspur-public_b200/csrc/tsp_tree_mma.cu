@@ -9,8 +9,9 @@
 // item's end the accumulator's row; 8..11 turn codes into the MMAs' tiles of K, 12..15 into those of V. Scores, weights, query rows and tiles are double-buffered, so
 // the QK of one unit runs under the softmax of the one before and the PV of the one before that.
 //
-// Measured: a tree of 64 tokens x 32 heads over 131072 slots of 8 kv heads, Q8_0, 128 dims: 283 us (867 with tiles of eight rows on the warps' MMAs; 293 with
-// K and V tiles by the same warps), the bytes alone 44 us, the products alone 84; four trees of 32 tokens over up to 20000 slots: 66 us (115). A unit takes about
+// Measured: a tree of 64 tokens x 32 heads over 131072 slots of 8 kv heads, Q8_0, 128 dims: 281 us back to back, 315 to 320 among other calls (867 with tiles of
+// eight rows on the warps' MMAs; 293 with K and V tiles by the same warps), the bytes alone 44 us, the products alone 84; four trees of 32 tokens over up to 20000
+// slots: 69 and 73 us (115). A unit takes about
 // 2050 cycles at 1.75 GHz, 1024 of them MMAs; without the tiles' arithmetic it takes 1850, without half of the MMAs 1880, without these, the softmax's and the
 // copies 1450: no stage alone but the hand-overs between them (barrier, fence, commit) bound it.
 //
