@@ -253,7 +253,8 @@ int tsp_residual_write(const float* d_streams, const float* d_output, const floa
  * the FFN sub-layer of the same rows, for hosts that keep the whole layer on the GPU. A step's rows are described once
  * (tsp_kv_batch) and go through tsp_qk_norm_rope_append -> tsp_tree_attention; after the verify tsp_kv_cache_keep compacts the
  * accepted path. dtype arguments: 0 = FP32 rows, 1 = binary16 rows. A row holds its heads densely ([heads][head_dim]); rows are a
- * byte stride apart (a multiple of 16), so that q, k and v may be parts of one fused row. head_dim 64, 128 or 256.
+ * byte stride apart (a multiple of 16), so that q, k and v may be parts of one fused row. head_dim 64, 128 or 256. What a call writes
+ * shares no memory with its other arguments but where it says so (an array may lie between two rows).
  *
  * Paged key / value cache. Token slot i of sequence s lies in page d_page_table[s * table_stride + i / page_tokens]; pages are
  * page_stride_bytes apart (a multiple of 16, >= tsp_kv_page_bytes). Inside a page (what tsp_kv_cache_append writes and

@@ -120,3 +120,34 @@ def test_a_page_table_that_is_part_of_a_wider_one_is_refused():
     with pytest.raises(ValueError, match="not next to one another"):
         A.KvCache(cache.pages, wide[:, :4], 16, 2, 64, "q8_0")
     assert A.KvCache(cache.pages, wide[:1, :4], 16, 2, 64, "q8_0").struct.table_stride == 4      # one row of it has no next
+
+
+def test_outputs_over_the_arrays_of_the_step_are_refused():
+    """Blocks look sequences, pages and tree words up while others write: output rows, pages and workspaces lie apart from them."""
+    from test_attention_host import Call
+    from tokspur_public_b200 import capi
+    row = 32 * 128 * 4                                 # bytes of a query row
+
+    def place(entry, field, at):
+        c = Call()
+        target, _, name = field.partition("__")
+        setattr(getattr(c, target) if name else c, name or target, at)
+        return getattr(c, entry)()
+    out, pages, scratch, kout = 4 << 40, 1 << 32, 6 << 40, 5 << 40
+    step = ["batch__d_row_offsets", "batch__d_lengths", "cache__d_page_table"]
+    turn = ["positions", "turn__d_q_norm", "turn__d_k_norm", "turn__d_inv_freq"]
+    for entry, fields, written in (("norm", turn, [out, out + 31 * row, kout]), ("fused", turn + step, [out, out + 31 * row + 256, pages, pages + 15 * Call().cache.page_stride_bytes]),
+                                   ("append", step, [pages]), ("read", step, [2 << 40, 3 << 40]), ("keep", step + ["accepted", "counts"], [pages + 64]),
+                                   ("attend", step + ["mask"], [out, scratch, scratch + (1 << 30) - 16])):
+        for field in fields:
+            for at in written:
+                assert place(entry, field, at) == capi.E_ARG, (entry, field, hex(at))
+                assert "overlap" in capi.last_error()
+    # an array between two rows, or behind the last, is nobody's (without a device the call ends there)
+    import torch
+    if not torch.cuda.is_available():
+        c = Call()
+        c.os, c.batch.d_lengths, c.mask = row + 512, out + row, out + 32 * (row + 512) - 512 + 8
+        assert c.attend() == capi.E_CUDA, capi.last_error()
+        c.batch.d_lengths = out + row + 500            # reaches into the second
+        assert c.attend() == capi.E_ARG

@@ -1,5 +1,6 @@
 // C ABI of the attention operators: argument validation (refused before any launch), then the launches.
 #include <cmath>
+#include <initializer_list>
 
 #include "tsp_kv.cuh"
 
@@ -56,6 +57,25 @@ static bool meet(const Rows& a, const Rows& b, uint64_t rows) { return a.p && b.
 static uint64_t pool_bytes(const tsp_kv_cache& c) {
     return (c.pages - 1) * c.page_stride_bytes + tsp_kv_page_bytes(c.type, c.page_tokens, c.kv_heads, c.head_dim);
 }
+// Arrays that a kernel reads, some of them again and again, while its other blocks write rows or pages
+struct Array { const void* p; uint64_t bytes; };
+static bool over(const Rows& w, uint64_t rows, std::initializer_list<Array> read) {
+    for (const Array& a : read) {
+        if (!w.p || !a.p || !a.bytes || !overlap(w.p, (rows - 1) * w.stride + w.bytes, a.p, a.bytes)) continue;
+        const uintptr_t x = reinterpret_cast<uintptr_t>(w.p), y = reinterpret_cast<uintptr_t>(a.p);
+        if (y < x) return true;
+        const uint64_t in = (y - x) % w.stride;   // an array may lie between two rows
+        if (in < w.bytes || in + a.bytes > w.stride) return true;
+    }
+    return false;
+}
+static bool over_step(const Rows& w, uint64_t rows, const tsp_kv_cache& c, const tsp_kv_batch& b) {
+    return over(w, rows, {{b.d_row_offsets, (b.sequences + 1) * 4ull}, {b.d_lengths, b.sequences * 4ull}, {c.d_page_table, static_cast<uint64_t>(b.sequences) * c.table_stride * 4}});
+}
+static bool over_turn(const Rows& w, uint64_t rows, const tsp_qk_norm_rope_args& a, const uint32_t* positions, uint64_t tokens) {
+    return over(w, rows, {{positions, a.rotary_dim ? tokens * 4 : 0}, {a.d_q_norm, a.head_dim * 4ull}, {a.d_k_norm, a.head_dim * 4ull}, {a.d_inv_freq, a.rotary_dim / 2 * 4ull}});
+}
+static Rows pool(const tsp_kv_cache& c) { return {c.d_pages, c.page_stride_bytes, tsp_kv_page_bytes(c.type, c.page_tokens, c.kv_heads, c.head_dim)}; }
 static bool meets_pages(const Rows& a, const tsp_kv_cache& c, uint64_t rows) {
     return a.p && overlap(a.p, (rows - 1) * a.stride + a.bytes, c.d_pages, pool_bytes(c));
 }
@@ -93,6 +113,7 @@ int tsp_qk_norm_rope(const tsp_qk_norm_rope_args* a, const void* d_q, uint64_t q
     const bool q_in_place = qo.p == q.p && q_stride == q_out_stride && in == out, k_in_place = ko.p == k.p && k_stride == k_out_stride && in == out;
     TSP_REQUIRE((q_in_place || !meet(qo, q, rows)) && (k_in_place || !meet(ko, k, rows)) && !meet(qo, k, rows) && !meet(ko, q, rows) && !meet(qo, ko, rows),
                 "norm and rotation: output rows overlap other rows");
+    TSP_REQUIRE(!over_turn(qo, rows, *a, d_positions, rows) && !over_turn(ko, rows, *a, d_positions, rows), "norm and rotation: output rows overlap positions, weights or frequencies");
     return launch_head_rows(*a, d_q, q_stride, d_k, k_stride, nullptr, 0, in_dtype, d_positions, rows, q_heads, kv_heads, d_q_out, q_out_stride, d_k_out, k_out_stride,
                             out_dtype, nullptr, nullptr, d_error, static_cast<cudaStream_t>(stream));
 }
@@ -115,6 +136,8 @@ int tsp_qk_norm_rope_append(const tsp_qk_norm_rope_args* a, const tsp_kv_cache* 
     const bool in_place = qo.p == q.p && q_stride == q_out_stride && in == out;
     TSP_REQUIRE((in_place || !meet(qo, q, rows)) && !meet(qo, k, rows) && !meet(qo, v, rows), "norm and rotation: output rows overlap other rows");
     TSP_REQUIRE(!meets_pages(q, *cache, rows) && !meets_pages(k, *cache, rows) && !meets_pages(v, *cache, rows) && !meets_pages(qo, *cache, rows), "kv cache: rows overlap the pages");
+    TSP_REQUIRE(!over_turn(qo, rows, *a, d_positions, rows) && !over_step(qo, rows, *cache, *batch) && !over_turn(pool(*cache), cache->pages, *a, d_positions, rows) &&
+                !over_step(pool(*cache), cache->pages, *cache, *batch), "kv cache: output rows or pages overlap the arrays that describe the step");
     return launch_head_rows(*a, d_q, q_stride, d_k, k_stride, d_v, v_stride, in_dtype, d_positions, rows, q_heads, 0, d_q_out, q_out_stride, nullptr, 0, out_dtype, cache,
                             batch, d_error, static_cast<cudaStream_t>(stream));
 }
@@ -126,6 +149,7 @@ int tsp_kv_cache_append(const tsp_kv_cache* cache, const tsp_kv_batch* batch, co
     if (int rc = check_head_rows(d_v, v_stride, cache->kv_heads, cache->head_dim, dtype, "v")) return rc;
     const uint64_t bytes = static_cast<uint64_t>(cache->kv_heads) * cache->head_dim * (dtype ? 2 : 4);
     TSP_REQUIRE(!meets_pages({d_k, k_stride, bytes}, *cache, batch->rows) && !meets_pages({d_v, v_stride, bytes}, *cache, batch->rows), "kv cache: rows overlap the pages");
+    TSP_REQUIRE(!over_step(pool(*cache), cache->pages, *cache, *batch), "kv cache: the pages overlap the arrays that describe the step");
     tsp_qk_norm_rope_args a = {};
     a.head_dim = cache->head_dim;
     a.magnitude = 1.f;
@@ -142,12 +166,15 @@ int tsp_kv_cache_read(const tsp_kv_cache* cache, const tsp_kv_batch* batch, void
     const uint64_t bytes = static_cast<uint64_t>(cache->kv_heads) * cache->head_dim * (dtype ? 2 : 4);
     const Rows k{d_k, k_stride, bytes}, v{d_v, v_stride, bytes};
     TSP_REQUIRE(!meet(k, v, batch->rows) && !meets_pages(k, *cache, batch->rows) && !meets_pages(v, *cache, batch->rows), "kv cache: output rows overlap each other or the pages");
+    TSP_REQUIRE(!over_step(k, batch->rows, *cache, *batch) && !over_step(v, batch->rows, *cache, *batch), "kv cache: output rows overlap the arrays that describe the step");
     return launch_cache_read(*cache, *batch, d_k, k_stride, d_v, v_stride, dtype, d_error, static_cast<cudaStream_t>(stream));
 }
 
 int tsp_kv_cache_keep(const tsp_kv_cache* cache, const tsp_kv_batch* batch, const uint32_t* d_accepted, const uint32_t* d_counts, uint32_t* d_error, void* stream) {
     if (int rc = check_cache(cache, batch)) return rc;
     TSP_REQUIRE(d_accepted && d_counts && aligned4(d_accepted) && aligned4(d_counts), "kv cache: null or unaligned accepted indices or counts");
+    TSP_REQUIRE(!over_step(pool(*cache), cache->pages, *cache, *batch) && !over(pool(*cache), cache->pages, {{d_accepted, batch->rows * 4ull}, {d_counts, batch->sequences * 4ull}}),
+                "kv cache: the pages overlap the arrays that describe the step");
     return launch_cache_keep(*cache, *batch, d_accepted, d_counts, d_error, static_cast<cudaStream_t>(stream));
 }
 
@@ -169,6 +196,9 @@ int tsp_tree_attention(const tsp_kv_cache* cache, const tsp_kv_batch* batch, con
     TSP_REQUIRE(!meet(q, out, batch->rows) && !meets_pages(out, *cache, batch->rows), "attention: output rows overlap the query rows or the pages");
     TSP_REQUIRE(!overlap(d_scratch, scratch_bytes, d_out, (batch->rows - 1) * out_stride + bytes) && !overlap(d_scratch, scratch_bytes, d_q, (batch->rows - 1) * q_stride + bytes) &&
                 !overlap(d_scratch, scratch_bytes, cache->d_pages, pool_bytes(*cache)), "attention: scratch overlaps other buffers");
+    const Rows scratch{d_scratch, scratch_bytes, scratch_bytes};
+    TSP_REQUIRE(!over_step(out, batch->rows, *cache, *batch) && !over_step(scratch, 1, *cache, *batch) && !over(out, batch->rows, {{d_tree_mask, batch->rows * 8ull}}) &&
+                !over(scratch, 1, {{d_tree_mask, batch->rows * 8ull}}), "attention: output rows or scratch overlap the arrays that describe the step");
     return launch_tree_attention(*cache, *batch, d_q, q_stride, d_tree_mask, q_heads, max_rows, scale, d_out, out_stride, dtype, d_scratch, d_error,
                                  static_cast<cudaStream_t>(stream));
 }
